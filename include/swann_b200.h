@@ -41,6 +41,7 @@ extern "C" {
 /* element types of the corpus */
 #define SWB_F32 0
 #define SWB_F16 1
+#define SWB_BF16 2          /* the key-value cache only */
 
 /* metrics and policies (swann/_engine.py:31-36) */
 #define SWB_METRIC_IP 0     /* distance = 1 - <q, x>, rows L2-normalised */
@@ -315,6 +316,86 @@ SWB_API int swb_fill_degree(int32_t* G, int64_t n, int W, const int32_t* cand, i
 SWB_API uint64_t swb_min_in_workspace(int64_t n);
 SWB_API int swb_enforce_min_in(int32_t* G, int64_t n, int W, const int32_t* cand, int C, int min_in, int rounds,
                        void* workspace, uint64_t ws_bytes, int32_t* stats, int* rounds_run, void* stream);
+
+/* --------------------------------------- attention over a paged cache -- */
+
+/* A paged key-value cache (no counterpart in the reference).  Slot j of
+ * sequence b is row j % page_size of page table[b * table_stride + j / page_size]
+ * of the pools, whose elements are at
+ *   page * page_stride + head * head_stride + row * row_stride + dimension
+ * (strides in elements, the same for k and v, rows on 16-byte boundaries).  A
+ * page below 0 or beyond `pages` holds nothing: its slots are not attended and
+ * nothing is written to them.  page_size is a power of two; with 1 the table
+ * lists rows, so the ids of a search are a table.  lengths are device counts,
+ * and a call reads them on its stream: slots beyond them are never read. */
+typedef struct swb_kv_cache {
+    void* k;
+    void* v;
+    int64_t page_stride, head_stride, row_stride;
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* lengths;     /* [seqs] slots that each sequence holds */
+    int32_t pages, max_pages;   /* of the pools; of a row of the table */
+    int32_t page_size, seqs, kv_heads;
+    int32_t head_dim;           /* 64 or 128 */
+    int32_t dtype;              /* SWB_F16 or SWB_BF16 */
+} swb_kv_cache;
+
+/* New tokens into the cache: queries and keys normed per head (x / sqrt(mean
+ * x^2 + eps) * weight; NULL weight = no norm), their first rot_dim dimensions
+ * rotated by (cos, sin)[position] (tables [table_rows, rot_dim / 2]; pairs
+ * (i, i + rot_dim / 2), or (2i, 2i + 1) when interleaved), in 32 bits with one
+ * rounding; queries to out [tokens, q_heads, head_dim], keys and values to
+ * their slots.  Tokens of sequence b are starts[b] .. starts[b + 1] - 1 and take
+ * the last of the lengths[b] slots, which count them already.  positions
+ * [tokens], or NULL: a token's slot; one outside the tables gives NaN.
+ * slot_positions [seqs, kv_heads, slot_width] records them, or NULL. */
+SWB_API int swb_rope_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                    int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                    int64_t v_head_stride, int q_heads, const int32_t* starts, int64_t tokens,
+                    const void* q_weight, const void* k_weight, float eps, const float* cos,
+                    const float* sin, int64_t table_rows, int rot_dim, int interleaved,
+                    const int32_t* positions, const swb_kv_cache* cache, void* out,
+                    int32_t* slot_positions, int64_t slot_width, void* stream);
+
+/* Attention of each sequence's newest token: q [seqs, q_heads, head_dim] over
+ * the slots j of its sequence with window == 0, j >= length - window or
+ * j < sinks.  out [seqs, q_heads, head_dim], lse [seqs, q_heads] (natural
+ * logarithm of the sum of e^(scale <q, k>)); where nothing is seen 0 and -inf.
+ *   prior_out / prior_lse  attention over other keys, [as out / lse], joined as
+ *            one more part; NULL = none
+ *   weights  [seqs, kv_heads, weights_width]: a slot's share of the joined
+ *            softmax, summed over the query heads of its key head; written (0
+ *            where a slot is not seen), or added to when `accumulate`; NULL =
+ *            not wanted
+ *   workspace: at least swb_attn_decode_workspace(...) bytes */
+SWB_API int swb_attn_decode(const void* q, int64_t q_seq_stride, int64_t q_head_stride, int q_heads,
+                    const swb_kv_cache* cache, float scale, int window, int sinks, const void* prior_out,
+                    const float* prior_lse, void* out, float* lse, float* weights, int64_t weights_width,
+                    int accumulate, void* workspace, uint64_t ws_bytes, void* stream);
+SWB_API uint64_t swb_attn_decode_workspace(const swb_kv_cache* cache, int q_heads, int with_weights);
+
+/* Attention of many new tokens, the last of their sequences' slots (starts as
+ * in swb_rope_append, the keys written before): the token at slot i sees the
+ * slots j <= i with window == 0, j > i - window or j < sinks.
+ * q [tokens, q_heads, head_dim]; out and lse contiguous. */
+SWB_API int swb_attn_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_heads,
+                     const int32_t* starts, int64_t tokens, const swb_kv_cache* cache, float scale,
+                     int window, int sinks, void* out, float* lse, void* stream);
+
+/* Cuts every sequence to `budget` slots.  Per key head the slots stay whose
+ * position is below `sinks` or among the `recent` newest of the seen[b] given
+ * out, then those with the largest weight, ties to the lowest slot (NaN below
+ * every number).  Kept slots below the budget stay in place; kept ones beyond
+ * it go, in order, to the free slots below it, in order.  Rows move in the
+ * pools; lengths, weights and positions [seqs, kv_heads, width] are written to
+ * new buffers (0 and -1 in slots that hold nothing).
+ *   workspace: at least swb_kv_evict_workspace(...) bytes */
+SWB_API int swb_kv_evict(const swb_kv_cache* cache, const int32_t* seen, const float* weights,
+                 const int32_t* positions, int64_t width, int budget, int sinks, int recent,
+                 int32_t* new_lengths, float* new_weights, int32_t* new_positions, void* workspace,
+                 uint64_t ws_bytes, void* stream);
+SWB_API uint64_t swb_kv_evict_workspace(int seqs, int kv_heads, int budget);
 
 /* --------------------------------------------------------------- utility -- */
 

@@ -16,9 +16,17 @@ HERE = Path(__file__).resolve().parent
 LIB_PATH = HERE / "libswann_b200.so"
 
 OK, ERR_ARG, ERR_TEAM, ERR_SMEM, ERR_BATCH, ERR_CUDA, ERR_TIMEOUT = range(7)
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2
 
 _vp, _i32, _i64, _u64, _f32 = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_float
+
+
+class KVCacheArg(C.Structure):
+    """swb_kv_cache of the header."""
+    _fields_ = [("k", _vp), ("v", _vp), ("page_stride", _i64), ("head_stride", _i64), ("row_stride", _i64),
+                ("table", _vp), ("table_stride", _i64), ("lengths", _vp), ("pages", _i32), ("max_pages", _i32),
+                ("page_size", _i32), ("seqs", _i32), ("kv_heads", _i32), ("head_dim", _i32), ("dtype", _i32)]
+
 
 # name -> (restype, argtypes), exactly the declarations of include/swann_b200.h
 SIGNATURES = {
@@ -59,6 +67,14 @@ SIGNATURES = {
                             _vp, _vp, _vp, _vp, _vp, _vp]),
     "swb_reverse_tc": (_i32, [_vp, _vp, _vp, _i32, _i32, _vp, _i64, _i32, _vp, _i32, _f32, _i32, _i32, _vp, _i64,
                               _i64, _vp, _vp, _u64, _vp, _vp, _vp]),
+    "swb_rope_append": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _vp, _f32,
+                               _vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "swb_attn_decode": (_i32, [_vp, _i64, _i64, _i32, _vp, _f32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i32,
+                               _vp, _u64, _vp]),
+    "swb_attn_decode_workspace": (_u64, [_vp, _i32, _i32]),
+    "swb_attn_prefill": (_i32, [_vp, _i64, _i64, _i32, _vp, _i64, _vp, _f32, _i32, _i32, _vp, _vp, _vp]),
+    "swb_kv_evict": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _u64, _vp]),
+    "swb_kv_evict_workspace": (_u64, [_i32, _i32, _i32]),
     "swb_last_error": (C.c_char_p, []),
     "swb_version": (_i32, []),
 }
