@@ -378,10 +378,12 @@ SWB_API uint64_t swb_attn_decode_workspace(const swb_kv_cache* cache, int q_head
 /* Attention of many new tokens, the last of their sequences' slots (starts as
  * in swb_rope_append, the keys written before): the token at slot i sees the
  * slots j <= i with window == 0, j > i - window or j < sinks.
- * q [tokens, q_heads, head_dim]; out and lse contiguous. */
+ * q [tokens, q_heads, head_dim]; out and lse contiguous, out on a 16-byte boundary.
+ *   status   optional int32 device word: SWB_ERR_TIMEOUT where a bounded device-side
+ *            wait gave up (the rows concerned are NaN) */
 SWB_API int swb_attn_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_heads,
                      const int32_t* starts, int64_t tokens, const swb_kv_cache* cache, float scale,
-                     int window, int sinks, void* out, float* lse, void* stream);
+                     int window, int sinks, void* out, float* lse, int32_t* status, void* stream);
 
 /* Cuts every sequence to `budget` slots.  Per key head the slots stay whose
  * position is below `sinks` or among the `recent` newest of the seen[b] given

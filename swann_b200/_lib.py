@@ -72,7 +72,7 @@ SIGNATURES = {
     "swb_attn_decode": (_i32, [_vp, _i64, _i64, _i32, _vp, _f32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i32,
                                _vp, _u64, _vp]),
     "swb_attn_decode_workspace": (_u64, [_vp, _i32, _i32]),
-    "swb_attn_prefill": (_i32, [_vp, _i64, _i64, _i32, _vp, _i64, _vp, _f32, _i32, _i32, _vp, _vp, _vp]),
+    "swb_attn_prefill": (_i32, [_vp, _i64, _i64, _i32, _vp, _i64, _vp, _f32, _i32, _i32, _vp, _vp, _vp, _vp]),
     "swb_kv_evict": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _u64, _vp]),
     "swb_kv_evict_workspace": (_u64, [_i32, _i32, _i32]),
     "swb_last_error": (C.c_char_p, []),

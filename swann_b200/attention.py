@@ -216,7 +216,7 @@ def prefill(q, k_cache, v_cache, table, starts, lengths, *, scale=None, window=0
         rc = N.lib().swb_attn_prefill(
             N.ptr(q), q.stride(0), q.stride(1), hq, N.ptr(starts), T, C.byref(arg),
             d ** -0.5 if scale is None else float(scale), int(window), int(sinks), N.ptr(out), N.ptr(lse),
-            N.stream_of(q))
+            None, N.stream_of(q))
     N.check(rc, what)
     return out, lse
 

@@ -1,8 +1,9 @@
-// attention.cu -- attention of new tokens over a paged key-value cache.
+// attention.cu -- attention of one new token a sequence over a paged key-value
+// cache.
 //
-// For a query row at slot i of its sequence, over the slots j it sees (j <= i
-// and, with a window w, j > i - w or j < sinks; slots whose page the table
-// does not name are not seen):
+// For a query row of the token at slot i = length - 1, over the slots j it sees
+// (j <= i and, with a window w, j > i - w or j < sinks; slots whose page the
+// table does not name are not seen):
 //   x_j = scale <q, k_j>,  lse = log sum_j e^x_j,  out = sum_j e^(x_j - lse) v_j
 // in one pass over K and V, with the running maximum m and sum l of a softmax
 // in base 2:  m' = max(m, x), l' = l 2^(m - m') + 2^(x - m'), and the
@@ -33,15 +34,13 @@ constexpr int STAGES = 3;
 struct Walk {
     Cache c;
     const void* q;
-    int64_t q_token_stride, q_head_stride;
-    const int32_t* starts;    // [seqs + 1] first token of each sequence; null: one token a sequence
-    int64_t tokens;
+    int64_t q_seq_stride, q_head_stride;
     int q_heads, group;       // query heads; of them per key head
-    int head_tiles, tile_heads, tile_tokens;
+    int head_tiles, tile_heads;
     int splits;
     float scale2;             // scale * log2(e)
     int window, sinks;
-    const void* prior_out;    // [tokens, q_heads, D] and [tokens, q_heads]; null: none
+    const void* prior_out;    // [seqs, q_heads, D] and [seqs, q_heads]; null: none
     const float* prior_lse;
     void* out;
     float* lse;
@@ -50,16 +49,16 @@ struct Walk {
     float* logits;            // [seqs * q_heads][capacity], for the weights; null: not wanted
 };
 
-// the slots a tile of tokens at slots pos_lo..pos_hi can see, as one range of
-// virtual places: the first tokens, then everything from `lo` on
+// the slots that the token at slot `pos` can see, as one range of virtual
+// places: the first tokens, then everything from `lo` on
 struct Range {
     int first, lo, n;
     __device__ __forceinline__ int slot(int u) const { return u < first ? u : lo + (u - first); }
 };
-__device__ __forceinline__ Range visible(int pos_lo, int pos_hi, int window, int sinks, int64_t capacity) {
+__device__ __forceinline__ Range visible(int pos, int window, int sinks, int64_t capacity) {
     Range r;
-    const int end = (int)min((int64_t)pos_hi + 1, capacity);     // nothing is held beyond the table
-    r.lo = window > 0 ? min(max(0, pos_lo - window + 1), max(0, end)) : 0;
+    const int end = (int)min((int64_t)pos + 1, capacity);     // nothing is held beyond the table
+    r.lo = window > 0 ? min(max(0, pos - window + 1), max(0, end)) : 0;
     r.first = min(sinks, r.lo);
     r.n = max(0, r.first + end - r.lo);
     return r;
@@ -80,39 +79,16 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const __grid_constant__ W
     __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    // -- which tokens, heads and stretch
+    // -- which sequence, heads and stretch
     int64_t item = blockIdx.x;
     const int split = (int)(item % P.splits);
     item /= P.splits;
     const int ht = (int)(item % P.head_tiles);
     item /= P.head_tiles;
-    const int g = (int)(item % P.c.kv_heads);
-    item /= P.c.kv_heads;
-    int b, tok0 = 0, ntok = 1;
-    int64_t token0;
-    if (P.starts) {
-        // tile `item` of the sequences' tiles laid end to end
-        int64_t left = item;
-        for (b = 0; b < P.c.seqs; ++b) {
-            const int n = clamp_start(P.starts, b + 1, P.tokens) - clamp_start(P.starts, b, P.tokens);
-            const int tiles = n > 0 ? (n + P.tile_tokens - 1) / P.tile_tokens : 0;
-            if (left < tiles) break;
-            left -= tiles;
-        }
-        if (b >= P.c.seqs) return;
-        tok0 = (int)left * P.tile_tokens;
-        token0 = clamp_start(P.starts, b, P.tokens);
-        ntok = (int)(clamp_start(P.starts, b + 1, P.tokens) - token0);
-    } else {
-        b = (int)item;
-        token0 = b;
-    }
+    const int g = (int)(item % P.c.kv_heads), b = (int)(item / P.c.kv_heads);
     const int heads = min(P.tile_heads, P.group - ht * P.tile_heads);
-    const int head0 = g * P.group + ht * P.tile_heads;
-    const int L = P.c.lengths[b];
-    const int live = min(P.tile_tokens, ntok - tok0);            // tokens of this tile
-    const int pos0 = L - ntok + tok0;                            // slot of its first token
-    const Range rg = visible(pos0, pos0 + live - 1, P.window, P.sinks, P.c.capacity());
+    const int64_t row0 = (int64_t)b * P.q_heads + g * P.group + ht * P.tile_heads;   // first output row
+    const Range rg = visible(P.c.lengths[b] - 1, P.window, P.sinks, P.c.capacity());
 
     // this CTA's stretch: a whole number of blocks for every warp
     const int per = ((rg.n + P.splits - 1) / P.splits + WARPS * KEYS - 1) / (WARPS * KEYS) * (WARPS * KEYS);
@@ -120,13 +96,12 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const __grid_constant__ W
     const int nblk = (u1 - u0 + KEYS - 1) / KEYS;                // blocks of the stretch; warp w has w, w + WARPS, ..
     const int mine = nblk > warp ? (nblk - warp - 1) / WARPS + 1 : 0;
 
-    // -- the query rows as matrix fragments: row r is token r / heads, head r % heads
-    const T* q = static_cast<const T*>(P.q);
+    // -- the query rows as matrix fragments: row r is head r of the tile
+    const T* q = static_cast<const T*>(P.q) + b * P.q_seq_stride + (int64_t)(g * P.group + ht * P.tile_heads) * P.q_head_stride;
     const int r0 = lane >> 2, r1 = r0 + 8;
-    const int t0 = r0 / heads, t1 = r1 / heads;
-    const bool ok0 = t0 < live, ok1 = t1 < live;
-    const T* q0 = q + (token0 + tok0 + t0) * P.q_token_stride + (int64_t)(head0 + r0 % heads) * P.q_head_stride;
-    const T* q1 = q + (token0 + tok0 + t1) * P.q_token_stride + (int64_t)(head0 + r1 % heads) * P.q_head_stride;
+    const bool ok0 = r0 < heads, ok1 = r1 < heads;
+    const T* q0 = q + r0 * P.q_head_stride;
+    const T* q1 = q + r1 * P.q_head_stride;
     uint32_t qf[D / 16][4];
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
@@ -136,9 +111,8 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const __grid_constant__ W
         qf[kk][2] = ok0 ? *reinterpret_cast<const uint32_t*>(q0 + c + 8) : 0u;
         qf[kk][3] = ok1 ? *reinterpret_cast<const uint32_t*>(q1 + c + 8) : 0u;
     }
-    const int p0 = ok0 ? pos0 + t0 : -1, p1 = ok1 ? pos0 + t1 : -1;   // the rows' own slots
-    float* lg0 = P.logits && ok0 ? P.logits + ((token0 + tok0 + t0) * P.q_heads + head0 + r0 % heads) * P.c.capacity() : nullptr;
-    float* lg1 = P.logits && ok1 ? P.logits + ((token0 + tok0 + t1) * P.q_heads + head0 + r1 % heads) * P.c.capacity() : nullptr;
+    float* lg0 = P.logits && ok0 ? P.logits + (row0 + r0) * P.c.capacity() : nullptr;
+    float* lg1 = P.logits && ok1 ? P.logits + (row0 + r1) * P.c.capacity() : nullptr;
 
     const T* kp = static_cast<const T*>(P.c.k) + (int64_t)g * P.c.head_stride;
     const T* vp = static_cast<const T*>(P.c.v) + (int64_t)g * P.c.head_stride;
@@ -203,13 +177,9 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const __grid_constant__ W
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int kx = n * 8 + (lane & 3) * 2 + (e & 1);
-                const int slot = rg.slot(ub + kx);
-                const int p = e < 2 ? p0 : p1;
-                const bool see = ((seen >> kx) & 1u) && slot <= p &&
-                                 (P.window <= 0 || slot > p - P.window || slot < P.sinks);
-                x[n][e] = see ? x[n][e] * P.scale2 : NEG_INF;
+                x[n][e] = (seen >> kx) & 1u ? x[n][e] * P.scale2 : NEG_INF;
                 float* lg = e < 2 ? lg0 : lg1;
-                if (lg && ub + kx < u1) lg[slot] = x[n][e];
+                if (lg && ub + kx < u1) lg[rg.slot(ub + kx)] = x[n][e];
             }
         float a0 = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
         float a1 = fmaxf(fmaxf(x[0][2], x[0][3]), fmaxf(x[1][2], x[1][3]));
@@ -287,15 +257,14 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const __grid_constant__ W
     constexpr int TPR = THREADS / ROWS;                // threads of a row
     constexpr int DPT = D / TPR;                       // dimensions of a thread
     const int r = threadIdx.x / TPR, d0 = (threadIdx.x % TPR) * 2;
-    const int t = r / heads;
-    if (t >= live) return;
+    if (r >= heads) return;
     float M = NEG_INF, l = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w][r]);
 #pragma unroll
     for (int w = 0; w < WARPS; ++w)
         if (s_l[w][r] != 0.f) l += s_l[w][r] * exp2_fast(s_m[w][r] - M);
-    const int64_t row = (token0 + tok0 + t) * P.q_heads + head0 + r % heads;
+    const int64_t row = row0 + r;
     float2 acc[DPT / 2];
 #pragma unroll
     for (int i = 0; i < DPT / 2; ++i) {
@@ -490,27 +459,17 @@ inline int run_join(const Join& j, int64_t blocks, int dtype, int d, cudaStream_
     return d == 64 ? launch_join<__nv_bfloat16, 64>(j, blocks, st) : launch_join<__nv_bfloat16, 128>(j, blocks, st);
 }
 
-inline int check_query(const void* q, int64_t ts, int64_t hs, int q_heads, const Cache& c) {
-    if (!q) return abi::fail(SWB_ERR_ARG, "null queries");
-    if (q_heads < 1 || q_heads % c.kv_heads)
-        return abi::fail(SWB_ERR_ARG, "query heads must be a multiple of the cache's key heads");
-    if (reinterpret_cast<uintptr_t>(q) % 16 || ts % 8 || hs % 8)
-        return abi::fail(SWB_ERR_ARG, "query rows must start on 16-byte boundaries");
-    return SWB_OK;
-}
-
 inline Walk make_walk(const Cache& c, const void* q, int64_t ts, int64_t hs, int q_heads, float scale, int window,
                       int sinks) {
     Walk w = {};
     w.c = c;
     w.q = q;
-    w.q_token_stride = ts;
+    w.q_seq_stride = ts;
     w.q_head_stride = hs;
     w.q_heads = q_heads;
     w.group = q_heads / c.kv_heads;
     w.tile_heads = w.group < ROWS ? w.group : ROWS;
     w.head_tiles = (w.group + w.tile_heads - 1) / w.tile_heads;
-    w.tile_tokens = 1;
     w.splits = 1;
     w.scale2 = scale * LOG2E;
     w.window = window;
@@ -602,28 +561,4 @@ extern "C" int swb_attn_decode(const void* q, int64_t q_seq_stride, int64_t q_he
     const int64_t blocks = j.rows + (weights ? (int64_t)c.seqs * c.kv_heads * j.chunks : 0);
     if (blocks >= ((int64_t)1 << 31)) return abi::fail(SWB_ERR_ARG, "too many sequences in one call");
     return run_join(j, blocks, cache->dtype, d, st);
-}
-
-extern "C" int swb_attn_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_heads,
-                                const int32_t* starts, int64_t tokens, const swb_kv_cache* cache, float scale,
-                                int window, int sinks, void* out, float* lse, void* stream) {
-    Cache c;
-    int rc = check_cache(cache, &c);
-    if (rc) return rc;
-    if (c.seqs == 0 || tokens <= 0) return SWB_OK;
-    rc = check_query(q, q_token_stride, q_head_stride, q_heads, c);
-    if (rc) return rc;
-    if (!starts || !out || !lse) return abi::fail(SWB_ERR_ARG, "null buffer");
-    if (window < 0 || sinks < 0) return abi::fail(SWB_ERR_ARG, "window and sinks must not be negative");
-    Walk w = make_walk(c, q, q_token_stride, q_head_stride, q_heads, scale, window, sinks);
-    w.starts = starts;
-    w.tokens = tokens;
-    w.tile_tokens = ROWS / w.tile_heads;
-    w.out = out;
-    w.lse = lse;
-    // every sequence may end in a tile that is not full
-    const int64_t tiles = (tokens + w.tile_tokens - 1) / w.tile_tokens + c.seqs;
-    const int64_t items = tiles * c.kv_heads * w.head_tiles;
-    if (items >= ((int64_t)1 << 31)) return abi::fail(SWB_ERR_ARG, "too many tokens in one call");
-    return run_walk(w, items, cache->dtype, cache->head_dim, (cudaStream_t)stream);
 }

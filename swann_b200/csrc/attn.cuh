@@ -151,6 +151,15 @@ inline int check_cache(const swb_kv_cache* c, Cache* out) {
     return SWB_OK;
 }
 
+inline int check_query(const void* q, int64_t ts, int64_t hs, int q_heads, const Cache& c) {
+    if (!q) return abi::fail(SWB_ERR_ARG, "null queries");
+    if (q_heads < 1 || q_heads % c.kv_heads)
+        return abi::fail(SWB_ERR_ARG, "query heads must be a multiple of the cache's key heads");
+    if (reinterpret_cast<uintptr_t>(q) % 16 || ts % 8 || hs % 8)
+        return abi::fail(SWB_ERR_ARG, "query rows must start on 16-byte boundaries");
+    return SWB_OK;
+}
+
 // Launches a kernel that may begin while the one before it in the stream ends:
 // the kernel itself waits (dependency_wait) before it reads what that wrote.
 template <typename... P, typename... A>

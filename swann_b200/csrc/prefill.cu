@@ -1,0 +1,612 @@
+// prefill.cu -- attention of many new tokens over a paged cache, on the
+// 5th-generation tensor cores.
+//
+// The definition is attention.cu's, for tokens at the last slots of their
+// sequences.  Two products a block of keys, 4 d flops a visible pair, decide the
+// time; the exponentials come next (one a pair against 16 a cycle and SM), so the
+// layout below keeps the tensor pipe on one tile while another's softmax runs.
+//
+// A CTA owns two tiles of 128 query rows that share a key head: row r of a tile is
+// token r / heads, head r % heads, so the heads of a group read each block of keys
+// once.  It walks the blocks of 128 keys that any of its rows sees:
+//   warps 8..11   producers: K and V rows by cp.async into a ring of 128-byte
+//                 swizzled tiles, one row address a lane.  Rows that no page holds
+//                 or that lie past the end are filled with zeros, so what is in
+//                 memory there reaches no product;
+//   warp 12       issues tcgen05.mma: S = Q K^T (both K-major) into the tile's 128
+//                 TMEM columns, O += P V with P read from TMEM and V as it lies
+//                 (MN-major);
+//   warps 0..3 and 4..7  softmax of tile 0 and 1: a thread is a row.  It reads S
+//                 twice (maximum, then weights: holding 128 values a thread would
+//                 not leave registers for two tiles), writes the weights, rounded
+//                 to the cache's 16 bits, over the S it has read, and keeps the
+//                 row's sum in 32 bits, before that rounding.
+// The running maximum that the exponentials are taken against is only raised when
+// a row's maximum has passed it by 2^8 (weights stay below 2^8 and sums in range);
+// only then is O rescaled in TMEM, which the first blocks of a row need and later
+// ones hardly ever do.
+//
+// MMAs of one thread run in order, so S of the next block may be issued right
+// after the product that reads the weights lying in the same columns.  All waits
+// are bounded; if one runs out the CTA's rows are NaN and the status word is set.
+
+#include "attn.cuh"
+#include "tcgen05.cuh"
+
+namespace swb {
+namespace attn {
+namespace pre {
+
+constexpr int TILE = 128;                   // rows of a query tile, keys of a block
+constexpr int THREADS = 512;
+constexpr int PRODUCER0 = 256, PRODUCERS = 128;
+constexpr int MMA_WARP = 12;
+constexpr int LAG = 2;                      // copies of a producer in flight behind the one being issued
+constexpr float RAISE = 8.f;                // log2 of how far a maximum may pass the one in use
+
+struct Prefill {
+    Cache c;
+    const void* q;
+    int64_t q_token_stride, q_head_stride;
+    const int32_t* starts;
+    int64_t tokens;
+    int q_heads, group, head_tiles, tile_heads, tile_tokens;
+    float scale2;               // |scale| * log2(e)
+    int flip;                   // scale below 0: the queries' signs are turned instead
+    int window, sinks;
+    void* out;
+    float* lse;
+    int32_t* status;
+};
+
+template <int D>
+struct Layout {
+    static constexpr int ROWB = TILE * 128;                     // a 64-dimension panel of a tile
+    static constexpr int TILEB = TILE * D * 2;
+    static constexpr int SLOTS = D == 128 ? 4 : 8;
+    static constexpr int Q = 0;                                 // two tiles
+    static constexpr int RING = 2 * TILEB;
+    static constexpr int BARS = RING + SLOTS * TILEB;           // full, empty, q, s[2], p[2], o[2]
+    static constexpr int SEEN = BARS + (2 * SLOTS + 7) * 8;     // uint32 [8][4]
+    static constexpr int TOTAL = SEEN + 8 * 4 * 4;
+};
+
+// chunk c (16 bytes) of row r of a tile made of 64-dimension panels
+__device__ __forceinline__ uint32_t place(int r, int c) {
+    return (uint32_t)((c >> 3) * (TILE * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+// V as the second operand: 64 dimensions x 8 keys in 1024 bytes, the next 8 keys
+// 1024 bytes on, the next 64 dimensions a panel on
+__device__ __forceinline__ uint64_t desc_v(uint32_t a) {
+    return ((uint64_t)(a >> 4) & 0x3FFFull) | ((uint64_t)(TILE * 128 / 16) << 16) | (64ull << 32) | (1ull << 46) |
+           (2ull << 61);
+}
+__device__ __forceinline__ uint64_t desc_k(uint32_t a) {
+    return ((uint64_t)(a >> 4) & 0x3FFFull) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+
+template <typename T>
+struct Format;
+template <>
+struct Format<__half> {
+    static constexpr uint32_t F = 0;
+};
+template <>
+struct Format<__nv_bfloat16> {
+    static constexpr uint32_t F = 1;
+};
+template <typename T>
+__host__ __device__ constexpr uint32_t instr(int n, bool b_mn_major) {
+    return (1u << 4) | (Format<T>::F << 7) | (Format<T>::F << 10) | (uint32_t(b_mn_major) << 16) |
+           (uint32_t(n >> 3) << 17) | (uint32_t(TILE >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+
+// 32 columns of this thread's TMEM lane; the values are there after tmem_arrived
+__device__ __forceinline__ void tmem_get32(uint32_t a, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(a)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_arrived(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_put32(uint32_t a, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+        "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+        "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(a)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_put16(uint32_t a, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(a)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// the low x bits of a word
+__device__ __forceinline__ uint32_t low_bits(int x) { return x >= 32 ? 0xffffffffu : x <= 0 ? 0u : (1u << x) - 1u; }
+
+// What the CTA's roles agree on.  A block's keys have virtual places u: the first
+// tokens, then everything from slot `lo` on.
+struct Job {
+    int b, g, head0, heads;
+    int64_t token0;             // of the batch: first token of tile 0
+    int pos0;                   // its slot
+    int live;                   // tokens of the CTA that exist
+    int first, lo, n, blocks;
+    __device__ __forceinline__ int slot(int u) const { return u < first ? u : lo + (u - first); }
+};
+
+__device__ __forceinline__ bool find_job(const Prefill& P, Job& J) {
+    const int lane = threadIdx.x & 31;
+    int64_t item = blockIdx.x;
+    const int ht = (int)(item % P.head_tiles);
+    item /= P.head_tiles;
+    J.g = (int)(item % P.c.kv_heads);
+    int64_t left = item / P.c.kv_heads;
+    const int step = 2 * P.tile_tokens;
+    // the sequences' tiles end to end, 32 sequences at a time
+    int b = -1, tiles = 0;
+    for (int b0 = 0; b0 < P.c.seqs; b0 += 32) {
+        const int mine = b0 + lane;
+        int t = 0;
+        if (mine < P.c.seqs) {
+            const int64_t n = clamp_start(P.starts, mine + 1, P.tokens) - clamp_start(P.starts, mine, P.tokens);
+            t = n > 0 ? (int)((n + step - 1) / step) : 0;
+        }
+        int sum = t;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const int y = __shfl_up_sync(FULL, sum, s);
+            if (lane >= s) sum += y;
+        }
+        const unsigned hit = __ballot_sync(FULL, left < sum);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            b = b0 + src;
+            tiles = __shfl_sync(FULL, t, src);
+            left -= __shfl_sync(FULL, sum, src) - tiles;
+            break;
+        }
+        left -= __shfl_sync(FULL, sum, 31);
+    }
+    if (b < 0) return false;
+    const int64_t s0 = clamp_start(P.starts, b, P.tokens);
+    const int ntok = (int)(clamp_start(P.starts, b + 1, P.tokens) - s0);
+    const int tile = tiles - 1 - (int)left;          // the longest rows first
+    J.b = b;
+    J.heads = min(P.tile_heads, P.group - ht * P.tile_heads);
+    J.head0 = J.g * P.group + ht * P.tile_heads;
+    J.token0 = s0 + (int64_t)tile * step;
+    J.live = min(step, ntok - tile * step);
+    J.pos0 = P.c.lengths[b] - ntok + tile * step;
+    const int end = (int)max((int64_t)0, min((int64_t)J.pos0 + J.live, P.c.capacity()));
+    J.lo = P.window > 0 ? min(max(0, J.pos0 - P.window + 1), end) : 0;
+    J.first = min(P.sinks, J.lo);
+    J.n = J.first + end - J.lo;
+    J.blocks = (J.n + TILE - 1) / TILE;
+    return true;
+}
+
+// the blocks a..z-1 that tile t's rows see (a is 0 or 1: its tokens begin at most
+// 128 slots after the CTA's first)
+struct Span {
+    int tokens, pos, a, z;
+};
+__device__ __forceinline__ Span span_of(const Prefill& P, const Job& J, int t) {
+    Span s;
+    s.tokens = max(0, min(P.tile_tokens, J.live - t * P.tile_tokens));
+    s.pos = J.pos0 + t * P.tile_tokens;
+    s.a = s.z = 0;
+    if (s.tokens == 0) return s;
+    const int ub = min(J.n, J.first + s.pos + s.tokens - J.lo);       // end of what its last token sees
+    s.z = (max(0, ub) + TILE - 1) / TILE;
+    if (P.window > 0 && P.sinks == 0 && s.z > 1 && J.slot(TILE - 1) <= s.pos - P.window) s.a = 1;
+    return s;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_constant__ Prefill P) {
+    using Ly = Layout<D>;
+    constexpr int SLOTS = Ly::SLOTS;
+    constexpr int CH = D / 8;
+    extern __shared__ __align__(1024) char sm[];
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm + Ly::BARS);
+    uint64_t* empty = full + SLOTS;
+    uint64_t* qbar = empty + SLOTS;
+    uint64_t* sbar = qbar + 1;
+    uint64_t* pbar = sbar + 2;
+    uint64_t* obar = pbar + 2;
+    volatile uint32_t* s_seen = reinterpret_cast<volatile uint32_t*>(sm + Ly::SEEN);
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort_store;
+    volatile int* s_abort = &s_abort_store;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    Job J;
+    if (!find_job(P, J)) return;
+    const Span sp[2] = {span_of(P, J, 0), span_of(P, J, 1)};
+
+    if (threadIdx.x == 0) {
+        *s_abort = (smem_u32(sm) & 1023u) ? 2 : 0;
+        for (int s = 0; s < SLOTS; ++s) {
+            mbar_init(&full[s], PRODUCERS);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(qbar, PRODUCERS);
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&sbar[t], 2);       // the product's commit and the issuing thread
+            mbar_init(&pbar[t], TILE);
+            mbar_init(&obar[t], 1);
+        }
+        fence_mbar_init();
+    }
+    if (warp == MMA_WARP) {
+        tmem_alloc(&s_tmem, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    const uint32_t base = smem_u32(sm);
+
+    if (warp >= PRODUCER0 / 32 && warp < MMA_WARP) {
+        // ---------------- producers
+        const int w = warp - PRODUCER0 / 32;
+        const T* q = static_cast<const T*>(P.q);
+        for (int t = 0; t < 2; ++t) {
+            const int r = w * 32 + lane, tok = r / J.heads;
+            const bool real = tok < sp[t].tokens;
+            const int64_t off = real ? (J.token0 + t * P.tile_tokens + tok) * P.q_token_stride +
+                                           (int64_t)(J.head0 + r % J.heads) * P.q_head_stride
+                                     : -1;
+#pragma unroll
+            for (int it = 0; it < CH; ++it) {
+                const int rr = (it * 32 + lane) / CH, c = (it * 32 + lane) % CH;
+                const int64_t o = __shfl_sync(FULL, (long long)off, rr);
+                cp_async16_or_zero(base + Ly::Q + t * Ly::TILEB + place(w * 32 + rr, c), q + (o >= 0 ? o + c * 8 : 0), o >= 0);
+            }
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        if (P.flip) {
+            // each thread turns the chunks that it copied itself
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int it = 0; it < CH; ++it) {
+                    const int rr = (it * 32 + lane) / CH, c = (it * 32 + lane) % CH;
+                    uint4* p = reinterpret_cast<uint4*>(sm + Ly::Q + t * Ly::TILEB + place(w * 32 + rr, c));
+                    uint4 x = *p;
+                    x.x ^= 0x80008000u;
+                    x.y ^= 0x80008000u;
+                    x.z ^= 0x80008000u;
+                    x.w ^= 0x80008000u;
+                    *p = x;
+                }
+        }
+        fence_async_smem();
+        mbar_arrive(qbar);
+
+        const T* kp = static_cast<const T*>(P.c.k) + (int64_t)J.g * P.c.head_stride;
+        const T* vp = static_cast<const T*>(P.c.v) + (int64_t)J.g * P.c.head_stride;
+        const int total = 2 * J.blocks;
+        int64_t off = -1;
+        int idx = 0;
+        for (; idx < total && !*s_abort; ++idx) {
+            const int slot = idx % SLOTS;
+            if ((idx & 1) == 0) {
+                const int u = (idx >> 1) * TILE + w * 32 + lane;
+                off = u < J.n ? P.c.row(J.b, J.slot(u)) : -1;
+                const unsigned seen = __ballot_sync(FULL, off >= 0);
+                if (lane == 0) s_seen[((idx >> 1) & 7) * 4 + w] = seen;
+            }
+            if (!mbar_wait(&empty[slot], ((idx / SLOTS) & 1) ^ 1)) {
+                *s_abort = 1;
+                break;
+            }
+            const T* src = (idx & 1) ? vp : kp;
+            const uint32_t dst = base + Ly::RING + slot * Ly::TILEB;
+#pragma unroll
+            for (int it = 0; it < CH; ++it) {
+                const int rr = (it * 32 + lane) / CH, c = (it * 32 + lane) % CH;
+                const int64_t o = __shfl_sync(FULL, (long long)off, rr);
+                cp_async16_or_zero(dst + place(w * 32 + rr, c), src + (o >= 0 ? o + c * 8 : 0), o >= 0);
+            }
+            cp_async_commit();
+            if (idx >= LAG) {
+                cp_async_wait<LAG>();
+                fence_async_smem();
+                mbar_arrive(&full[(idx - LAG) % SLOTS]);
+            }
+            __syncwarp();
+        }
+        cp_async_wait<0>();
+        fence_async_smem();
+        for (int i = max(0, idx - LAG); i < idx; ++i) mbar_arrive(&full[i % SLOTS]);
+    } else if (warp == MMA_WARP) {
+        // ---------------- MMA issuer
+        if (lane == 0) {
+            constexpr uint32_t IS = instr<T>(TILE, false), IO = instr<T>(D, true);
+            bool ok = mbar_wait(qbar, 0);
+            for (int j = 0; ok && j <= J.blocks; ++j) {
+                const int ki = 2 * j, vi = 2 * j - 1;
+                if (j > 0) ok = ok && mbar_wait(&full[vi % SLOTS], (vi / SLOTS) & 1);
+                if (j < J.blocks) ok = ok && mbar_wait(&full[ki % SLOTS], (ki / SLOTS) & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t ks = base + Ly::RING + (ki % SLOTS) * Ly::TILEB;
+                const uint32_t vs = base + Ly::RING + (vi % SLOTS) * Ly::TILEB;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const uint32_t st = tmem + t * TILE, ot = tmem + 2 * TILE + t * D;
+                    if (j > sp[t].a && j <= sp[t].z) {
+                        ok = ok && mbar_wait(&pbar[t], (j - 1 - sp[t].a) & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int k = 0; k < TILE / 16; ++k)
+                            mma_ts(ot, st + k * 8, desc_v(vs + k * 2048), IO, (j - 1 > sp[t].a || k > 0) ? 1u : 0u);
+                        umma_commit(&obar[t]);
+                    }
+                    if (j >= sp[t].a && j < sp[t].z) {
+                        const uint32_t qs = base + Ly::Q + t * Ly::TILEB;
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k) {
+                            const uint32_t o = (k >> 2) * Ly::ROWB + (k & 3) * 32;
+                            mma_ss(st, desc_k(qs + o), desc_k(ks + o), IS, k > 0 ? 1u : 0u);
+                        }
+                        umma_commit(&sbar[t]);
+                        mbar_arrive(&sbar[t]);
+                    }
+                }
+                if (!ok) break;
+                if (j > 0) umma_commit(&empty[vi % SLOTS]);
+                if (j < J.blocks) umma_commit(&empty[ki % SLOTS]);
+            }
+            if (!ok) *s_abort = 1;
+        }
+        __syncwarp();
+    } else if (warp < PRODUCER0 / 32) {
+        // ---------------- softmax: thread r of the tile's warps is row r
+        const int t = warp >> 2, r = threadIdx.x & (TILE - 1);
+        const Span S = sp[t];
+        const int tok = r / J.heads;
+        const bool live = tok < S.tokens;
+        const int pos = S.pos + min(tok, S.tokens - 1);     // rows of no token see what the last one does
+        const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t st = tmem + quarter + t * TILE, ot = tmem + quarter + 2 * TILE + t * D;
+        // the row sees the places u < sinks and ua <= u, below ub
+        const int ub = J.first + pos + 1 - J.lo;
+        const int ua = P.window > 0 ? J.first + max(0, pos - P.window + 1 - J.lo) : 0;
+        float m = NEG_INF, l0 = 0.f, l1 = 0.f;
+        bool ok = true;
+        for (int j = S.a; j < S.z; ++j) {
+            const int i = j - S.a, u0 = j * TILE;
+            ok = ok && !*s_abort && mbar_wait(&sbar[t], i & 1);
+            if (!__all_sync(FULL, ok)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            uint32_t vis[4];
+            bool whole = true;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int u = u0 + c * 32;
+                vis[c] = low_bits(ub - u) & (low_bits(P.sinks - u) | ~low_bits(ua - u)) & s_seen[(j & 7) * 4 + c];
+                whole = whole && vis[c] == 0xffffffffu;
+            }
+            const bool masked = __any_sync(FULL, !whole);
+            // the row's largest logit
+            float top = NEG_INF;
+            {
+                uint32_t x[2][32];
+                tmem_get32(st, x[0]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    tmem_arrived(x[c & 1]);
+                    if (c < 3) tmem_get32(st + (c + 1) * 32, x[(c + 1) & 1]);
+                    float a[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+                    if (masked) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            a[e & 3] = fmaxf(a[e & 3], (vis[c] >> e) & 1u ? __uint_as_float(x[c & 1][e]) : NEG_INF);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) a[e & 3] = fmaxf(a[e & 3], __uint_as_float(x[c & 1][e]));
+                    }
+                    top = fmaxf(top, fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
+                }
+            }
+            top = top == NEG_INF ? NEG_INF : top * P.scale2;
+            const bool raise = top > m + RAISE || (m == NEG_INF && top != NEG_INF);
+            if (__any_sync(FULL, raise)) {
+                const float f = raise && m != NEG_INF ? exp2_fast(m - top) : 1.f;
+                if (raise) m = top;
+                l0 *= f;
+                l1 *= f;
+                if (i > 0) {
+                    ok = mbar_wait(&obar[t], (i - 1) & 1);
+                    if (!__all_sync(FULL, ok)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t x[32];
+                        tmem_get32(ot + c * 32, x);
+                        tmem_arrived(x);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+                        tmem_put32(ot + c * 32, x);
+                    }
+                    tmem_stored();
+                }
+            }
+            const float off = m == NEG_INF ? 0.f : -m;
+            // weights over the logits that were read
+            {
+                uint32_t x[2][32];
+                tmem_get32(st, x[0]);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    tmem_arrived(x[c & 1]);
+                    if (c < 3) tmem_get32(st + (c + 1) * 32, x[(c + 1) & 1]);
+                    uint32_t p[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        float y0 = fmaf(__uint_as_float(x[c & 1][2 * e]), P.scale2, off);
+                        float y1 = fmaf(__uint_as_float(x[c & 1][2 * e + 1]), P.scale2, off);
+                        if (masked) {
+                            y0 = (vis[c] >> (2 * e)) & 1u ? y0 : NEG_INF;
+                            y1 = (vis[c] >> (2 * e + 1)) & 1u ? y1 : NEG_INF;
+                        }
+                        const float w0 = exp2_fast(y0), w1 = exp2_fast(y1);
+                        l0 += w0;
+                        l1 += w1;
+                        p[e] = Elem<T>::pack(w0, w1);
+                    }
+                    tmem_put16(st + c * 16, p);
+                }
+            }
+            tmem_stored();
+            tc_fence_before();
+            mbar_arrive(&pbar[t]);
+        }
+        // ---- the rows
+        const int blocks = S.z - S.a;
+        if (blocks > 0) ok = ok && !*s_abort && mbar_wait(&obar[t], (blocks - 1) & 1);
+        ok = __all_sync(FULL, ok);
+        if (!ok) *s_abort = 1;
+        tc_fence_after();
+        const float l = l0 + l1;
+        const float inv = ok ? (l == 0.f ? 0.f : 1.f / l) : __int_as_float(0x7fffffff);
+        const int64_t row = (J.token0 + t * P.tile_tokens + tok) * P.q_heads + J.head0 + r % J.heads;
+        uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(P.out) + row * D);
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+            uint32_t x[32];
+            if (blocks > 0) {
+                tmem_get32(ot + c * 32, x);
+                tmem_arrived(x);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[e] = 0u;
+            }
+            if (live) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t p[4];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+                        p[y] = Elem<T>::pack(__uint_as_float(x[8 * e + 2 * y]) * inv, __uint_as_float(x[8 * e + 2 * y + 1]) * inv);
+                    out[c * 4 + e] = make_uint4(p[0], p[1], p[2], p[3]);
+                }
+            }
+        }
+        if (live) P.lse[row] = !ok ? inv : l == 0.f ? NEG_INF : (m + log2f(l)) * LN2;
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (*s_abort && threadIdx.x == 0 && P.status) atomicExch(P.status, *s_abort == 2 ? SWB_ERR_SMEM : ERR_TIMEOUT);
+    if (warp == MMA_WARP) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <typename T, int D>
+int launch(const Prefill& p, int64_t items, cudaStream_t st) {
+    const cudaError_t e = cudaFuncSetAttribute(prefill_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               Layout<D>::TOTAL);
+    if (e != cudaSuccess) return abi::cuda_fail(e, "cudaFuncSetAttribute(prefill)");
+    prefill_kernel<T, D><<<(unsigned)items, THREADS, Layout<D>::TOTAL, st>>>(p);
+    return abi::cuda_check("prefill launch");
+}
+
+}  // namespace pre
+}  // namespace attn
+}  // namespace swb
+
+using namespace swb;
+using namespace swb::attn;
+
+extern "C" int swb_attn_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_heads,
+                                const int32_t* starts, int64_t tokens, const swb_kv_cache* cache, float scale,
+                                int window, int sinks, void* out, float* lse, int32_t* status, void* stream) {
+    pre::Prefill p = {};
+    int rc = check_cache(cache, &p.c);
+    if (rc) return rc;
+    if (p.c.seqs == 0 || tokens <= 0) return SWB_OK;
+    rc = check_query(q, q_token_stride, q_head_stride, q_heads, p.c);
+    if (rc) return rc;
+    if (!starts || !out || !lse) return abi::fail(SWB_ERR_ARG, "null buffer");
+    if (reinterpret_cast<uintptr_t>(out) % 16) return abi::fail(SWB_ERR_ARG, "out must start on a 16-byte boundary");
+    if (window < 0 || sinks < 0) return abi::fail(SWB_ERR_ARG, "window and sinks must not be negative");
+    p.q = q;
+    p.q_token_stride = q_token_stride;
+    p.q_head_stride = q_head_stride;
+    p.starts = starts;
+    p.tokens = tokens;
+    p.q_heads = q_heads;
+    p.group = q_heads / p.c.kv_heads;
+    p.tile_heads = p.group < pre::TILE ? p.group : pre::TILE;
+    p.head_tiles = (p.group + p.tile_heads - 1) / p.tile_heads;
+    p.tile_tokens = pre::TILE / p.tile_heads;
+    p.flip = scale < 0.f;
+    p.scale2 = (scale < 0.f ? -scale : scale) * LOG2E;
+    p.window = window;
+    p.sinks = sinks;
+    p.out = out;
+    p.lse = lse;
+    p.status = status;
+    // every sequence may end in a tile that is not full
+    const int64_t step = 2 * p.tile_tokens;
+    const int64_t items = ((tokens + step - 1) / step + p.c.seqs) * p.c.kv_heads * p.head_tiles;
+    if (items >= ((int64_t)1 << 31)) return abi::fail(SWB_ERR_ARG, "too many tokens in one call");
+    cudaStream_t st = (cudaStream_t)stream;
+    if (cache->dtype == SWB_F16)
+        return cache->head_dim == 64 ? pre::launch<__half, 64>(p, items, st) : pre::launch<__half, 128>(p, items, st);
+    return cache->head_dim == 64 ? pre::launch<__nv_bfloat16, 64>(p, items, st)
+                                 : pre::launch<__nv_bfloat16, 128>(p, items, st);
+}
