@@ -28,6 +28,8 @@ class KVCacheArg(C.Structure):
                 ("page_size", _i32), ("seqs", _i32), ("kv_heads", _i32), ("head_dim", _i32), ("dtype", _i32)]
 
 
+_kv = C.POINTER(KVCacheArg)
+
 # name -> (restype, argtypes), exactly the declarations of include/swann_b200.h
 SIGNATURES = {
     "swb_search_init": (_i32, [_vp, _i32, _i64, _i32, _vp, _vp, _i32, _i32, _i32,
@@ -68,12 +70,12 @@ SIGNATURES = {
     "swb_reverse_tc": (_i32, [_vp, _vp, _vp, _i32, _i32, _vp, _i64, _i32, _vp, _i32, _f32, _i32, _i32, _vp, _i64,
                               _i64, _vp, _vp, _u64, _vp, _vp, _vp]),
     "swb_rope_append": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _vp, _f32,
-                               _vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),
-    "swb_attn_decode": (_i32, [_vp, _i64, _i64, _i32, _vp, _f32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i32,
+                               _vp, _vp, _i64, _i32, _i32, _vp, _kv, _vp, _vp, _i64, _vp]),
+    "swb_attn_decode": (_i32, [_vp, _i64, _i64, _i32, _kv, _f32, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i32,
                                _vp, _u64, _vp]),
-    "swb_attn_decode_workspace": (_u64, [_vp, _i32, _i32]),
-    "swb_attn_prefill": (_i32, [_vp, _i64, _i64, _i32, _vp, _i64, _vp, _f32, _i32, _i32, _vp, _vp, _vp, _vp]),
-    "swb_kv_evict": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _u64, _vp]),
+    "swb_attn_decode_workspace": (_u64, [_kv, _i32, _i32]),
+    "swb_attn_prefill": (_i32, [_vp, _i64, _i64, _i32, _vp, _i64, _kv, _f32, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "swb_kv_evict": (_i32, [_kv, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _u64, _vp]),
     "swb_kv_evict_workspace": (_u64, [_i32, _i32, _i32]),
     "swb_last_error": (C.c_char_p, []),
     "swb_version": (_i32, []),

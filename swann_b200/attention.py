@@ -28,9 +28,6 @@ models, it does not train them.
 """
 from __future__ import annotations
 
-import contextlib
-import ctypes as C
-
 import torch
 
 from . import _lib as N
@@ -39,61 +36,83 @@ _DTYPES = {torch.float16: N.F16, torch.bfloat16: N.BF16}
 HEAD_DIMS = (64, 128)
 
 
+_stream = torch._C._cuda_getCurrentRawStream       # of a device index: no Stream object is made
+
+
 def _fail(what, why):
     raise ValueError(f"{what}: {why}")
 
 
-def _on(t):
-    """Kernels launch on the tensors' device."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _call(what, fn, t, *args):
+    """A native call on the tensors' device and its current stream."""
+    dev = t.get_device()
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream(dev))
+    if rc:
+        N.check(rc, what)
 
 
-def _ints(what, name, t, shape, device):
-    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
-        _fail(what, f"{name} must be contiguous int32 {list(shape)} on {device}")
+def _ints(what, name, t, shape, dev):
+    if t.dtype is not torch.int32 or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+        _fail(what, f"{name} must be contiguous int32 {list(shape)} on cuda:{dev}")
 
 
 def _cache_arg(what, k, v, table, lengths):
-    if k.device.type != "cuda":
+    """The cache as the native calls take it, and its device."""
+    dev = k.get_device()
+    if dev < 0:
         _fail(what, "the cache must be on the GPU")
-    if k.dtype not in _DTYPES or v.dtype != k.dtype:
+    kind = _DTYPES.get(k.dtype)
+    if kind is None or v.dtype is not k.dtype:
         _fail(what, "the cache must be float16 or bfloat16")
-    if k.dim() != 4 or v.shape != k.shape or v.stride() != k.stride() or v.device != k.device:
+    shape, strides = k.shape, k.stride()
+    if len(shape) != 4 or v.shape != shape or v.stride() != strides or v.get_device() != dev:
         _fail(what, "k and v must be [pages, kv_heads, page_size, head_dim] with the same strides")
-    pages, heads, page, d = k.shape
-    ps, hs, rs, es = k.stride()
+    pages, heads, page, d = shape
+    ps, hs, rs, es = strides
     if d not in HEAD_DIMS:
         _fail(what, f"head_dim must be one of {HEAD_DIMS}")
     if es != 1:
         _fail(what, "the rows of the cache must be contiguous")
     if page < 1 or page & (page - 1):
         _fail(what, "page_size must be a power of two")
-    if table.dim() != 2 or table.dtype != torch.int32 or table.device != k.device or \
-            (table.shape[1] > 1 and table.stride(1) != 1):
-        _fail(what, f"the page table must be int32 [seqs, max_pages] on {k.device}, rows contiguous")
-    _ints(what, "lengths", lengths, (table.shape[0],), k.device)
-    return N.KVCacheArg(N.ptr(k), N.ptr(v), ps, hs, rs, N.ptr(table), table.stride(0), N.ptr(lengths), pages,
-                        table.shape[1], page, table.shape[0], heads, d, _DTYPES[k.dtype])
+    at = table.shape
+    if len(at) != 2 or table.dtype is not torch.int32 or table.get_device() != dev or \
+            (at[1] > 1 and table.stride(1) != 1):
+        _fail(what, f"the page table must be int32 [seqs, max_pages] on cuda:{dev}, rows contiguous")
+    seqs, most = at
+    if lengths.dtype is not torch.int32 or lengths.get_device() != dev or lengths.shape != (seqs,) or \
+            not lengths.is_contiguous():
+        _fail(what, f"lengths must be contiguous int32 [{seqs}] on cuda:{dev}")
+    return N.KVCacheArg(k.data_ptr(), v.data_ptr(), ps, hs, rs, table.data_ptr(), table.stride(0), lengths.data_ptr(),
+                        pages, most, page, seqs, heads, d, kind), dev
 
 
-def _heads(what, name, t, k, heads=None):
-    """[tokens, heads, head_dim] of the cache's type, any strides with contiguous rows."""
-    if t.dim() != 3 or t.shape[2] != k.shape[3] or t.dtype != k.dtype or t.device != k.device:
-        _fail(what, f"{name} must be [tokens, heads, {k.shape[3]}] {k.dtype} on {k.device}")
-    if heads is not None and t.shape[1] != heads:
+def _heads(what, name, t, k, dev, heads=None):
+    """[tokens, heads, head_dim] of the cache's type, any strides with contiguous rows; its shape and strides."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != k.shape[3] or t.dtype is not k.dtype or t.get_device() != dev:
+        _fail(what, f"{name} must be [tokens, heads, {k.shape[3]}] {k.dtype} on cuda:{dev}")
+    if heads is not None and shape[1] != heads:
         _fail(what, f"{name} must have {heads} heads")
-    if t.stride(2) != 1:
+    strides = t.stride()
+    if strides[2] != 1:
         _fail(what, f"the rows of {name} must be contiguous")
+    return shape, strides
 
 
-def _out(what, name, t, like_shape, dtype, device):
-    if t is None:
-        return torch.empty(like_shape, dtype=dtype, device=device)
-    if tuple(t.shape) != tuple(like_shape) or t.dtype != dtype or t.device != device or not t.is_contiguous():
-        _fail(what, f"{name} must be contiguous {dtype} {list(like_shape)} on {device}")
+def _given(what, name, t, shape, dtype, dev):
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+        _fail(what, f"{name} must be contiguous {dtype} {list(shape)} on cuda:{dev}")
     return t
+
+
+def _group(what, q_heads, kv_heads):
+    if q_heads < 1 or q_heads % kv_heads:
+        _fail(what, "query heads must be a multiple of the cache's key heads")
 
 
 def rope_append(q, k, v, cos, sin, k_cache, v_cache, table, starts, lengths, *, q_norm=None, k_norm=None, eps=1e-6,
@@ -110,40 +129,36 @@ def rope_append(q, k, v, cos, sin, k_cache, v_cache, table, starts, lengths, *, 
     None for no norm.  slot_positions int32 [seqs, kv_heads, slots] records the
     positions.  Returns the queries [tokens, q_heads, d]."""
     what = "rope_append"
-    arg = _cache_arg(what, k_cache, v_cache, table, lengths)
-    T, hq, d = q.shape if q.dim() == 3 else (0, 0, 0)
-    hkv = k_cache.shape[1]
-    _heads(what, "q", q, k_cache)
-    _heads(what, "k", k, k_cache, hkv)
-    _heads(what, "v", v, k_cache, hkv)
-    if k.shape[0] != T or v.shape[0] != T:
+    arg, dev = _cache_arg(what, k_cache, v_cache, table, lengths)
+    hkv, seqs = arg.kv_heads, arg.seqs
+    (T, hq, d), qs = _heads(what, "q", q, k_cache, dev)
+    ksh, ks = _heads(what, "k", k, k_cache, dev, hkv)
+    vsh, vs = _heads(what, "v", v, k_cache, dev, hkv)
+    if ksh[0] != T or vsh[0] != T:
         _fail(what, "q, k and v must have the same tokens")
-    if hq < 1 or hq % hkv:
-        _fail(what, "query heads must be a multiple of the cache's key heads")
-    dev = q.device
-    _ints(what, "starts", starts, (table.shape[0] + 1,), dev)
-    if cos.dim() != 2 or cos.shape != sin.shape:
+    _group(what, hq, hkv)
+    _ints(what, "starts", starts, (seqs + 1,), dev)
+    rows = cos.shape
+    if len(rows) != 2 or sin.shape != rows:
         _fail(what, "cos and sin must be [positions, rotated / 2]")
     for t in (cos, sin):
-        if t.dtype != torch.float32 or t.device != dev or not t.is_contiguous():
-            _fail(what, f"cos and sin must be contiguous float32 on {dev}")
-    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if w is not None and (w.dtype != q.dtype or w.device != dev or tuple(w.shape) != (d,) or not w.is_contiguous()):
-            _fail(what, f"{name} must be contiguous {q.dtype} [{d}] on {dev}")
+        if t.dtype is not torch.float32 or t.get_device() != dev or not t.is_contiguous():
+            _fail(what, f"cos and sin must be contiguous float32 on cuda:{dev}")
+    if q_norm is not None:
+        _given(what, "q_norm", q_norm, (d,), q.dtype, dev)
+    if k_norm is not None:
+        _given(what, "k_norm", k_norm, (d,), q.dtype, dev)
     if positions is not None:
         _ints(what, "positions", positions, (T,), dev)
     width = 0
     if slot_positions is not None:
         width = slot_positions.shape[-1]
-        _ints(what, "slot_positions", slot_positions, (table.shape[0], hkv, width), dev)
-    out = _out(what, "out", out, (T, hq, d), q.dtype, dev)
-    with _on(q):
-        rc = N.lib().swb_rope_append(
-            N.ptr(q), q.stride(0), q.stride(1), N.ptr(k), k.stride(0), k.stride(1), N.ptr(v), v.stride(0), v.stride(1),
-            hq, N.ptr(starts), T, N.ptr(q_norm), N.ptr(k_norm), float(eps), N.ptr(cos), N.ptr(sin), cos.shape[0],
-            2 * cos.shape[1], int(bool(interleaved)), N.ptr(positions), C.byref(arg), N.ptr(out),
-            N.ptr(slot_positions), width, N.stream_of(q))
-    N.check(rc, what)
+        _ints(what, "slot_positions", slot_positions, (seqs, hkv, width), dev)
+    out = q.new_empty((T, hq, d)) if out is None else _given(what, "out", out, (T, hq, d), q.dtype, dev)
+    if T:
+        _call(what, N.lib().swb_rope_append, q, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0],
+              vs[1], hq, starts.data_ptr(), T, N.ptr(q_norm), N.ptr(k_norm), eps, cos.data_ptr(), sin.data_ptr(), rows[0],
+              2 * rows[1], bool(interleaved), N.ptr(positions), arg, out.data_ptr(), N.ptr(slot_positions), width)
     return out
 
 
@@ -159,37 +174,31 @@ def decode(q, k_cache, v_cache, table, lengths, *, scale=None, window=0, sinks=0
     is written there, or added with `accumulate`.  Returns out [seqs, q_heads,
     d] and lse float32 [seqs, q_heads], 0 and -inf where nothing is seen."""
     what = "decode"
-    arg = _cache_arg(what, k_cache, v_cache, table, lengths)
-    _heads(what, "q", q, k_cache)
-    B, hq, d = q.shape
-    if B != table.shape[0]:
-        _fail(what, f"q must have one token for each of the {table.shape[0]} sequences")
-    if hq < 1 or hq % k_cache.shape[1]:
-        _fail(what, "query heads must be a multiple of the cache's key heads")
-    dev = q.device
-    po = pl = None
+    arg, dev = _cache_arg(what, k_cache, v_cache, table, lengths)
+    (B, hq, d), qs = _heads(what, "q", q, k_cache, dev)
+    if B != arg.seqs:
+        _fail(what, f"q must have one token for each of the {arg.seqs} sequences")
+    _group(what, hq, arg.kv_heads)
+    po = pl = wp = None
     if prior is not None:
-        po = _out(what, "the prior rows", prior[0], (B, hq, d), q.dtype, dev)
-        pl = _out(what, "the prior lse", prior[1], (B, hq), torch.float32, dev)
+        po = _given(what, "the prior rows", prior[0], (B, hq, d), q.dtype, dev).data_ptr()
+        pl = _given(what, "the prior lse", prior[1], (B, hq), torch.float32, dev).data_ptr()
     width = 0
     if weights is not None:
         width = weights.shape[-1]
-        _out(what, "weights", weights, (B, k_cache.shape[1], width), torch.float32, dev)
-        if width < table.shape[1] * k_cache.shape[2]:
+        wp = _given(what, "weights", weights, (B, arg.kv_heads, width), torch.float32, dev).data_ptr()
+        if width < arg.max_pages * arg.page_size:
             _fail(what, "weights are narrower than the page table's slots")
-    out = _out(what, "out", out, (B, hq, d), q.dtype, dev)
-    lse = torch.empty((B, hq), dtype=torch.float32, device=dev)
+    out = q.new_empty((B, hq, d)) if out is None else _given(what, "out", out, (B, hq, d), q.dtype, dev)
+    lse = torch.empty((B, hq), dtype=torch.float32, device=q.device)
     if B == 0:
         return out, lse
     L = N.lib()
-    with _on(q):
-        need = L.swb_attn_decode_workspace(C.byref(arg), hq, int(weights is not None))
-        ws = torch.empty((need if need < 1 << 62 else 0,), dtype=torch.uint8, device=dev)
-        rc = L.swb_attn_decode(
-            N.ptr(q), q.stride(0), q.stride(1), hq, C.byref(arg), d ** -0.5 if scale is None else float(scale),
-            int(window), int(sinks), N.ptr(po), N.ptr(pl), N.ptr(out), N.ptr(lse), N.ptr(weights), width,
-            int(bool(accumulate)), N.ptr(ws), ws.numel(), N.stream_of(q))
-    N.check(rc, what)
+    need = L.swb_attn_decode_workspace(arg, hq, wp is not None)
+    # a size that says the call will be refused is left to the call
+    ws = torch.empty(need if need < 1 << 62 else 0, dtype=torch.uint8, device=q.device)
+    _call(what, L.swb_attn_decode, q, q.data_ptr(), qs[0], qs[1], hq, arg, d ** -0.5 if scale is None else scale, window,
+          sinks, po, pl, out.data_ptr(), lse.data_ptr(), wp, width, bool(accumulate), ws.data_ptr(), need)
     return out, lse
 
 
@@ -201,23 +210,15 @@ def prefill(q, k_cache, v_cache, table, starts, lengths, *, scale=None, window=0
     a window, of those only j > i - window and j < sinks.  Returns out
     [tokens, q_heads, d] and lse float32 [tokens, q_heads]."""
     what = "prefill"
-    arg = _cache_arg(what, k_cache, v_cache, table, lengths)
-    _heads(what, "q", q, k_cache)
-    T, hq, d = q.shape
-    if hq < 1 or hq % k_cache.shape[1]:
-        _fail(what, "query heads must be a multiple of the cache's key heads")
-    dev = q.device
-    _ints(what, "starts", starts, (table.shape[0] + 1,), dev)
-    out = _out(what, "out", out, (T, hq, d), q.dtype, dev)
-    lse = torch.empty((T, hq), dtype=torch.float32, device=dev)
-    if T == 0:
-        return out, lse
-    with _on(q):
-        rc = N.lib().swb_attn_prefill(
-            N.ptr(q), q.stride(0), q.stride(1), hq, N.ptr(starts), T, C.byref(arg),
-            d ** -0.5 if scale is None else float(scale), int(window), int(sinks), N.ptr(out), N.ptr(lse),
-            None, N.stream_of(q))
-    N.check(rc, what)
+    arg, dev = _cache_arg(what, k_cache, v_cache, table, lengths)
+    (T, hq, d), qs = _heads(what, "q", q, k_cache, dev)
+    _group(what, hq, arg.kv_heads)
+    _ints(what, "starts", starts, (arg.seqs + 1,), dev)
+    out = q.new_empty((T, hq, d)) if out is None else _given(what, "out", out, (T, hq, d), q.dtype, dev)
+    lse = torch.empty((T, hq), dtype=torch.float32, device=q.device)
+    if T:
+        _call(what, N.lib().swb_attn_prefill, q, q.data_ptr(), qs[0], qs[1], hq, starts.data_ptr(), T, arg,
+              d ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(), lse.data_ptr(), None)
     return out, lse
 
 
@@ -233,15 +234,13 @@ def evict(k_cache, v_cache, table, lengths, weights, positions, budget, *, seen,
     Rows move inside the pools; returns the new (lengths, weights, positions)
     as tensors of their own, 0 and -1 in slots that hold nothing."""
     what = "evict"
-    arg = _cache_arg(what, k_cache, v_cache, table, lengths)
-    B, hkv, dev = table.shape[0], k_cache.shape[1], k_cache.device
-    if weights.dim() != 3:
-        _fail(what, "weights must be float32 [seqs, kv_heads, slots]")
-    width = weights.shape[2]
-    _out(what, "weights", weights, (B, hkv, width), torch.float32, dev)
+    arg, dev = _cache_arg(what, k_cache, v_cache, table, lengths)
+    B, hkv = arg.seqs, arg.kv_heads
+    width = weights.shape[-1]
+    _given(what, "weights", weights, (B, hkv, width), torch.float32, dev)
     _ints(what, "positions", positions, (B, hkv, width), dev)
     _ints(what, "seen", seen, (B,), dev)
-    if width < table.shape[1] * k_cache.shape[2]:
+    if width < arg.max_pages * arg.page_size:
         _fail(what, "weights are narrower than the page table's slots")
     if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
         _fail(what, "the budget must be at least 1, and hold sinks and recent")
@@ -249,9 +248,8 @@ def evict(k_cache, v_cache, table, lengths, weights, positions, budget, *, seen,
     if B == 0:
         return nl, nw, np_
     L = N.lib()
-    with _on(k_cache):
-        ws = torch.empty((L.swb_kv_evict_workspace(B, hkv, int(budget)),), dtype=torch.uint8, device=dev)
-        rc = L.swb_kv_evict(C.byref(arg), N.ptr(seen), N.ptr(weights), N.ptr(positions), width, int(budget), int(sinks),
-                            int(recent), N.ptr(nl), N.ptr(nw), N.ptr(np_), N.ptr(ws), ws.numel(), N.stream_of(k_cache))
-    N.check(rc, what)
+    need = L.swb_kv_evict_workspace(B, hkv, budget)
+    ws = torch.empty(need, dtype=torch.uint8, device=weights.device)
+    _call(what, L.swb_kv_evict, weights, arg, seen.data_ptr(), weights.data_ptr(), positions.data_ptr(), width, budget, sinks,
+          recent, nl.data_ptr(), nw.data_ptr(), np_.data_ptr(), ws.data_ptr(), need)
     return nl, nw, np_

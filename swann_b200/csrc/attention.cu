@@ -8,27 +8,32 @@
 // in one pass over K and V, with the running maximum m and sum l of a softmax
 // in base 2:  m' = max(m, x), l' = l 2^(m - m') + 2^(x - m'), and the
 // accumulated rows scaled by the same 2^(m - m').  Where nothing is seen the
-// row is 0 and lse is -inf.
+// row is 0 and lse is -inf.  The bytes of K and V bound it.
 //
-// One warp owns up to 16 query rows that share a key head and walks blocks of
-// 16 keys on its own: keys and values arrive by cp.async in a ring of shared
-// memory stages (128-byte swizzle, rows that are not seen filled with zeros, so
-// nothing that lies in them reaches a product), logits and the weighted sum run
-// on mma.sync with fp32 accumulators.  Weights are rounded to the cache's 16
-// bits for the second product, as its other operand is; their sum l is taken
-// before that rounding.  The warps of a CTA interleave the blocks of one stretch
-// of the sequence and join through shared memory at the end; the stretches of a
-// long sequence are joined by a second kernel.
+// One warp owns up to 16 query rows that share a key head (a pair: a sequence
+// and those rows) and walks blocks of 16 keys on its own: keys and values arrive
+// by cp.async in a ring of shared memory stages (128-byte swizzle, rows that are
+// not seen filled with zeros, so nothing that lies in them reaches a product),
+// logits and the weighted sum run on mma.sync with fp32 accumulators (16 rows at
+// most: a tcgen05 tile of 128 would be seven eighths empty, and the tensor pipe
+// is not what bounds this).  Weights are rounded to the cache's 16 bits for the
+// second product, as its other operand is; their sum l is taken before that.
+//
+// Who walks what.  Few pairs: the pairs' units of 64 keys are laid end to end
+// and every CTA of a grid that the SMs hold at once takes an equal run of them,
+// whatever the sequences' lengths are; a pair cut by the end of a run leaves
+// parts (m, l, unnormalised rows), at most two a CTA, which a second kernel
+// joins.  Very many pairs: a one-warp CTA each.
 
 #include "attn.cuh"
 
 namespace swb {
 namespace attn {
 
-constexpr int WARPS = 4;
-constexpr int THREADS = WARPS * 32;
+constexpr int WARPS = 4;      // of a CTA that takes a run of units
 constexpr int ROWS = 16;      // query rows of a tile
 constexpr int KEYS = 16;      // keys a warp scores at a time
+constexpr int UNIT = WARPS * KEYS;
 constexpr int STAGES = 3;
 
 struct Walk {
@@ -37,16 +42,17 @@ struct Walk {
     int64_t q_seq_stride, q_head_stride;
     int q_heads, group;       // query heads; of them per key head
     int head_tiles, tile_heads;
-    int splits;
     float scale2;             // scale * log2(e)
     int window, sinks;
     const void* prior_out;    // [seqs, q_heads, D] and [seqs, q_heads]; null: none
     const float* prior_lse;
     void* out;
     float* lse;
-    float* part_out;          // [rows][splits][D]
-    float2* part_ml;          // [rows][splits]
+    int runs;                 // CTAs that share the units; 0: a CTA a pair
+    float* part_out;          // [2 * runs][ROWS][D]
+    float2* part_ml;          // [2 * runs][ROWS]
     float* logits;            // [seqs * q_heads][capacity], for the weights; null: not wanted
+    float* lse2;              // [seqs * q_heads] in base 2, with logits
 };
 
 // the slots that the token at slot `pos` can see, as one range of virtual
@@ -69,32 +75,125 @@ __device__ __forceinline__ uint32_t swz(int row, int chunk) {
     return (uint32_t)(row * D * 2 + ((chunk ^ (row & 7)) << 4));
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(THREADS) walk_kernel(const __grid_constant__ Walk P) {
+__device__ __forceinline__ int units_of(const Walk& P, int b) {
+    const Range r = visible(P.c.lengths[b] - 1, P.window, P.sinks, P.c.capacity());
+    return max(1, (r.n + UNIT - 1) / UNIT);
+}
+
+// The sequences' units laid end to end, counted by all threads of a CTA: thread t
+// sums a stretch of sequences.
+template <int THREADS>
+struct Layout {
+    int64_t before;           // units of a pair row (one key head) ahead of this thread's stretch
+    int64_t mine;
+    int64_t total;            // of all sequences, one key head tile
+    int per;                  // sequences of a stretch
+    __device__ __forceinline__ void count(const Walk& P, int64_t* s_sum) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        per = (P.c.seqs + THREADS - 1) / THREADS;
+        const int b0 = min(P.c.seqs, (int)threadIdx.x * per), b1 = min(P.c.seqs, b0 + per);
+        mine = 0;
+        for (int b = b0; b < b1; ++b) mine += units_of(P, b);
+        int64_t sum = mine;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const int64_t y = __shfl_up_sync(FULL, (long long)sum, s);
+            if (lane >= s) sum += y;
+        }
+        if (lane == 31) s_sum[warp] = sum;
+        __syncthreads();
+        before = sum - mine;
+        total = 0;
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; ++w) {
+            before += w < warp ? s_sum[w] : 0;
+            total += s_sum[w];
+        }
+        __syncthreads();
+    }
+};
+
+// a place among the units: a pair, its key head tile and the unit inside it
+struct Spot {
+    int b, h;                 // sequence; key head * head_tiles + tile
+    int unit, units;          // of the pair
+};
+
+// CTA-wide: where unit x of the whole lies.  Sequence-major: all head tiles of a
+// sequence, then the next.
+template <int THREADS>
+__device__ __forceinline__ Spot spot_of(const Walk& P, const Layout<THREADS>& L, int64_t x, Spot* s_spot) {
+    const int tiles = P.c.kv_heads * P.head_tiles;
+    int64_t left = x - L.before * tiles;
+    if (left >= 0 && left < L.mine * tiles) {
+        int b = threadIdx.x * L.per;
+        for (;; ++b) {
+            const int n = units_of(P, b);
+            if (left < (int64_t)n * tiles) {
+                s_spot->b = b;
+                s_spot->h = (int)(left / n);
+                s_spot->unit = (int)(left % n);
+                s_spot->units = n;
+                break;
+            }
+            left -= (int64_t)n * tiles;
+        }
+    }
+    __syncthreads();
+    return *s_spot;
+}
+
+// CTAs that take a run, and where a run begins
+__device__ __forceinline__ int64_t runs_used(const Walk& P, int64_t all) { return min((int64_t)P.runs, all); }
+
+// CTAs of a run that an SM holds, by their shared memory and registers
+constexpr int cta_per_sm(int d) { return d == 128 ? 2 : 4; }
+
+template <typename T, int D, int W>
+__global__ void __launch_bounds__(W * 32, W > 1 ? cta_per_sm(D) : 8) walk_kernel(const __grid_constant__ Walk P) {
+    constexpr int THREADS = W * 32;
+    constexpr bool RUNS = W > 1;                       // an equal run of units a CTA, or a pair a warp
     constexpr int CH = D / 8;                          // 16-byte chunks of a row
     constexpr int STAGE = 2 * KEYS * D * 2;            // K and V of a block of keys
     constexpr int NT = D / 8;                          // 8-wide output tiles
     extern __shared__ __align__(128) char smem[];
-    __shared__ unsigned s_seen[WARPS][STAGES];
-    __shared__ float s_m[WARPS][ROWS], s_l[WARPS][ROWS];
+    __shared__ unsigned s_seen[W][STAGES];
+    __shared__ float s_m[W][ROWS], s_l[W][ROWS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    // -- which sequence, heads and stretch
-    int64_t item = blockIdx.x;
-    const int split = (int)(item % P.splits);
-    item /= P.splits;
-    const int ht = (int)(item % P.head_tiles);
-    item /= P.head_tiles;
-    const int g = (int)(item % P.c.kv_heads), b = (int)(item / P.c.kv_heads);
+    const uint32_t ring = smem_u32(smem) + warp * (STAGES * STAGE);
+
+    // -- which pairs, and which of their keys
+    Spot at;
+    int64_t left = 1;                                  // units still to walk
+    if constexpr (RUNS) {
+        __shared__ int64_t s_sum[W];
+        __shared__ Spot s_spot;
+        Layout<THREADS> lay;
+        lay.count(P, s_sum);
+        const int64_t all = lay.total * P.c.kv_heads * P.head_tiles, used = runs_used(P, all);
+        if (blockIdx.x >= used) return;
+        const int64_t x0 = all * blockIdx.x / used;
+        left = all * (blockIdx.x + 1) / used - x0;
+        at = spot_of(P, lay, x0, &s_spot);
+    } else {
+        const int tiles = P.c.kv_heads * P.head_tiles;
+        at.b = (int)(blockIdx.x / tiles);
+        at.h = (int)(blockIdx.x % tiles);
+        at.unit = 0;
+        at.units = 1;
+    }
+
+    for (bool first = true; left > 0; first = false) {
+    const int b = at.b, g = at.h / P.head_tiles, ht = at.h % P.head_tiles;
     const int heads = min(P.tile_heads, P.group - ht * P.tile_heads);
     const int64_t row0 = (int64_t)b * P.q_heads + g * P.group + ht * P.tile_heads;   // first output row
     const Range rg = visible(P.c.lengths[b] - 1, P.window, P.sinks, P.c.capacity());
-
-    // this CTA's stretch: a whole number of blocks for every warp
-    const int per = ((rg.n + P.splits - 1) / P.splits + WARPS * KEYS - 1) / (WARPS * KEYS) * (WARPS * KEYS);
-    const int u0 = min(rg.n, split * per), u1 = min(rg.n, u0 + per);
-    const int nblk = (u1 - u0 + KEYS - 1) / KEYS;                // blocks of the stretch; warp w has w, w + WARPS, ..
-    const int mine = nblk > warp ? (nblk - warp - 1) / WARPS + 1 : 0;
+    const int take = (int)min(left, (int64_t)(at.units - at.unit));
+    const int u0 = RUNS ? min(rg.n, at.unit * UNIT) : 0, u1 = RUNS ? min(rg.n, u0 + take * UNIT) : rg.n;
+    const bool entire = take == at.units;              // nothing of the pair is left to others
+    const int nblk = (u1 - u0 + KEYS - 1) / KEYS;      // blocks of the stretch; warp w has w, w + W, ..
+    const int mine = nblk > warp ? (nblk - warp - 1) / W + 1 : 0;
 
     // -- the query rows as matrix fragments: row r is head r of the tile
     const T* q = static_cast<const T*>(P.q) + b * P.q_seq_stride + (int64_t)(g * P.group + ht * P.tile_heads) * P.q_head_stride;
@@ -116,11 +215,9 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const __grid_constant__ W
 
     const T* kp = static_cast<const T*>(P.c.k) + (int64_t)g * P.c.head_stride;
     const T* vp = static_cast<const T*>(P.c.v) + (int64_t)g * P.c.head_stride;
-    const uint32_t ring = smem_u32(smem) + warp * (STAGES * STAGE);
-
     // lane < 16: the row of key `lane` of this warp's block i, or -1
     auto find = [&](int i) -> int64_t {
-        const int u = u0 + (i * WARPS + warp) * KEYS + lane;
+        const int u = u0 + (i * W + warp) * KEYS + lane;
         return (lane < KEYS && i < mine && u < u1) ? P.c.row(b, rg.slot(u)) : -1;
     };
     auto issue = [&](int i, int64_t off) {
@@ -171,7 +268,7 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const __grid_constant__ W
             Elem<T>::mma(x[0], qf[kk], f[0], f[1]);
             Elem<T>::mma(x[1], qf[kk], f[2], f[3]);
         }
-        const int ub = u0 + (i * WARPS + warp) * KEYS;
+        const int ub = u0 + (i * W + warp) * KEYS;
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -241,12 +338,12 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const __grid_constant__ W
     __syncthreads();      // the ring is free too
     float M0 = NEG_INF, M1 = NEG_INF;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
+    for (int w = 0; w < W; ++w) {
         M0 = fmaxf(M0, s_m[w][r0]);
         M1 = fmaxf(M1, s_m[w][r1]);
     }
     const float f0 = l0 == 0.f ? 0.f : exp2_fast(m0 - M0), f1 = l1 == 0.f ? 0.f : exp2_fast(m1 - M1);
-    float* so = reinterpret_cast<float*>(smem);       // [WARPS][ROWS][D]
+    float* so = reinterpret_cast<float*>(smem);       // [W][ROWS][D]
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
         const int c = j * 8 + (lane & 3) * 2;
@@ -257,12 +354,12 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const __grid_constant__ W
     constexpr int TPR = THREADS / ROWS;                // threads of a row
     constexpr int DPT = D / TPR;                       // dimensions of a thread
     const int r = threadIdx.x / TPR, d0 = (threadIdx.x % TPR) * 2;
-    if (r >= heads) return;
+    if (r < heads) {
     float M = NEG_INF, l = 0.f;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_m[w][r]);
+    for (int w = 0; w < W; ++w) M = fmaxf(M, s_m[w][r]);
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w)
+    for (int w = 0; w < W; ++w)
         if (s_l[w][r] != 0.f) l += s_l[w][r] * exp2_fast(s_m[w][r] - M);
     const int64_t row = row0 + r;
     float2 acc[DPT / 2];
@@ -270,20 +367,20 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const __grid_constant__ W
     for (int i = 0; i < DPT / 2; ++i) {
         acc[i] = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float2 y = *reinterpret_cast<const float2*>(so + (w * ROWS + r) * D + d0 + i * 2 * TPR);
             acc[i].x += y.x;
             acc[i].y += y.y;
         }
     }
-    if (P.splits > 1 || P.logits) {
-        float* po = P.part_out + (row * P.splits + split) * D;
+    if (!entire) {
+        const int64_t part = 2 * (int64_t)blockIdx.x + (first ? 0 : 1);
+        float* po = P.part_out + (part * ROWS + r) * D;
 #pragma unroll
         for (int i = 0; i < DPT / 2; ++i) *reinterpret_cast<float2*>(po + d0 + i * 2 * TPR) = acc[i];
-        if (threadIdx.x % TPR == 0) P.part_ml[row * P.splits + split] = make_float2(M, l);
-        return;
-    }
-    // one stretch: this is the answer, up to the prior part
+        if (threadIdx.x % TPR == 0) P.part_ml[part * ROWS + r] = make_float2(M, l);
+    } else {
+    // the whole pair: this is the answer, up to the prior part
     float pm = P.prior_lse ? P.prior_lse[row] * LOG2E : NEG_INF;
     const float top = fmaxf(M, pm);
     const float fa = l == 0.f ? 0.f : exp2_fast(M - top), fb = pm == NEG_INF ? 0.f : exp2_fast(pm - top);
@@ -301,195 +398,215 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const __grid_constant__ W
         }
         out[(d0 + i * 2 * TPR) / 2] = Elem<T>::pack(y.x * inv, y.y * inv);
     }
-    if (threadIdx.x % TPR == 0) P.lse[row] = sum == 0.f ? NEG_INF : (top + log2f(sum)) * LN2;
+    if (threadIdx.x % TPR == 0) {
+        const float x = sum == 0.f ? NEG_INF : top + log2f(sum);
+        P.lse[row] = x * LN2;
+        if (P.lse2) P.lse2[row] = x;
+    }
+    }
+    }
+    left -= take;
+    at.unit = 0;
+    if (left > 0) {
+        if (++at.h == P.c.kv_heads * P.head_tiles) {
+            at.h = 0;
+            ++at.b;
+            at.units = units_of(P, at.b);
+        }
+        __syncthreads();      // the joined rows have been read: the ring is free
+    }
+    }
 }
 
-// -- the join of a row's stretches, and the weights of the slots ----------------
+// -- the join of a pair's parts ------------------------------------------------
 
-struct Join {
-    Cache c;
-    int q_heads, group, splits;
-    int64_t rows;             // seqs * q_heads
-    int window, sinks;
-    const float* part_out;
-    const float2* part_ml;
-    const void* prior_out;
-    const float* prior_lse;
-    void* out;
-    float* lse;
-    const float* logits;
-    float* weights;           // [seqs][kv_heads][width]; null: not wanted
-    int64_t width;
-    int accumulate;
-    int chunks;               // blocks of JOIN_SLOTS slots of a row of weights
-};
+constexpr int JOIN_THREADS = 256;
 
-constexpr int JOIN_THREADS = 128;
-constexpr int JOIN_SLOTS = 1024;
+// CTA (i, r): row r of the pair that the end of run i cuts, if no earlier end cuts it
+template <typename T, int D>
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ Walk P) {
+    constexpr int W = JOIN_THREADS / 32, E = D / 32;
+    __shared__ int64_t s_sum[W];
+    __shared__ Spot s_spot;
+    __shared__ float s_o[W][D];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y;
+    Layout<JOIN_THREADS> lay;
+    lay.count(P, s_sum);       // lengths are not what the kernel before this one writes
+    const int64_t all = lay.total * P.c.kv_heads * P.head_tiles, used = runs_used(P, all);
+    const int64_t i = blockIdx.x, cut = all * (i + 1) / used;
+    const bool inside = i + 1 < used;
+    const Spot at = spot_of(P, lay, inside ? cut : 0, &s_spot);
+    // every CTA waits, also those without work: a kernel after this one may then
+    // rely on the one before it
+    dependency_wait();
+    if (!inside || at.unit == 0) return;                                       // the cut lies between two pairs
+    const int64_t p0 = cut - at.unit, p1 = p0 + at.units;           // the pair's units
+    if (p0 < all * i / used) return;                                // run i does not begin it: an earlier cut has it
+    const int g = at.h / P.head_tiles, ht = at.h % P.head_tiles;
+    if (r >= min(P.tile_heads, P.group - ht * P.tile_heads)) return;
+    const int64_t row = (int64_t)at.b * P.q_heads + g * P.group + ht * P.tile_heads + r;
+    // runs i .. i + n - 1 hold parts: run i in its first place if the pair begins it, else in its second
+    int64_t n = 1;
+    while (all * (i + n) / used < p1) ++n;
+    const int64_t part0 = 2 * i + (all * i / used == p0 ? 0 : 1);
 
-// maximum and sum of a row's stretches and its prior part, by one warp
-__device__ __forceinline__ float2 row_total(const Join& P, int64_t row, int lane) {
-    float m = NEG_INF;
-    for (int s = lane; s < P.splits; s += 32) m = fmaxf(m, P.part_ml[row * P.splits + s].x);
-    if (P.prior_lse && lane == 0) m = fmaxf(m, P.prior_lse[row] * LOG2E);
+    const float prior = P.prior_lse ? P.prior_lse[row] * LOG2E : NEG_INF;
+    float m = prior;
+    for (int64_t s = lane; s < n; s += 32) m = fmaxf(m, P.part_ml[(s ? 2 * (i + s) : part0) * ROWS + r].x);
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, x));
-    float l = 0.f;
-    for (int s = lane; s < P.splits; s += 32) {
-        const float2 y = P.part_ml[row * P.splits + s];
-        if (y.y != 0.f) l += y.y * exp2_fast(y.x - m);
+    float l = 0.f, acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 4
+    for (int64_t s = warp; s < n; s += W) {
+        const int64_t part = (s ? 2 * (i + s) : part0) * ROWS + r;
+        const float2 ml = P.part_ml[part];
+        float x[E];
+        if constexpr (E == 4) {
+            const float4 y = *reinterpret_cast<const float4*>(P.part_out + part * D + lane * 4);
+            x[0] = y.x;
+            x[1] = y.y;
+            x[2] = y.z;
+            x[3] = y.w;
+        } else {
+            const float2 y = *reinterpret_cast<const float2*>(P.part_out + part * D + lane * 2);
+            x[0] = y.x;
+            x[1] = y.y;
+        }
+        const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - m);    // nothing seen there: 0
+        l += ml.y * f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += x[e] * f;
     }
-    if (P.prior_lse && lane == 0) {
-        const float p = P.prior_lse[row] * LOG2E;
-        if (p != NEG_INF) l += exp2_fast(p - m);
+    if (warp == W - 1 && prior != NEG_INF) {
+        const float f = exp2_fast(prior - m);
+        l += f;
+        const T* po = static_cast<const T*>(P.prior_out) + row * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += f * (float)po[e];
     }
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(FULL, l, x);
-    return make_float2(m, l);
+    for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = acc[e];
+    __shared__ float s_l[W];
+    if (lane == 0) s_l[warp] = l;
+    __syncthreads();
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) sum += s_l[w];
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (threadIdx.x < D) {
+        float y = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) y += s_o[w][threadIdx.x];
+        static_cast<T*>(P.out)[row * D + threadIdx.x] = T(y * inv);
+    }
+    if (threadIdx.x == 0) {
+        const float x = sum == 0.f ? NEG_INF : m + log2f(sum);
+        P.lse[row] = x * LN2;
+        if (P.lse2) P.lse2[row] = x;
+    }
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ Join P) {
-    dependency_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int W = JOIN_THREADS / 32, E = D / 32;
-    if ((int64_t)blockIdx.x < P.rows) {
-        __shared__ float s_o[W][D];
-        const int64_t row = blockIdx.x;
-        const float2 ml = row_total(P, row, lane);
-        float acc[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = 0.f;
-        for (int s = warp; s < P.splits; s += W) {
-            const float2 mine = P.part_ml[row * P.splits + s];
-            if (mine.y == 0.f) continue;      // nothing seen there: its rows are not read
-            const float f = exp2_fast(mine.x - ml.x);
-            const float* po = P.part_out + (row * P.splits + s) * D;
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] += f * po[lane + 32 * e];
-        }
-        if (warp == 0 && P.prior_lse) {
-            const float p = P.prior_lse[row] * LOG2E;
-            if (p != NEG_INF) {
-                const float f = exp2_fast(p - ml.x);
-                const T* po = static_cast<const T*>(P.prior_out) + row * D;
-#pragma unroll
-                for (int e = 0; e < E; ++e) acc[e] += f * (float)po[lane + 32 * e];
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < E; ++e) s_o[warp][lane + 32 * e] = acc[e];
-        __syncthreads();
-        const float inv = ml.y == 0.f ? 0.f : 1.f / ml.y;
-        for (int d = threadIdx.x; d < D; d += JOIN_THREADS) {
-            float y = 0.f;
-#pragma unroll
-            for (int w = 0; w < W; ++w) y += s_o[w][d];
-            static_cast<T*>(P.out)[row * D + d] = T(y * inv);
-        }
-        if (threadIdx.x == 0) P.lse[row] = ml.y == 0.f ? NEG_INF : (ml.x + log2f(ml.y)) * LN2;
-        return;
-    }
-    // the weights of JOIN_SLOTS slots of one key head, summed over its query heads
-    int64_t item = blockIdx.x - P.rows;
+// -- the slots' weights ----------------------------------------------------------
+
+struct Shares {
+    Cache c;
+    int q_heads, group, window, sinks;
+    const float* logits;
+    const float* lse2;
+    float* weights;           // [seqs][kv_heads][width]
+    int64_t width;
+    int accumulate;
+    int chunks;               // blocks of SHARE_SLOTS slots of a row of weights
+};
+
+constexpr int SHARE_THREADS = 256;
+constexpr int SHARE_SLOTS = 1024;
+
+// a slot's share of the softmax, summed over the query heads of its key head
+__global__ void __launch_bounds__(SHARE_THREADS) share_kernel(const __grid_constant__ Shares P) {
+    constexpr int PER = SHARE_SLOTS / SHARE_THREADS;
+    int64_t item = blockIdx.x;
     const int chunk = (int)(item % P.chunks);
     item /= P.chunks;
     const int g = (int)(item % P.c.kv_heads), b = (int)(item / P.c.kv_heads);
     const int far = P.window > 0 ? max(0, P.c.lengths[b] - P.window) : 0;
     const int L = P.c.length(b);
-    float acc[JOIN_SLOTS / JOIN_THREADS];
+    const int64_t s0 = (int64_t)chunk * SHARE_SLOTS + threadIdx.x;
+    float acc[PER];
 #pragma unroll
-    for (int i = 0; i < JOIN_SLOTS / JOIN_THREADS; ++i) acc[i] = 0.f;
-    const int64_t s0 = (int64_t)chunk * JOIN_SLOTS + threadIdx.x;
+    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+    dependency_wait();
+    const int64_t row0 = (int64_t)b * P.q_heads + (int64_t)g * P.group;
+#pragma unroll 4
     for (int h = 0; h < P.group; ++h) {
-        const int64_t row = (int64_t)b * P.q_heads + g * P.group + h;
-        const float2 ml = row_total(P, row, lane);
-        const float lse2 = ml.y == 0.f ? __int_as_float(0x7f800000) : ml.x + log2f(ml.y);
+        const float lse2 = P.lse2[row0 + h];
+        const float off = lse2 == NEG_INF ? 0.f : lse2;             // nothing seen: every logit is -inf
+        const float* x = P.logits + (row0 + h) * P.c.capacity();
 #pragma unroll
-        for (int i = 0; i < JOIN_SLOTS / JOIN_THREADS; ++i) {
-            const int64_t j = s0 + i * JOIN_THREADS;
-            if (j < L && (j >= far || j < P.sinks)) acc[i] += exp2_fast(P.logits[row * P.c.capacity() + j] - lse2);
+        for (int i = 0; i < PER; ++i) {
+            const int64_t j = s0 + i * SHARE_THREADS;
+            if (j < L && (j >= far || j < P.sinks)) acc[i] += exp2_fast(x[j] - off);
         }
     }
     float* w = P.weights + ((int64_t)b * P.c.kv_heads + g) * P.width;
 #pragma unroll
-    for (int i = 0; i < JOIN_SLOTS / JOIN_THREADS; ++i) {
-        const int64_t j = s0 + i * JOIN_THREADS;
+    for (int i = 0; i < PER; ++i) {
+        const int64_t j = s0 + i * SHARE_THREADS;
         if (j < P.width) w[j] = P.accumulate ? w[j] + acc[i] : acc[i];
     }
 }
 
 // -- host side --------------------------------------------------------------
 
-// How many stretches a sequence is cut into: enough CTAs for two rounds of the
-// two that an SM holds, no stretch planned below 256 slots of a full sequence.
-inline int plan_splits(const Cache& c, int64_t tiles) {
-    if (tiles <= 0) return 1;
-    const int64_t want = (4ll * abi::num_sms() + tiles - 1) / tiles;
-    const int64_t most = (c.capacity() + 255) / 256;
-    const int64_t s = want < most ? want : most;
-    return (int)(s < 1 ? 1 : s > 512 ? 512 : s);
+// Whether every pair gets a warp of its own.  With short tables (search results)
+// a run would be many short pairs one after the other, each a chain of dependent
+// reads; a warp a pair has as many chains in flight as the SMs hold warps.  With
+// long ones it needs enough pairs that the last round of unequal lengths is short.
+inline bool warp_a_pair(const Cache& c, int64_t pairs) {
+    const int64_t warps = 8ll * abi::num_sms();
+    return c.capacity() <= 512 ? pairs >= warps / 2 : pairs >= 16 * warps;
 }
 
-template <typename T, int D>
-int launch_walk(const Walk& w, int64_t items, cudaStream_t st) {
-    constexpr int smem = WARPS * STAGES * 2 * KEYS * D * 2;
-    cudaError_t e = cudaFuncSetAttribute(walk_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <typename T, int D, int W>
+int launch_walk(const Walk& w, int64_t ctas, cudaStream_t st) {
+    constexpr int ring = W * STAGES * 2 * KEYS * D * 2, joined = W * ROWS * D * 4;
+    constexpr int smem = ring > joined ? ring : joined;
+    cudaError_t e = cudaFuncSetAttribute(walk_kernel<T, D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return abi::cuda_fail(e, "cudaFuncSetAttribute(attention)");
-    walk_kernel<T, D><<<(unsigned)items, THREADS, smem, st>>>(w);
+    walk_kernel<T, D, W><<<(unsigned)ctas, W * 32, smem, st>>>(w);
     return abi::cuda_check("attention launch");
 }
 
 template <typename T, int D>
-int launch_join(const Join& j, int64_t blocks, cudaStream_t st) {
-    const cudaError_t e = launch_after(join_kernel<T, D>, dim3((unsigned)blocks), dim3(JOIN_THREADS), 0, st, j);
+int launch_decode(const Walk& w, int64_t pairs, cudaStream_t st) {
+    if (!w.runs) return launch_walk<T, D, 1>(w, pairs, st);
+    const int rc = launch_walk<T, D, WARPS>(w, w.runs, st);
+    if (rc || w.runs == 1) return rc;
+    const cudaError_t e = launch_after(join_kernel<T, D>, dim3((unsigned)(w.runs - 1), (unsigned)w.tile_heads),
+                                       dim3(JOIN_THREADS), 0, st, w);
     if (e != cudaSuccess) return abi::cuda_fail(e, "attention join launch");
     return abi::cuda_check("attention join launch");
 }
 
-inline int run_walk(const Walk& w, int64_t items, int dtype, int d, cudaStream_t st) {
-    if (dtype == SWB_F16)
-        return d == 64 ? launch_walk<__half, 64>(w, items, st) : launch_walk<__half, 128>(w, items, st);
-    return d == 64 ? launch_walk<__nv_bfloat16, 64>(w, items, st) : launch_walk<__nv_bfloat16, 128>(w, items, st);
-}
-
-inline int run_join(const Join& j, int64_t blocks, int dtype, int d, cudaStream_t st) {
-    if (dtype == SWB_F16)
-        return d == 64 ? launch_join<__half, 64>(j, blocks, st) : launch_join<__half, 128>(j, blocks, st);
-    return d == 64 ? launch_join<__nv_bfloat16, 64>(j, blocks, st) : launch_join<__nv_bfloat16, 128>(j, blocks, st);
-}
-
-inline Walk make_walk(const Cache& c, const void* q, int64_t ts, int64_t hs, int q_heads, float scale, int window,
-                      int sinks) {
-    Walk w = {};
-    w.c = c;
-    w.q = q;
-    w.q_seq_stride = ts;
-    w.q_head_stride = hs;
-    w.q_heads = q_heads;
-    w.group = q_heads / c.kv_heads;
-    w.tile_heads = w.group < ROWS ? w.group : ROWS;
-    w.head_tiles = (w.group + w.tile_heads - 1) / w.tile_heads;
-    w.splits = 1;
-    w.scale2 = scale * LOG2E;
-    w.window = window;
-    w.sinks = sinks;
-    return w;
-}
-
-struct DecodeSpace {
-    int splits;
-    uint64_t ml, out, logits, total;   // byte offsets
+struct Space {
+    int runs;
+    uint64_t out, ml, lse2, logits, total;   // byte offsets
 };
-inline DecodeSpace decode_space(const Cache& c, int d, int q_heads, bool weights) {
-    DecodeSpace s;
-    const int group = q_heads / c.kv_heads, tiles = (group + ROWS - 1) / ROWS;
-    s.splits = plan_splits(c, (int64_t)c.seqs * c.kv_heads * tiles);
+inline int tiles_of(int group) { return (group + ROWS - 1) / ROWS; }
+inline Space decode_space(const Cache& c, int d, int q_heads, bool weights) {
+    Space s;
+    const int64_t pairs = (int64_t)c.seqs * c.kv_heads * tiles_of(q_heads / c.kv_heads);
+    s.runs = warp_a_pair(c, pairs) ? 0 : cta_per_sm(d) * abi::num_sms();
+    // no more runs than there can be units
+    const int64_t most = pairs * ((c.capacity() + UNIT - 1) / UNIT + 1);
+    if (s.runs > most) s.runs = (int)most;
     const uint64_t rows = (uint64_t)c.seqs * q_heads;
-    const bool join = s.splits > 1 || weights;
     s.out = 0;
-    s.ml = join ? rows * s.splits * d * 4 : 0;
-    s.logits = s.ml + (join ? rows * s.splits * 8 : 0);
+    s.ml = (uint64_t)s.runs * 2 * ROWS * d * 4;
+    s.lse2 = s.ml + (uint64_t)s.runs * 2 * ROWS * 8;
+    s.logits = s.lse2 + (weights ? (rows * 4 + 15) / 16 * 16 : 0);
     s.total = s.logits + (weights ? rows * (uint64_t)c.capacity() * 4 : 0);
     return s;
 }
@@ -510,9 +627,10 @@ extern "C" int swb_attn_decode(const void* q, int64_t q_seq_stride, int64_t q_he
                                const swb_kv_cache* cache, float scale, int window, int sinks, const void* prior_out,
                                const float* prior_lse, void* out, float* lse, float* weights, int64_t weights_width,
                                int accumulate, void* workspace, uint64_t ws_bytes, void* stream) {
-    Cache c;
-    int rc = check_cache(cache, &c);
+    Walk w = {};
+    int rc = check_cache(cache, &w.c);
     if (rc) return rc;
+    const Cache& c = w.c;
     if (c.seqs == 0) return SWB_OK;
     rc = check_query(q, q_seq_stride, q_head_stride, q_heads, c);
     if (rc) return rc;
@@ -522,43 +640,52 @@ extern "C" int swb_attn_decode(const void* q, int64_t q_seq_stride, int64_t q_he
     if (weights && weights_width < c.capacity())
         return abi::fail(SWB_ERR_ARG, "weights are narrower than the page table's slots");
     const int d = cache->head_dim;
-    const DecodeSpace sp = decode_space(c, d, q_heads, weights != nullptr);
+    const Space sp = decode_space(c, d, q_heads, weights != nullptr);
     if (sp.total && (!workspace || ws_bytes < sp.total)) return abi::fail(SWB_ERR_ARG, "workspace too small");
     cudaStream_t st = (cudaStream_t)stream;
     char* ws = static_cast<char*>(workspace);
-    Walk w = make_walk(c, q, q_seq_stride, q_head_stride, q_heads, scale, window, sinks);
-    const int64_t items = (int64_t)c.seqs * c.kv_heads * w.head_tiles * sp.splits;
-    if (items >= ((int64_t)1 << 31)) return abi::fail(SWB_ERR_ARG, "too many sequences in one call");
-    w.splits = sp.splits;
+    w.q = q;
+    w.q_seq_stride = q_seq_stride;
+    w.q_head_stride = q_head_stride;
+    w.q_heads = q_heads;
+    w.group = q_heads / c.kv_heads;
+    w.tile_heads = w.group < ROWS ? w.group : ROWS;
+    w.head_tiles = tiles_of(w.group);
+    w.scale2 = scale * LOG2E;
+    w.window = window;
+    w.sinks = sinks;
     w.prior_out = prior_out;
     w.prior_lse = prior_lse;
     w.out = out;
     w.lse = lse;
+    w.runs = sp.runs;
     w.part_out = reinterpret_cast<float*>(ws + sp.out);
     w.part_ml = reinterpret_cast<float2*>(ws + sp.ml);
+    w.lse2 = weights ? reinterpret_cast<float*>(ws + sp.lse2) : nullptr;
     w.logits = weights ? reinterpret_cast<float*>(ws + sp.logits) : nullptr;
-    rc = run_walk(w, items, cache->dtype, d, st);
-    if (rc || (sp.splits == 1 && !weights)) return rc;
-    Join j = {};
-    j.c = c;
-    j.q_heads = q_heads;
-    j.group = w.group;
-    j.splits = sp.splits;
-    j.rows = (int64_t)c.seqs * q_heads;
-    j.window = window;
-    j.sinks = sinks;
-    j.part_out = w.part_out;
-    j.part_ml = w.part_ml;
-    j.prior_out = prior_out;
-    j.prior_lse = prior_lse;
-    j.out = out;
-    j.lse = lse;
-    j.logits = w.logits;
-    j.weights = weights;
-    j.width = weights_width;
-    j.accumulate = accumulate;
-    j.chunks = (int)((weights_width + JOIN_SLOTS - 1) / JOIN_SLOTS);
-    const int64_t blocks = j.rows + (weights ? (int64_t)c.seqs * c.kv_heads * j.chunks : 0);
-    if (blocks >= ((int64_t)1 << 31)) return abi::fail(SWB_ERR_ARG, "too many sequences in one call");
-    return run_join(j, blocks, cache->dtype, d, st);
+    const int64_t pairs = (int64_t)c.seqs * c.kv_heads * w.head_tiles;
+    const int64_t chunks = (weights_width + SHARE_SLOTS - 1) / SHARE_SLOTS;
+    const int64_t shares = weights ? chunks * c.seqs * c.kv_heads : 0;
+    if (pairs >= ((int64_t)1 << 31) || shares >= ((int64_t)1 << 31))
+        return abi::fail(SWB_ERR_ARG, "too many sequences in one call");
+    if (cache->dtype == SWB_F16)
+        rc = d == 64 ? launch_decode<__half, 64>(w, pairs, st) : launch_decode<__half, 128>(w, pairs, st);
+    else
+        rc = d == 64 ? launch_decode<__nv_bfloat16, 64>(w, pairs, st) : launch_decode<__nv_bfloat16, 128>(w, pairs, st);
+    if (rc || !weights) return rc;
+    Shares h = {};
+    h.c = c;
+    h.q_heads = q_heads;
+    h.group = w.group;
+    h.window = window;
+    h.sinks = sinks;
+    h.logits = w.logits;
+    h.lse2 = w.lse2;
+    h.weights = weights;
+    h.width = weights_width;
+    h.accumulate = accumulate;
+    h.chunks = (int)chunks;
+    const cudaError_t e = launch_after(share_kernel, dim3((unsigned)shares), dim3(SHARE_THREADS), 0, st, h);
+    if (e != cudaSuccess) return abi::cuda_fail(e, "attention weights launch");
+    return abi::cuda_check("attention weights launch");
 }
