@@ -13,11 +13,13 @@
 // One warp owns up to 16 query rows that share a key head (a pair: a sequence
 // and those rows) and walks blocks of 16 keys on its own: keys and values arrive
 // by cp.async in a ring of shared memory stages (128-byte swizzle, rows that are
-// not seen filled with zeros, so nothing that lies in them reaches a product),
-// logits and the weighted sum run on mma.sync with fp32 accumulators (16 rows at
-// most: a tcgen05 tile of 128 would be seven eighths empty, and the tensor pipe
-// is not what bounds this).  Weights are rounded to the cache's 16 bits for the
-// second product, as its other operand is; their sum l is taken before that.
+// not seen filled with zeros, so nothing that lies in them reaches a product).
+// Logits and the weighted sum run on mma.sync with fp32 accumulators, as K Q^T and
+// V^T P^T: keys and dimensions fill the 16 rows of a product and the query rows
+// its 8 columns, so a group of up to 8 heads wastes little (a tcgen05 tile of 128
+// would be nine tenths empty, and the tensor pipe is not what bounds this).
+// Weights are rounded to the cache's 16 bits for the second product, as its other
+// operand is; their sum l is taken before that.
 //
 // Who walks what.  Few pairs: the pairs' units of 64 keys are laid end to end
 // and every CTA of a grid that the SMs hold at once takes an equal run of them,
@@ -31,10 +33,9 @@ namespace swb {
 namespace attn {
 
 constexpr int WARPS = 4;      // of a CTA that takes a run of units
-constexpr int ROWS = 16;      // query rows of a tile
+constexpr int ROWS = 16;      // query rows of a tile, at most
 constexpr int KEYS = 16;      // keys a warp scores at a time
 constexpr int UNIT = WARPS * KEYS;
-constexpr int STAGES = 3;
 
 struct Walk {
     Cache c;
@@ -49,6 +50,8 @@ struct Walk {
     void* out;
     float* lse;
     int runs;                 // CTAs that share the units; 0: a CTA a pair
+    int4* cuts;               // [runs] the pair that run i begins and leaves to others: its first
+                              // output row, rows, parts, first part
     float* part_out;          // [2 * runs][ROWS][D]
     float2* part_ml;          // [2 * runs][ROWS]
     float* logits;            // [seqs * q_heads][capacity], for the weights; null: not wanted
@@ -80,36 +83,27 @@ __device__ __forceinline__ int units_of(const Walk& P, int b) {
     return max(1, (r.n + UNIT - 1) / UNIT);
 }
 
-// The sequences' units laid end to end, counted by all threads of a CTA: thread t
-// sums a stretch of sequences.
-template <int THREADS>
-struct Layout {
-    int64_t before;           // units of a pair row (one key head) ahead of this thread's stretch
-    int64_t mine;
-    int64_t total;            // of all sequences, one key head tile
+// The sequences' units laid end to end, counted by every warp for itself (no
+// barrier): lane t sums a stretch of sequences.
+struct Units {
+    int before, mine;         // units of one head tile ahead of this lane's stretch, and in it
+    int total;                // of one head tile
     int per;                  // sequences of a stretch
-    __device__ __forceinline__ void count(const Walk& P, int64_t* s_sum) {
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        per = (P.c.seqs + THREADS - 1) / THREADS;
-        const int b0 = min(P.c.seqs, (int)threadIdx.x * per), b1 = min(P.c.seqs, b0 + per);
+    __device__ __forceinline__ void count(const Walk& P) {
+        const int lane = threadIdx.x & 31;
+        per = (P.c.seqs + 31) / 32;
+        const int b0 = min(P.c.seqs, lane * per), b1 = min(P.c.seqs, b0 + per);
         mine = 0;
+#pragma unroll 4
         for (int b = b0; b < b1; ++b) mine += units_of(P, b);
-        int64_t sum = mine;
+        int sum = mine;
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) {
-            const int64_t y = __shfl_up_sync(FULL, (long long)sum, s);
+            const int y = __shfl_up_sync(FULL, sum, s);
             if (lane >= s) sum += y;
         }
-        if (lane == 31) s_sum[warp] = sum;
-        __syncthreads();
         before = sum - mine;
-        total = 0;
-#pragma unroll
-        for (int w = 0; w < THREADS / 32; ++w) {
-            before += w < warp ? s_sum[w] : 0;
-            total += s_sum[w];
-        }
-        __syncthreads();
+        total = __shfl_sync(FULL, sum, 31);
     }
 };
 
@@ -119,65 +113,88 @@ struct Spot {
     int unit, units;          // of the pair
 };
 
-// CTA-wide: where unit x of the whole lies.  Sequence-major: all head tiles of a
-// sequence, then the next.
-template <int THREADS>
-__device__ __forceinline__ Spot spot_of(const Walk& P, const Layout<THREADS>& L, int64_t x, Spot* s_spot) {
-    const int tiles = P.c.kv_heads * P.head_tiles;
-    int64_t left = x - L.before * tiles;
-    if (left >= 0 && left < L.mine * tiles) {
-        int b = threadIdx.x * L.per;
-        for (;; ++b) {
-            const int n = units_of(P, b);
-            if (left < (int64_t)n * tiles) {
-                s_spot->b = b;
-                s_spot->h = (int)(left / n);
-                s_spot->unit = (int)(left % n);
-                s_spot->units = n;
-                break;
-            }
-            left -= (int64_t)n * tiles;
+// where unit x of the whole lies, by every warp for itself.  Sequence-major: all
+// head tiles of a sequence, then the next.
+__device__ __forceinline__ Spot spot_of(const Walk& P, const Units& U, int x) {
+    const int tiles = P.c.kv_heads * P.head_tiles, lane = threadIdx.x & 31;
+    int left = x - U.before * tiles;
+    const bool here = left >= 0 && left < U.mine * tiles;
+    Spot at = {0, 0, 0, 1};
+    if (here) {
+        int n;
+        for (at.b = lane * U.per;; ++at.b) {
+            n = units_of(P, at.b);
+            if (left < n * tiles) break;
+            left -= n * tiles;
         }
+        at.units = n;
+        at.h = left / n;
+        at.unit = left - at.h * n;
     }
-    __syncthreads();
-    return *s_spot;
+    const int src = __ffs(__ballot_sync(FULL, here)) - 1;
+    at.b = __shfl_sync(FULL, at.b, src);
+    at.h = __shfl_sync(FULL, at.h, src);
+    at.unit = __shfl_sync(FULL, at.unit, src);
+    at.units = __shfl_sync(FULL, at.units, src);
+    return at;
 }
 
-// CTAs that take a run, and where a run begins
-__device__ __forceinline__ int64_t runs_used(const Walk& P, int64_t all) { return min((int64_t)P.runs, all); }
+// `all` units in `used` runs that differ by one unit at most
+struct Runs {
+    int used, size, more;     // the first `more` runs have size + 1 units
+    __device__ __forceinline__ Runs(int all, int runs) : used(min(runs, all)), size(all / used), more(all - used * size) {}
+    __device__ __forceinline__ int begin(int i) const { return i * size + min(i, more); }
+    __device__ __forceinline__ int owner(int x) const {
+        const int big = more * (size + 1);
+        return x < big ? x / (size + 1) : more + (x - big) / size;
+    }
+};
 
-// CTAs of a run that an SM holds, by their shared memory and registers
-constexpr int cta_per_sm(int d) { return d == 128 ? 2 : 4; }
+// 8 x 8 16-bit elements across a warp, transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 
-template <typename T, int D, int W>
-__global__ void __launch_bounds__(W * 32, W > 1 ? cta_per_sm(D) : 8) walk_kernel(const __grid_constant__ Walk P) {
+// stages of a warp's ring, and CTAs that an SM holds by shared memory and registers
+constexpr int stages_of(int warps) { return warps > 1 ? 3 : 2; }
+constexpr int cta_per_sm(int d, int warps) { return warps > 1 ? (d == 128 ? 2 : 4) : (d == 128 ? 12 : 16); }
+
+// W warps; up to 8 * NT query rows
+template <typename T, int D, int W, int NT>
+__global__ void __launch_bounds__(W * 32, cta_per_sm(D, W)) walk_kernel(const __grid_constant__ Walk P) {
     constexpr int THREADS = W * 32;
     constexpr bool RUNS = W > 1;                       // an equal run of units a CTA, or a pair a warp
+    constexpr int STAGES = stages_of(W);
     constexpr int CH = D / 8;                          // 16-byte chunks of a row
     constexpr int STAGE = 2 * KEYS * D * 2;            // K and V of a block of keys
-    constexpr int NT = D / 8;                          // 8-wide output tiles
+    constexpr int MT = D / 16;                         // 16-high tiles of the dimensions
+    constexpr int R = 8 * NT;
+    constexpr int LD = D + 4;                          // of the joined rows: no two of a warp's stores meet in a bank
     extern __shared__ __align__(128) char smem[];
     __shared__ unsigned s_seen[W][STAGES];
-    __shared__ float s_m[W][ROWS], s_l[W][ROWS];
+    __shared__ float s_m[W][R], s_l[W][R];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
     const uint32_t ring = smem_u32(smem) + warp * (STAGES * STAGE);
+    const int tiles = P.c.kv_heads * P.head_tiles;
 
     // -- which pairs, and which of their keys
     Spot at;
-    int64_t left = 1;                                  // units still to walk
+    int left = 1, x = 0;                               // units still to walk; the next one
+    int all = 1;
     if constexpr (RUNS) {
-        __shared__ int64_t s_sum[W];
-        __shared__ Spot s_spot;
-        Layout<THREADS> lay;
-        lay.count(P, s_sum);
-        const int64_t all = lay.total * P.c.kv_heads * P.head_tiles, used = runs_used(P, all);
-        if (blockIdx.x >= used) return;
-        const int64_t x0 = all * blockIdx.x / used;
-        left = all * (blockIdx.x + 1) / used - x0;
-        at = spot_of(P, lay, x0, &s_spot);
+        Units U;
+        U.count(P);
+        const Runs runs(U.total * tiles, P.runs);
+        const int i = blockIdx.x;
+        if (threadIdx.x == 0) P.cuts[i] = make_int4(0, 0, 0, 0);
+        if (i >= runs.used) return;
+        x = runs.begin(i);
+        left = runs.begin(i + 1) - x;
+        at = spot_of(P, U, x);
+        all = U.total * tiles;
     } else {
-        const int tiles = P.c.kv_heads * P.head_tiles;
         at.b = (int)(blockIdx.x / tiles);
         at.h = (int)(blockIdx.x % tiles);
         at.unit = 0;
@@ -185,236 +202,251 @@ __global__ void __launch_bounds__(W * 32, W > 1 ? cta_per_sm(D) : 8) walk_kernel
     }
 
     for (bool first = true; left > 0; first = false) {
-    const int b = at.b, g = at.h / P.head_tiles, ht = at.h % P.head_tiles;
-    const int heads = min(P.tile_heads, P.group - ht * P.tile_heads);
-    const int64_t row0 = (int64_t)b * P.q_heads + g * P.group + ht * P.tile_heads;   // first output row
-    const Range rg = visible(P.c.lengths[b] - 1, P.window, P.sinks, P.c.capacity());
-    const int take = (int)min(left, (int64_t)(at.units - at.unit));
-    const int u0 = RUNS ? min(rg.n, at.unit * UNIT) : 0, u1 = RUNS ? min(rg.n, u0 + take * UNIT) : rg.n;
-    const bool entire = take == at.units;              // nothing of the pair is left to others
-    const int nblk = (u1 - u0 + KEYS - 1) / KEYS;      // blocks of the stretch; warp w has w, w + W, ..
-    const int mine = nblk > warp ? (nblk - warp - 1) / W + 1 : 0;
+        const int b = at.b, g = at.h / P.head_tiles, ht = at.h % P.head_tiles;
+        const int heads = min(P.tile_heads, P.group - ht * P.tile_heads);
+        const int64_t row0 = (int64_t)b * P.q_heads + g * P.group + ht * P.tile_heads;   // first output row
+        const Range rg = visible(P.c.lengths[b] - 1, P.window, P.sinks, P.c.capacity());
+        const int take = min(left, at.units - at.unit);
+        const int u0 = RUNS ? min(rg.n, at.unit * UNIT) : 0, u1 = RUNS ? min(rg.n, u0 + take * UNIT) : rg.n;
+        const bool entire = take == at.units;          // nothing of the pair is left to others
+        const int nblk = (u1 - u0 + KEYS - 1) / KEYS;  // blocks of the stretch; warp w has w, w + W, ..
+        const int mine = nblk > warp ? (nblk - warp - 1) / W + 1 : 0;
 
-    // -- the query rows as matrix fragments: row r is head r of the tile
-    const T* q = static_cast<const T*>(P.q) + b * P.q_seq_stride + (int64_t)(g * P.group + ht * P.tile_heads) * P.q_head_stride;
-    const int r0 = lane >> 2, r1 = r0 + 8;
-    const bool ok0 = r0 < heads, ok1 = r1 < heads;
-    const T* q0 = q + r0 * P.q_head_stride;
-    const T* q1 = q + r1 * P.q_head_stride;
-    uint32_t qf[D / 16][4];
+        const T* kp = static_cast<const T*>(P.c.k) + (int64_t)g * P.c.head_stride;
+        const T* vp = static_cast<const T*>(P.c.v) + (int64_t)g * P.c.head_stride;
+        // lane < 16: the row of key `lane` of this warp's block i, or -1
+        auto find = [&](int i) -> int64_t {
+            const int u = u0 + (i * W + warp) * KEYS + lane;
+            return (lane < KEYS && i < mine && u < u1) ? P.c.row(b, rg.slot(u)) : -1;
+        };
+        auto issue = [&](int i, int64_t off) {
+            const uint32_t st = ring + (i % STAGES) * STAGE;
+            if (i < mine) {
+                const unsigned seen = __ballot_sync(FULL, off >= 0);
+                if (lane == 0) s_seen[warp][i % STAGES] = seen;
 #pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-        const int c = kk * 16 + (lane & 3) * 2;
-        qf[kk][0] = ok0 ? *reinterpret_cast<const uint32_t*>(q0 + c) : 0u;
-        qf[kk][1] = ok1 ? *reinterpret_cast<const uint32_t*>(q1 + c) : 0u;
-        qf[kk][2] = ok0 ? *reinterpret_cast<const uint32_t*>(q0 + c + 8) : 0u;
-        qf[kk][3] = ok1 ? *reinterpret_cast<const uint32_t*>(q1 + c + 8) : 0u;
-    }
-    float* lg0 = P.logits && ok0 ? P.logits + (row0 + r0) * P.c.capacity() : nullptr;
-    float* lg1 = P.logits && ok1 ? P.logits + (row0 + r1) * P.c.capacity() : nullptr;
+                for (int it = 0; it < KEYS * CH / 32; ++it) {
+                    const int r = (it * 32 + lane) / CH, c = (it * 32 + lane) % CH;
+                    const int64_t o = __shfl_sync(FULL, (long long)off, r);
+                    const bool real = o >= 0;
+                    const int64_t e = real ? o + c * 8 : 0;
+                    cp_async16_or_zero(st + swz<D>(r, c), kp + e, real);
+                    cp_async16_or_zero(st + KEYS * D * 2 + swz<D>(r, c), vp + e, real);
+                }
+            }
+            cp_async_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; ++i) issue(i, find(i));
+        int64_t next = find(STAGES - 1);
 
-    const T* kp = static_cast<const T*>(P.c.k) + (int64_t)g * P.c.head_stride;
-    const T* vp = static_cast<const T*>(P.c.v) + (int64_t)g * P.c.head_stride;
-    // lane < 16: the row of key `lane` of this warp's block i, or -1
-    auto find = [&](int i) -> int64_t {
-        const int u = u0 + (i * W + warp) * KEYS + lane;
-        return (lane < KEYS && i < mine && u < u1) ? P.c.row(b, rg.slot(u)) : -1;
-    };
-    auto issue = [&](int i, int64_t off) {
-        const uint32_t st = ring + (i % STAGES) * STAGE;
-        if (i < mine) {
-            const unsigned seen = __ballot_sync(FULL, off >= 0);
-            if (lane == 0) s_seen[warp][i % STAGES] = seen;
+        // -- the query rows as fragments of the second operand: column r is head r of the tile
+        const T* q = static_cast<const T*>(P.q) + b * P.q_seq_stride +
+                     (int64_t)(g * P.group + ht * P.tile_heads) * P.q_head_stride;
+        uint32_t qf[D / 16][NT][2];
 #pragma unroll
-            for (int it = 0; it < KEYS * CH / 32; ++it) {
-                const int r = (it * 32 + lane) / CH, c = (it * 32 + lane) % CH;
-                const int64_t o = __shfl_sync(FULL, (long long)off, r);
-                const bool real = o >= 0;
-                const int64_t e = real ? o + c * 8 : 0;
-                cp_async16_or_zero(st + swz<D>(r, c), kp + e, real);
-                cp_async16_or_zero(st + KEYS * D * 2 + swz<D>(r, c), vp + e, real);
+        for (int n = 0; n < NT; ++n) {
+            const int r = n * 8 + (lane >> 2);
+            const T* qr = q + r * P.q_head_stride + (lane & 3) * 2;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                qf[kk][n][0] = r < heads ? *reinterpret_cast<const uint32_t*>(qr + kk * 16) : 0u;
+                qf[kk][n][1] = r < heads ? *reinterpret_cast<const uint32_t*>(qr + kk * 16 + 8) : 0u;
             }
         }
-        cp_async_commit();
-    };
 
-    float o[NT][4];
+        // this thread's columns: heads n * 8 + (lane & 3) * 2 + e
+        float o[MT][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
-    float m0 = NEG_INF, m1 = NEG_INF, l0 = 0.f, l1 = 0.f;
-
+            for (int j = 0; j < MT; ++j)
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) issue(i, find(i));
-    int64_t next = find(STAGES - 1);
-    for (int i = 0; i < mine; ++i) {
-        cp_async_wait<STAGES - 2>();
-        __syncwarp();
-        issue(i + STAGES - 1, next);      // the stage that block i - 1 has left
-        next = find(i + STAGES);
-        const uint32_t st = ring + (i % STAGES) * STAGE;
-        const unsigned seen = s_seen[warp][i % STAGES];
-
-        float x[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[n][e] = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-            uint32_t f[4];
-            ldmatrix4(f, st + swz<D>((lane >> 4) * 8 + (lane & 7), 2 * kk + ((lane >> 3) & 1)));
-            Elem<T>::mma(x[0], qf[kk], f[0], f[1]);
-            Elem<T>::mma(x[1], qf[kk], f[2], f[3]);
+                for (int e = 0; e < 4; ++e) o[j][n][e] = 0.f;
+            m[n][0] = m[n][1] = NEG_INF;
+            l[n][0] = l[n][1] = 0.f;
         }
-        const int ub = u0 + (i * W + warp) * KEYS;
+        for (int i = 0; i < mine; ++i) {
+            cp_async_wait<STAGES - 2>();
+            __syncwarp();
+            issue(i + STAGES - 1, next);      // into the stage that block i - 1 has left
+            next = find(i + STAGES);
+            const uint32_t st = ring + (i % STAGES) * STAGE;
+            const unsigned seen = s_seen[warp][i % STAGES];
+
+            float y[NT][4];
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int kx = n * 8 + (lane & 3) * 2 + (e & 1);
-                x[n][e] = (seen >> kx) & 1u ? x[n][e] * P.scale2 : NEG_INF;
-                float* lg = e < 2 ? lg0 : lg1;
-                if (lg && ub + kx < u1) lg[rg.slot(ub + kx)] = x[n][e];
+                for (int e = 0; e < 4; ++e) y[n][e] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                uint32_t f[4];
+                ldmatrix4(f, st + swz<D>(((lane >> 3) & 1) * 8 + (lane & 7), 2 * kk + (lane >> 4)));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) Elem<T>::mma(y[n], f, qf[kk][n][0], qf[kk][n][1]);
             }
-        float a0 = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
-        float a1 = fmaxf(fmaxf(x[0][2], x[0][3]), fmaxf(x[1][2], x[1][3]));
+            const int k0 = lane >> 2;         // this thread's keys: k0 and k0 + 8
+            const bool see0 = (seen >> k0) & 1u, see1 = (seen >> (k0 + 8)) & 1u;
 #pragma unroll
-        for (int s = 1; s <= 2; s <<= 1) {
-            a0 = fmaxf(a0, __shfl_xor_sync(FULL, a0, s));
-            a1 = fmaxf(a1, __shfl_xor_sync(FULL, a1, s));
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[n][e] = (e < 2 ? see0 : see1) ? y[n][e] * P.scale2 : NEG_INF;
+            if (P.logits) {
+                const int u = u0 + (i * W + warp) * KEYS + k0;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = n * 8 + (lane & 3) * 2 + (e & 1), v = u + (e < 2 ? 0 : 8);
+                        if (r < heads && v < u1) P.logits[(row0 + r) * P.c.capacity() + rg.slot(v)] = y[n][e];
+                    }
+            }
+            bool grows = false;
+            float a[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    a[n][e] = fmaxf(y[n][e], y[n][e + 2]);
+#pragma unroll
+                    for (int s = 4; s <= 16; s <<= 1) a[n][e] = fmaxf(a[n][e], __shfl_xor_sync(FULL, a[n][e], s));
+                    grows = grows || a[n][e] > m[n][e];
+                }
+            if (__any_sync(FULL, grows)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float f[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float t = fmaxf(m[n][e], a[n][e]);
+                        f[e] = t == NEG_INF ? 1.f : exp2_fast(m[n][e] - t);
+                        m[n][e] = t;
+                        l[n][e] *= f[e];
+                    }
+#pragma unroll
+                    for (int j = 0; j < MT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[j][n][e] *= f[e & 1];
+                }
+            }
+            uint32_t pf[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float s0 = m[n][0] == NEG_INF ? 0.f : m[n][0], s1 = m[n][1] == NEG_INF ? 0.f : m[n][1];
+                const float w0 = exp2_fast(y[n][0] - s0), w1 = exp2_fast(y[n][1] - s1);
+                const float w2 = exp2_fast(y[n][2] - s0), w3 = exp2_fast(y[n][3] - s1);
+                l[n][0] += w0 + w2;
+                l[n][1] += w1 + w3;
+                pf[n][0] = transposed(Elem<T>::pack(w0, w1));
+                pf[n][1] = transposed(Elem<T>::pack(w2, w3));
+            }
+            const uint32_t sv = st + KEYS * D * 2;
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+                uint32_t f[4];
+                ldmatrix4_t(f, sv + swz<D>((lane >> 4) * 8 + (lane & 7), 2 * j + ((lane >> 3) & 1)));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) Elem<T>::mma(o[j][n], f, pf[n][0], pf[n][1]);
+            }
+            __syncwarp();
         }
-        if (__any_sync(FULL, a0 > m0 || a1 > m1)) {
-            const float n0 = fmaxf(m0, a0), n1 = fmaxf(m1, a1);
-            const float f0 = n0 == NEG_INF ? 1.f : exp2_fast(m0 - n0), f1 = n1 == NEG_INF ? 1.f : exp2_fast(m1 - n1);
-            m0 = n0;
-            m1 = n1;
-            l0 *= f0;
-            l1 *= f1;
+        cp_async_wait<0>();
+
+        // -- join the warps
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                o[j][0] *= f0;
-                o[j][1] *= f0;
-                o[j][2] *= f1;
-                o[j][3] *= f1;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int s = 4; s <= 16; s <<= 1) l[n][e] += __shfl_xor_sync(FULL, l[n][e], s);
+                if (lane < 4) {
+                    s_m[warp][n * 8 + lane * 2 + e] = m[n][e];
+                    s_l[warp][n * 8 + lane * 2 + e] = l[n][e];
+                }
+            }
+        __syncthreads();      // the ring is free too
+        float* so = reinterpret_cast<float*>(smem);    // [W][R][LD]
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = n * 8 + (lane & 3) * 2 + e;
+                float top = NEG_INF;
+#pragma unroll
+                for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w][r]);
+                const float f = l[n][e] == 0.f ? 0.f : exp2_fast(m[n][e] - top);
+                float* dst = so + (warp * R + r) * LD + (lane >> 2);
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    dst[j * 16] = o[j][n][e] * f;
+                    dst[j * 16 + 8] = o[j][n][e + 2] * f;
+                }
+            }
+        __syncthreads();
+        for (int i = threadIdx.x; i < heads * (D / 4); i += THREADS) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            float top = NEG_INF, sum = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w][r]);
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                if (s_l[w][r] != 0.f) sum += s_l[w][r] * exp2_fast(s_m[w][r] - top);
+                const float4 z = *reinterpret_cast<const float4*>(so + (w * R + r) * LD + d);
+                acc.x += z.x;
+                acc.y += z.y;
+                acc.z += z.z;
+                acc.w += z.w;
+            }
+            if (!entire) {
+                const int64_t part = (2 * (int64_t)blockIdx.x + (first ? 0 : 1)) * ROWS + r;
+                *reinterpret_cast<float4*>(P.part_out + part * D + d) = acc;
+                if (d == 0) P.part_ml[part] = make_float2(top, sum);
+                continue;
+            }
+            // the whole pair: this is the answer, up to the prior part
+            const int64_t row = row0 + r;
+            const float pm = P.prior_lse ? P.prior_lse[row] * LOG2E : NEG_INF;
+            const float most = fmaxf(top, pm);
+            const float fa = sum == 0.f ? 0.f : exp2_fast(top - most), fb = pm == NEG_INF ? 0.f : exp2_fast(pm - most);
+            const float whole = sum * fa + fb;
+            const float inv = whole == 0.f ? 0.f : 1.f / whole;
+            acc = make_float4(acc.x * fa, acc.y * fa, acc.z * fa, acc.w * fa);
+            if (pm != NEG_INF) {
+                const uint2 z = *reinterpret_cast<const uint2*>(static_cast<const T*>(P.prior_out) + row * D + d);
+                const float2 z0 = Elem<T>::wide(z.x), z1 = Elem<T>::wide(z.y);
+                acc.x += fb * z0.x;
+                acc.y += fb * z0.y;
+                acc.z += fb * z1.x;
+                acc.w += fb * z1.y;
+            }
+            *reinterpret_cast<uint2*>(static_cast<T*>(P.out) + row * D + d) =
+                make_uint2(Elem<T>::pack(acc.x * inv, acc.y * inv), Elem<T>::pack(acc.z * inv, acc.w * inv));
+            if (d == 0) {
+                const float z = whole == 0.f ? NEG_INF : most + log2f(whole);
+                P.lse[row] = z * LN2;
+                if (P.lse2) P.lse2[row] = z;
             }
         }
-        const float s0 = m0 == NEG_INF ? 0.f : m0, s1 = m1 == NEG_INF ? 0.f : m1;
-        uint32_t pf[4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const float w0 = exp2_fast(x[n][0] - s0), w1 = exp2_fast(x[n][1] - s0);
-            const float w2 = exp2_fast(x[n][2] - s1), w3 = exp2_fast(x[n][3] - s1);
-            l0 += w0 + w1;
-            l1 += w2 + w3;
-            pf[2 * n] = Elem<T>::pack(w0, w1);
-            pf[2 * n + 1] = Elem<T>::pack(w2, w3);
+        if constexpr (RUNS) {
+            if (!entire && at.unit == 0 && threadIdx.x == 0) {
+                // the pair begins here and goes on in the runs that follow
+                const int last = Runs(all, P.runs).owner(x + at.units - 1);
+                P.cuts[blockIdx.x] = make_int4((int)row0, heads, last - (int)blockIdx.x + 1, 2 * blockIdx.x + (first ? 0 : 1));
+            }
         }
-        const uint32_t sv = st + KEYS * D * 2;
-#pragma unroll
-        for (int j = 0; j < NT / 2; ++j) {
-            uint32_t f[4];
-            ldmatrix4_t(f, sv + swz<D>(((lane >> 3) & 1) * 8 + (lane & 7), 2 * j + (lane >> 4)));
-            Elem<T>::mma(o[2 * j], pf, f[0], f[1]);
-            Elem<T>::mma(o[2 * j + 1], pf, f[2], f[3]);
+        left -= take;
+        x += take;
+        if (left > 0) {
+            at.unit = 0;
+            if (++at.h == tiles) {
+                at.h = 0;
+                ++at.b;
+                at.units = units_of(P, at.b);
+            }
+            __syncthreads();      // the joined rows have been read: the ring is free
         }
-        __syncwarp();
-    }
-    cp_async_wait<0>();
-#pragma unroll
-    for (int s = 1; s <= 2; s <<= 1) {
-        l0 += __shfl_xor_sync(FULL, l0, s);
-        l1 += __shfl_xor_sync(FULL, l1, s);
-    }
-
-    // -- join the warps
-    if ((lane & 3) == 0) {
-        s_m[warp][r0] = m0;
-        s_m[warp][r1] = m1;
-        s_l[warp][r0] = l0;
-        s_l[warp][r1] = l1;
-    }
-    __syncthreads();      // the ring is free too
-    float M0 = NEG_INF, M1 = NEG_INF;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-        M0 = fmaxf(M0, s_m[w][r0]);
-        M1 = fmaxf(M1, s_m[w][r1]);
-    }
-    const float f0 = l0 == 0.f ? 0.f : exp2_fast(m0 - M0), f1 = l1 == 0.f ? 0.f : exp2_fast(m1 - M1);
-    float* so = reinterpret_cast<float*>(smem);       // [W][ROWS][D]
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const int c = j * 8 + (lane & 3) * 2;
-        *reinterpret_cast<float2*>(so + (warp * ROWS + r0) * D + c) = make_float2(o[j][0] * f0, o[j][1] * f0);
-        *reinterpret_cast<float2*>(so + (warp * ROWS + r1) * D + c) = make_float2(o[j][2] * f1, o[j][3] * f1);
-    }
-    __syncthreads();
-    constexpr int TPR = THREADS / ROWS;                // threads of a row
-    constexpr int DPT = D / TPR;                       // dimensions of a thread
-    const int r = threadIdx.x / TPR, d0 = (threadIdx.x % TPR) * 2;
-    if (r < heads) {
-    float M = NEG_INF, l = 0.f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) M = fmaxf(M, s_m[w][r]);
-#pragma unroll
-    for (int w = 0; w < W; ++w)
-        if (s_l[w][r] != 0.f) l += s_l[w][r] * exp2_fast(s_m[w][r] - M);
-    const int64_t row = row0 + r;
-    float2 acc[DPT / 2];
-#pragma unroll
-    for (int i = 0; i < DPT / 2; ++i) {
-        acc[i] = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const float2 y = *reinterpret_cast<const float2*>(so + (w * ROWS + r) * D + d0 + i * 2 * TPR);
-            acc[i].x += y.x;
-            acc[i].y += y.y;
-        }
-    }
-    if (!entire) {
-        const int64_t part = 2 * (int64_t)blockIdx.x + (first ? 0 : 1);
-        float* po = P.part_out + (part * ROWS + r) * D;
-#pragma unroll
-        for (int i = 0; i < DPT / 2; ++i) *reinterpret_cast<float2*>(po + d0 + i * 2 * TPR) = acc[i];
-        if (threadIdx.x % TPR == 0) P.part_ml[part * ROWS + r] = make_float2(M, l);
-    } else {
-    // the whole pair: this is the answer, up to the prior part
-    float pm = P.prior_lse ? P.prior_lse[row] * LOG2E : NEG_INF;
-    const float top = fmaxf(M, pm);
-    const float fa = l == 0.f ? 0.f : exp2_fast(M - top), fb = pm == NEG_INF ? 0.f : exp2_fast(pm - top);
-    const float sum = l * fa + fb;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<T*>(P.out) + row * D);
-    const uint32_t* po = fb > 0.f ? reinterpret_cast<const uint32_t*>(static_cast<const T*>(P.prior_out) + row * D) : nullptr;
-#pragma unroll
-    for (int i = 0; i < DPT / 2; ++i) {
-        float2 y = make_float2(acc[i].x * fa, acc[i].y * fa);
-        if (po) {
-            const float2 z = Elem<T>::wide(po[(d0 + i * 2 * TPR) / 2]);
-            y.x += fb * z.x;
-            y.y += fb * z.y;
-        }
-        out[(d0 + i * 2 * TPR) / 2] = Elem<T>::pack(y.x * inv, y.y * inv);
-    }
-    if (threadIdx.x % TPR == 0) {
-        const float x = sum == 0.f ? NEG_INF : top + log2f(sum);
-        P.lse[row] = x * LN2;
-        if (P.lse2) P.lse2[row] = x;
-    }
-    }
-    }
-    left -= take;
-    at.unit = 0;
-    if (left > 0) {
-        if (++at.h == P.c.kv_heads * P.head_tiles) {
-            at.h = 0;
-            ++at.b;
-            at.units = units_of(P, at.b);
-        }
-        __syncthreads();      // the joined rows have been read: the ring is free
-    }
     }
 }
 
@@ -422,45 +454,31 @@ __global__ void __launch_bounds__(W * 32, W > 1 ? cta_per_sm(D) : 8) walk_kernel
 
 constexpr int JOIN_THREADS = 256;
 
-// CTA (i, r): row r of the pair that the end of run i cuts, if no earlier end cuts it
+// CTA (i, r): row r of the pair that run i begins and others go on with, if any
 template <typename T, int D>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ Walk P) {
     constexpr int W = JOIN_THREADS / 32, E = D / 32;
-    __shared__ int64_t s_sum[W];
-    __shared__ Spot s_spot;
-    __shared__ float s_o[W][D];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y;
-    Layout<JOIN_THREADS> lay;
-    lay.count(P, s_sum);       // lengths are not what the kernel before this one writes
-    const int64_t all = lay.total * P.c.kv_heads * P.head_tiles, used = runs_used(P, all);
-    const int64_t i = blockIdx.x, cut = all * (i + 1) / used;
-    const bool inside = i + 1 < used;
-    const Spot at = spot_of(P, lay, inside ? cut : 0, &s_spot);
+    __shared__ float s_o[W][D], s_l[W];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = blockIdx.x, r = blockIdx.y;
     // every CTA waits, also those without work: a kernel after this one may then
     // rely on the one before it
     dependency_wait();
-    if (!inside || at.unit == 0) return;                                       // the cut lies between two pairs
-    const int64_t p0 = cut - at.unit, p1 = p0 + at.units;           // the pair's units
-    if (p0 < all * i / used) return;                                // run i does not begin it: an earlier cut has it
-    const int g = at.h / P.head_tiles, ht = at.h % P.head_tiles;
-    if (r >= min(P.tile_heads, P.group - ht * P.tile_heads)) return;
-    const int64_t row = (int64_t)at.b * P.q_heads + g * P.group + ht * P.tile_heads + r;
-    // runs i .. i + n - 1 hold parts: run i in its first place if the pair begins it, else in its second
-    int64_t n = 1;
-    while (all * (i + n) / used < p1) ++n;
-    const int64_t part0 = 2 * i + (all * i / used == p0 ? 0 : 1);
+    const int4 cut = P.cuts[i];
+    if (r >= cut.y) return;
+    const int64_t row = (int64_t)cut.x + r;
+    const int n = cut.z, part0 = cut.w;
 
     const float prior = P.prior_lse ? P.prior_lse[row] * LOG2E : NEG_INF;
     float m = prior;
-    for (int64_t s = lane; s < n; s += 32) m = fmaxf(m, P.part_ml[(s ? 2 * (i + s) : part0) * ROWS + r].x);
+    for (int s = lane; s < n; s += 32) m = fmaxf(m, P.part_ml[(int64_t)(s ? 2 * (i + s) : part0) * ROWS + r].x);
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, x));
     float l = 0.f, acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
 #pragma unroll 4
-    for (int64_t s = warp; s < n; s += W) {
-        const int64_t part = (s ? 2 * (i + s) : part0) * ROWS + r;
+    for (int s = warp; s < n; s += W) {
+        const int64_t part = (int64_t)(s ? 2 * (i + s) : part0) * ROWS + r;
         const float2 ml = P.part_ml[part];
         float x[E];
         if constexpr (E == 4) {
@@ -488,7 +506,6 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constan
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = acc[e];
-    __shared__ float s_l[W];
     if (lane == 0) s_l[warp] = l;
     __syncthreads();
     float sum = 0.f;
@@ -569,20 +586,21 @@ inline bool warp_a_pair(const Cache& c, int64_t pairs) {
     return c.capacity() <= 512 ? pairs >= warps / 2 : pairs >= 16 * warps;
 }
 
-template <typename T, int D, int W>
+template <typename T, int D, int W, int NT>
 int launch_walk(const Walk& w, int64_t ctas, cudaStream_t st) {
-    constexpr int ring = W * STAGES * 2 * KEYS * D * 2, joined = W * ROWS * D * 4;
+    constexpr int ring = W * stages_of(W) * 2 * KEYS * D * 2, joined = W * 8 * NT * (D + 4) * 4;
     constexpr int smem = ring > joined ? ring : joined;
-    cudaError_t e = cudaFuncSetAttribute(walk_kernel<T, D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = cudaFuncSetAttribute(walk_kernel<T, D, W, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return abi::cuda_fail(e, "cudaFuncSetAttribute(attention)");
-    walk_kernel<T, D, W><<<(unsigned)ctas, W * 32, smem, st>>>(w);
+    walk_kernel<T, D, W, NT><<<(unsigned)ctas, W * 32, smem, st>>>(w);
     return abi::cuda_check("attention launch");
 }
 
 template <typename T, int D>
 int launch_decode(const Walk& w, int64_t pairs, cudaStream_t st) {
-    if (!w.runs) return launch_walk<T, D, 1>(w, pairs, st);
-    const int rc = launch_walk<T, D, WARPS>(w, w.runs, st);
+    const bool wide = w.tile_heads > 8;
+    if (!w.runs) return wide ? launch_walk<T, D, 1, 2>(w, pairs, st) : launch_walk<T, D, 1, 1>(w, pairs, st);
+    const int rc = wide ? launch_walk<T, D, WARPS, 2>(w, w.runs, st) : launch_walk<T, D, WARPS, 1>(w, w.runs, st);
     if (rc || w.runs == 1) return rc;
     const cudaError_t e = launch_after(join_kernel<T, D>, dim3((unsigned)(w.runs - 1), (unsigned)w.tile_heads),
                                        dim3(JOIN_THREADS), 0, st, w);
@@ -592,20 +610,21 @@ int launch_decode(const Walk& w, int64_t pairs, cudaStream_t st) {
 
 struct Space {
     int runs;
-    uint64_t out, ml, lse2, logits, total;   // byte offsets
+    uint64_t out, ml, cuts, lse2, logits, total;   // byte offsets
 };
 inline int tiles_of(int group) { return (group + ROWS - 1) / ROWS; }
 inline Space decode_space(const Cache& c, int d, int q_heads, bool weights) {
     Space s;
     const int64_t pairs = (int64_t)c.seqs * c.kv_heads * tiles_of(q_heads / c.kv_heads);
-    s.runs = warp_a_pair(c, pairs) ? 0 : cta_per_sm(d) * abi::num_sms();
+    s.runs = warp_a_pair(c, pairs) ? 0 : cta_per_sm(d, WARPS) * abi::num_sms();
     // no more runs than there can be units
     const int64_t most = pairs * ((c.capacity() + UNIT - 1) / UNIT + 1);
     if (s.runs > most) s.runs = (int)most;
     const uint64_t rows = (uint64_t)c.seqs * q_heads;
     s.out = 0;
     s.ml = (uint64_t)s.runs * 2 * ROWS * d * 4;
-    s.lse2 = s.ml + (uint64_t)s.runs * 2 * ROWS * 8;
+    s.cuts = s.ml + (uint64_t)s.runs * 2 * ROWS * 8;
+    s.lse2 = s.cuts + (uint64_t)s.runs * 16;
     s.logits = s.lse2 + (weights ? (rows * 4 + 15) / 16 * 16 : 0);
     s.total = s.logits + (weights ? rows * (uint64_t)c.capacity() * 4 : 0);
     return s;
@@ -661,12 +680,15 @@ extern "C" int swb_attn_decode(const void* q, int64_t q_seq_stride, int64_t q_he
     w.runs = sp.runs;
     w.part_out = reinterpret_cast<float*>(ws + sp.out);
     w.part_ml = reinterpret_cast<float2*>(ws + sp.ml);
+    w.cuts = reinterpret_cast<int4*>(ws + sp.cuts);
     w.lse2 = weights ? reinterpret_cast<float*>(ws + sp.lse2) : nullptr;
     w.logits = weights ? reinterpret_cast<float*>(ws + sp.logits) : nullptr;
     const int64_t pairs = (int64_t)c.seqs * c.kv_heads * w.head_tiles;
+    const int64_t rows = (int64_t)c.seqs * q_heads;
     const int64_t chunks = (weights_width + SHARE_SLOTS - 1) / SHARE_SLOTS;
     const int64_t shares = weights ? chunks * c.seqs * c.kv_heads : 0;
-    if (pairs >= ((int64_t)1 << 31) || shares >= ((int64_t)1 << 31))
+    // units, output rows and cuts are counted in 32 bits
+    if (pairs * ((c.capacity() + UNIT - 1) / UNIT + 1) >= ((int64_t)1 << 31) || rows >= ((int64_t)1 << 31) || shares >= ((int64_t)1 << 31))
         return abi::fail(SWB_ERR_ARG, "too many sequences in one call");
     if (cache->dtype == SWB_F16)
         rc = d == 64 ? launch_decode<__half, 64>(w, pairs, st) : launch_decode<__half, 128>(w, pairs, st);
