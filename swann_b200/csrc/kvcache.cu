@@ -11,10 +11,13 @@
 // swb_kv_evict: per key head, the `budget` slots with the largest accumulated
 // weight stay (first and newest positions before all), and rows that lie beyond
 // the budget move to the places that became free below it.  A slot's key is its
-// weight's bits in an order that compares as the numbers do; four counting passes
-// over 8 bits each find the budget-th largest key, and one pass in slot order
+// weight's bits in an order that compares as the numbers do; three counting passes
+// (11, 11 and 10 bits) find the budget-th largest key, and a pass in slot order
 // splits the slots into those that stay, the free and the ones to move.  Counts
-// and order are whole numbers: the result does not depend on timing.
+// and order are whole numbers: the result does not depend on timing.  A CTA a key
+// head; each of its warps has a contiguous piece of the slots, so ranks need
+// ballots and one sum over warps.  The moved rows' bytes bound it when many move;
+// one row moves in a step of one token, and then it is the chain of passes.
 
 #include "attn.cuh"
 
@@ -46,112 +49,122 @@ struct Append {
     int64_t width;
 };
 
-constexpr int APPEND_THREADS = 256;
+constexpr int APPEND_THREADS = 128;
+constexpr int APPEND_HEADS = 4;      // heads of a thread, their loads in flight together
 
+// A token, and APPEND_HEADS * (128 threads / lanes of a head) of its heads, a
+// CTA: a thread has the same chunk of each of its heads, so the token's place and
+// its rotation are read once.
 template <typename T, int D>
 __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const __grid_constant__ Append P) {
-    constexpr int LPH = D / 8;
-    const int heads = P.q_heads + 2 * P.c.kv_heads;
-    const int64_t at = (int64_t)blockIdx.x * APPEND_THREADS + threadIdx.x;
-    const int64_t item = at / LPH;
-    const int c = (int)(at % LPH);
-    const int64_t tok = item / heads;
-    const int h = (int)(item % heads);
-    const bool live = tok < P.tokens;      // whole heads: the shuffles below stay inside one
+    constexpr int LPH = D / 8, HP = APPEND_THREADS / LPH, U = APPEND_HEADS;
+    const int heads = P.q_heads + 2 * P.c.kv_heads, keys = P.q_heads, values = P.q_heads + P.c.kv_heads;
+    const int64_t tok = blockIdx.x;
+    const int c = threadIdx.x % LPH;
+    const int h0 = blockIdx.y * (HP * U) + threadIdx.x / LPH;
+
+    uint4 raw[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int h = h0 + i * HP;
+        const T* src = h < keys ? static_cast<const T*>(P.q) + tok * P.q_ts + h * P.q_hs
+                     : h < values ? static_cast<const T*>(P.k) + tok * P.k_ts + (h - keys) * P.k_hs
+                                  : static_cast<const T*>(P.v) + tok * P.v_ts + (h - values) * P.v_hs;
+        raw[i] = h < heads ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u);
+    }
 
     // the token's sequence: the last one that starts at or before it
-    int b = 0;
-    if (live) {
-        int hi = P.c.seqs;
-        while (hi - b > 1) {
-            const int mid = (b + hi) >> 1;
-            if (P.starts[mid] <= tok) b = mid;
-            else hi = mid;
-        }
+    int b = 0, hi = P.c.seqs;
+    while (hi - b > 1) {
+        const int mid = (b + hi) >> 1;
+        if (P.starts[mid] <= tok) b = mid;
+        else hi = mid;
     }
-    const int64_t slot = live ? (int64_t)P.c.lengths[b] - (P.starts[b + 1] - tok) : -1;
-    const int64_t pos = live ? (P.positions ? (int64_t)P.positions[tok] : slot) : 0;
+    const int64_t slot = (int64_t)P.c.lengths[b] - (P.starts[b + 1] - tok);
+    const int64_t pos = P.positions ? (int64_t)P.positions[tok] : slot;
+    const int64_t row = slot >= 0 && slot < P.c.capacity() ? P.c.row(b, (int)slot) : -1;
 
-    const bool is_q = h < P.q_heads, is_v = h >= P.q_heads + P.c.kv_heads;
-    const int kh = is_v ? h - P.q_heads - P.c.kv_heads : h - P.q_heads;
-    const T* src = is_q ? static_cast<const T*>(P.q) + tok * P.q_ts + h * P.q_hs
-                 : is_v ? static_cast<const T*>(P.v) + tok * P.v_ts + kh * P.v_hs
-                        : static_cast<const T*>(P.k) + tok * P.k_ts + kh * P.k_hs;
-    uint4 raw = live ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u);
-    float x[8];
-    {
-        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    // this chunk's rotation: 8 angles (halves) or 4 (neighbours)
+    const int hc = P.half / 8;
+    const bool turned = c < 2 * hc, lower = c < hc;
+    const int partner = turned && !P.interleaved ? (lower ? c + hc : c - hc) : c;
+    float co[8], si[8];
+    if (turned) {
+        if (pos >= 0 && pos < P.table_rows) {
+            const int64_t at = pos * P.half + (P.interleaved ? c * 4 : (lower ? c : c - hc) * 8);
+            *reinterpret_cast<float4*>(co) = *reinterpret_cast<const float4*>(P.cos + at);
+            *reinterpret_cast<float4*>(si) = *reinterpret_cast<const float4*>(P.sin + at);
+            if (!P.interleaved) {
+                *reinterpret_cast<float4*>(co + 4) = *reinterpret_cast<const float4*>(P.cos + at + 4);
+                *reinterpret_cast<float4*>(si + 4) = *reinterpret_cast<const float4*>(P.sin + at + 4);
+            }
+        } else {                                            // a position outside the tables gives NaN
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = Elem<T>::wide(w[i]);
-            x[2 * i] = f.x;
-            x[2 * i + 1] = f.y;
+            for (int e = 0; e < 8; ++e) co[e] = si[e] = __int_as_float(0x7fffffff);
         }
     }
-    const void* weight = is_v ? nullptr : is_q ? P.q_weight : P.k_weight;
-    float ss = 0.f;
+    const int base = (threadIdx.x & 31) / LPH * LPH;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+    for (int i = 0; i < U; ++i) {
+        const int h = h0 + i * HP;
+        const bool is_q = h < keys, is_v = h >= values;
+        float x[8];
+        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        float ss = 0.f;
 #pragma unroll
-    for (int s = LPH / 2; s > 0; s >>= 1) ss += __shfl_xor_sync(FULL, ss, s);
-    if (weight) {
-        const float inv = rsqrtf(ss * (1.f / D) + P.eps);
-        const uint4 wr = *reinterpret_cast<const uint4*>(static_cast<const T*>(weight) + c * 8);
-        const uint32_t w[4] = {wr.x, wr.y, wr.z, wr.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = Elem<T>::wide(w[i]);
-            x[2 * i] *= inv * f.x;
-            x[2 * i + 1] *= inv * f.y;
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = Elem<T>::wide(w[e]);
+            x[2 * e] = f.x;
+            x[2 * e + 1] = f.y;
+            ss += f.x * f.x;
+            ss += f.y * f.y;
         }
-    }
-    const bool turned = !is_v && c * 8 < 2 * P.half;
-    const bool known = pos >= 0 && pos < P.table_rows;     // a position outside the tables gives NaN
-    const float NaN = __int_as_float(0x7fffffff);
-    if (P.interleaved) {
-        if (turned) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float co = known ? P.cos[pos * P.half + c * 4 + i] : NaN;
-                const float si = known ? P.sin[pos * P.half + c * 4 + i] : NaN;
-                const float a = x[2 * i], e = x[2 * i + 1];
-                x[2 * i] = a * co - e * si;
-                x[2 * i + 1] = e * co + a * si;
+        for (int s = LPH / 2; s > 0; s >>= 1) ss += __shfl_xor_sync(FULL, ss, s);
+        const T* weight = static_cast<const T*>(is_v ? nullptr : is_q ? P.q_weight : P.k_weight);
+        if (weight) {
+            const float inv = rsqrtf(ss * (1.f / D) + P.eps);
+            const uint4 wr = *reinterpret_cast<const uint4*>(weight + c * 8);
+            const uint32_t v[4] = {wr.x, wr.y, wr.z, wr.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = Elem<T>::wide(v[e]);
+                x[2 * e] *= inv * f.x;
+                x[2 * e + 1] *= inv * f.y;
             }
         }
-    } else {
-        const int hc = P.half / 8;
-        const bool lower = c < hc;
-        const int partner = turned ? (lower ? c + hc : c - hc) : c;
-        const int base = (threadIdx.x & 31) / LPH * LPH;
-        float y[8];
+        if (P.interleaved) {
+            if (turned && !is_v) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(FULL, x[i], base + partner);
-        if (turned) {
-            const int64_t row = pos * P.half + (lower ? c : c - hc) * 8;
+                for (int e = 0; e < 4; ++e) {
+                    const float a = x[2 * e], z = x[2 * e + 1];
+                    x[2 * e] = a * co[e] - z * si[e];
+                    x[2 * e + 1] = z * co[e] + a * si[e];
+                }
+            }
+        } else {
+            float y[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float co = known ? P.cos[row + i] : NaN;
-                const float si = known ? P.sin[row + i] : NaN;
-                x[i] = lower ? x[i] * co - y[i] * si : x[i] * co + y[i] * si;
+            for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(FULL, x[e], base + partner);
+            if (turned && !is_v) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = lower ? x[e] * co[e] - y[e] * si[e] : x[e] * co[e] + y[e] * si[e];
             }
         }
+        if (h >= heads) continue;
+        if (weight || (turned && !is_v))
+            raw[i] = make_uint4(Elem<T>::pack(x[0], x[1]), Elem<T>::pack(x[2], x[3]), Elem<T>::pack(x[4], x[5]),
+                                Elem<T>::pack(x[6], x[7]));
+        if (is_q) {
+            *reinterpret_cast<uint4*>(static_cast<T*>(P.out) + (tok * P.q_heads + h) * D + c * 8) = raw[i];
+        } else if (row >= 0) {
+            const int kh = is_v ? h - values : h - keys;
+            T* pool = static_cast<T*>(const_cast<void*>(is_v ? P.c.v : P.c.k));
+            *reinterpret_cast<uint4*>(pool + row + kh * P.c.head_stride + c * 8) = raw[i];
+            if (P.slot_positions && !is_v && c == 0 && slot < P.width)
+                P.slot_positions[((int64_t)b * P.c.kv_heads + kh) * P.width + slot] = (int32_t)pos;
+        }
     }
-    if (!live) return;
-    if (weight || turned)
-        raw = make_uint4(Elem<T>::pack(x[0], x[1]), Elem<T>::pack(x[2], x[3]), Elem<T>::pack(x[4], x[5]),
-                         Elem<T>::pack(x[6], x[7]));
-    if (is_q) {
-        *reinterpret_cast<uint4*>(static_cast<T*>(P.out) + (tok * P.q_heads + h) * D + c * 8) = raw;
-        return;
-    }
-    if (slot < 0 || slot >= P.c.capacity()) return;
-    const int64_t row = P.c.row(b, (int)slot);
-    if (row < 0) return;
-    T* pool = static_cast<T*>(const_cast<void*>(is_v ? P.c.v : P.c.k));
-    *reinterpret_cast<uint4*>(pool + row + kh * P.c.head_stride + c * 8) = raw;
-    if (P.slot_positions && !is_v && c == 0 && slot < P.width)
-        P.slot_positions[((int64_t)b * P.c.kv_heads + kh) * P.width + slot] = (int32_t)pos;
 }
 
 // -- eviction -----------------------------------------------------------------
@@ -171,7 +184,9 @@ struct Evict {
     int row_chunks;               // 16-byte chunks of a row
 };
 
-constexpr int SELECT_THREADS = 512;
+constexpr int SELECT_THREADS = 1024;
+constexpr int SELECT_WARPS = SELECT_THREADS / 32;
+constexpr int BINS = 2048;
 
 // a slot's key: larger stays.  First and newest positions above every weight,
 // then the weights as numbers, NaN below all of them.
@@ -182,25 +197,31 @@ __device__ __forceinline__ uint32_t keep_key(float w, int pos, int sinks, int64_
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// exclusive sum of a 0/1 flag over the block, and the total
-__device__ __forceinline__ int block_rank(bool flag, int* s_warp, int& total) {
+// sum of x over the warps before this one (x the same in a warp's lanes), and
+// over all; called by the whole CTA
+__device__ __forceinline__ int warps_before(int x, int* s_warp, int& total) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const unsigned m = __ballot_sync(FULL, flag);
-    if (lane == 0) s_warp[warp] = __popc(m);
     __syncthreads();
-    int before = 0, all = 0;
+    if (lane == 0) s_warp[warp] = x;
+    __syncthreads();
+    const int y = s_warp[lane];
+    int sum = y;
 #pragma unroll
-    for (int w = 0; w < SELECT_THREADS / 32; ++w) {
-        before += w < warp ? s_warp[w] : 0;
-        all += s_warp[w];
+    for (int s = 1; s < 32; s <<= 1) {
+        const int z = __shfl_up_sync(FULL, sum, s);
+        if (lane >= s) sum += z;
     }
-    __syncthreads();
-    total = all;
-    return before + __popc(m & lanemask_lt());
+    total = __shfl_sync(FULL, sum, 31);
+    return __shfl_sync(FULL, sum - y, warp);
 }
+static_assert(SELECT_WARPS == 32, "one lane a warp");
 
+// KEEP: 32-slot steps of a warp whose keys stay in registers; beyond that they are
+// read again in each pass
+template <int KEEP>
 __global__ void __launch_bounds__(SELECT_THREADS) select_kernel(const __grid_constant__ Evict P) {
-    __shared__ int s_hist[256], s_warp[SELECT_THREADS / 32], s_pick[2];
+    __shared__ int s_hist[BINS], s_warp[SELECT_WARPS], s_pick[2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t head = blockIdx.x;                       // sequence * kv_heads + key head
     const int b = (int)(head / P.c.kv_heads);
     const int n = (int)max((int64_t)0, min((int64_t)P.c.lengths[b], min(P.c.capacity(), P.width)));
@@ -223,66 +244,101 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_kernel(const __grid_con
         if (threadIdx.x == 0) P.counts[head] = 0;
         return;
     }
-    // the m-th largest key, 8 bits at a time from the top; `need` of the keys
+    // this warp's slots: 32 at a time from j0 on
+    const int steps = (n + SELECT_THREADS - 1) / SELECT_THREADS, j0 = warp * steps * 32 + lane;
+    auto key_at = [&](int i) -> uint32_t {
+        const int j = j0 + i * 32;
+        return j < n ? keep_key(w[j], pos[j], P.sinks, fresh) : 0u;
+    };
+    uint32_t held[KEEP];
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) held[i] = i < steps ? key_at(i) : 0u;
+    // f(step, key, whether there is a slot) for this warp's steps, in order
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i)
+            if (i < steps) f(i, held[i], j0 + i * 32 < n);
+        for (int i = KEEP; i < steps; ++i) f(i, key_at(i), j0 + i * 32 < n);
+    };
+
+    // the m-th largest key, some bits at a time from the top; `need` of the keys
     // that share the bits found so far are among the m largest
     uint32_t prefix = 0, mask = 0;
     int need = m;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = threadIdx.x; i < 256; i += SELECT_THREADS) s_hist[i] = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t digit = pass == 2 ? 1023u : 2047u;
+        s_hist[threadIdx.x] = 0;
+        s_hist[threadIdx.x + 1024] = 0;
         __syncthreads();
-        for (int j = threadIdx.x; j < n; j += SELECT_THREADS) {
-            const uint32_t key = keep_key(w[j], pos[j], P.sinks, fresh);
-            if ((key & mask) == prefix) atomicAdd(&s_hist[(key >> shift) & 255], 1);
+        each([&](int, uint32_t key, bool there) {
+            if (there && (key & mask) == prefix) atomicAdd(&s_hist[(key >> shift) & digit], 1);
+        });
+        __syncthreads();
+        // bins from the largest down, two a thread: the one that holds the need-th
+        const int hi = s_hist[BINS - 1 - 2 * threadIdx.x], lo = s_hist[BINS - 2 - 2 * threadIdx.x];
+        int sum = hi + lo;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const int z = __shfl_up_sync(FULL, sum, s);
+            if (lane >= s) sum += z;
         }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            int left = need, bin = 255;
-            while (bin > 0 && s_hist[bin] < left) left -= s_hist[bin--];
-            s_pick[0] = bin;
-            s_pick[1] = left;
+        int total;
+        const int before = warps_before(__shfl_sync(FULL, sum, 31), s_warp, total) + sum - hi - lo;
+        if (before < need && need <= before + hi + lo) {
+            const bool top = need <= before + hi;
+            s_pick[0] = BINS - 1 - 2 * threadIdx.x - (top ? 0 : 1);
+            s_pick[1] = need - before - (top ? 0 : hi);
         }
         __syncthreads();
         prefix |= (uint32_t)s_pick[0] << shift;
-        mask |= 255u << shift;
+        mask |= digit << shift;
         need = s_pick[1];
-        __syncthreads();
     }
-    // in slot order: equal keys to the lowest slots, free places and rows to move
-    int ties = 0, free = 0, late = 0;
+
+    // in slot order: equal keys to the lowest slots
+    int total, mine = 0;
+    each([&](int, uint32_t key, bool there) { mine += __popc(__ballot_sync(FULL, there && key == prefix)); });
+    const int ties0 = warps_before(mine, s_warp, total);
+    int ties = ties0, free = 0, late = 0;
+    auto keeps = [&](uint32_t key, bool there) -> bool {
+        const unsigned t = __ballot_sync(FULL, there && key == prefix);
+        const bool keep = there && (key > prefix || (key == prefix && ties + __popc(t & lanemask_lt()) < need));
+        ties += __popc(t);
+        return keep;
+    };
+    each([&](int i, uint32_t key, bool there) {
+        const bool keep = keeps(key, there);
+        const int j = j0 + i * 32;
+        free += __popc(__ballot_sync(FULL, j < m && !keep));
+        late += __popc(__ballot_sync(FULL, j >= m && keep));
+    });
+    int moved;
+    free = warps_before(free, s_warp, total);
+    late = warps_before(late, s_warp, moved);
+    ties = ties0;
     int32_t* from = P.moves + head * 2 * m;
     int32_t* to = from + m;
-    for (int j0 = 0; j0 < n; j0 += SELECT_THREADS) {
-        const int j = j0 + threadIdx.x;
-        float wj = 0.f;
-        int pj = 0;
-        uint32_t key = 0;
-        if (j < n) {
-            wj = w[j];
-            pj = pos[j];
-            key = keep_key(wj, pj, P.sinks, fresh);
+    each([&](int i, uint32_t key, bool there) {
+        const bool keep = keeps(key, there);
+        const int j = j0 + i * 32;
+        const unsigned f = __ballot_sync(FULL, j < m && !keep), l = __ballot_sync(FULL, j >= m && keep);
+        if (j < m && keep) {
+            nw[j] = w[j];
+            np[j] = pos[j];
         }
-        int total;
-        const bool tie = j < n && key == prefix;
-        const int tr = block_rank(tie, s_warp, total) + ties;
-        ties += total;
-        const bool keep = j < n && (key > prefix || (tie && tr < need));
-        if (keep && j < m) {
-            nw[j] = wj;
-            np[j] = pj;
-        }
-        const int fr = block_rank(j < m && !keep, s_warp, total) + free;
-        free += total;
-        if (j < m && !keep) to[fr] = j;
-        const int lr = block_rank(j >= m && keep, s_warp, total) + late;
-        late += total;
-        if (j >= m && keep) from[lr] = j;
-    }
+        if (j < m && !keep) to[free + __popc(f & lanemask_lt())] = j;
+        if (j >= m && keep) from[late + __popc(l & lanemask_lt())] = j;
+        free += __popc(f);
+        late += __popc(l);
+    });
     __syncthreads();
-    for (int i = threadIdx.x; i < late; i += SELECT_THREADS) {
+    for (int i = threadIdx.x; i < moved; i += SELECT_THREADS) {
         nw[to[i]] = w[from[i]];
         np[to[i]] = pos[from[i]];
     }
-    if (threadIdx.x == 0) P.counts[head] = late;
+    if (threadIdx.x == 0) P.counts[head] = moved;
 }
 
 constexpr int MOVE_THREADS = 256;
@@ -317,10 +373,10 @@ using namespace swb::attn;
 
 template <typename T, int D>
 static int launch_append(const Append& a, cudaStream_t st) {
-    const int64_t lanes = a.tokens * (a.q_heads + 2 * a.c.kv_heads) * (D / 8);
-    const int64_t blocks = (lanes + APPEND_THREADS - 1) / APPEND_THREADS;
-    if (blocks >= ((int64_t)1 << 31)) return abi::fail(SWB_ERR_ARG, "too many tokens in one call");
-    append_kernel<T, D><<<(unsigned)blocks, APPEND_THREADS, 0, st>>>(a);
+    constexpr int per = APPEND_THREADS / (D / 8) * APPEND_HEADS;
+    const int64_t by = ((int64_t)a.q_heads + 2 * a.c.kv_heads + per - 1) / per;
+    if (a.tokens >= ((int64_t)1 << 31) || by > 65535) return abi::fail(SWB_ERR_ARG, "too many tokens or heads in one call");
+    append_kernel<T, D><<<dim3((unsigned)a.tokens, (unsigned)by), APPEND_THREADS, 0, st>>>(a);
     return abi::cuda_check("append launch");
 }
 
@@ -341,6 +397,8 @@ extern "C" int swb_rope_append(const void* q, int64_t q_token_stride, int64_t q_
     if (rot_dim < 0 || rot_dim % 16 || rot_dim > cache->head_dim)
         return abi::fail(SWB_ERR_ARG, "the rotated dimensions must be a multiple of 16, at most head_dim");
     if (rot_dim && (!cos || !sin)) return abi::fail(SWB_ERR_ARG, "null rotation tables");
+    if (reinterpret_cast<uintptr_t>(cos) % 16 || reinterpret_cast<uintptr_t>(sin) % 16)
+        return abi::fail(SWB_ERR_ARG, "the rotation tables must start on 16-byte boundaries");
     const void* at[6] = {q, k, v, out, q_weight, k_weight};
     const int64_t strides[6] = {q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride};
     for (int i = 0; i < 6; ++i)
@@ -414,7 +472,8 @@ extern "C" int swb_kv_evict(const swb_kv_cache* cache, const int32_t* seen, cons
     e.counts = e.moves + heads * 2 * budget;
     e.row_chunks = cache->head_dim / 8;
     cudaStream_t st = (cudaStream_t)stream;
-    select_kernel<<<(unsigned)heads, SELECT_THREADS, 0, st>>>(e);
+    if (e.c.capacity() <= 4 * SELECT_THREADS) select_kernel<4><<<(unsigned)heads, SELECT_THREADS, 0, st>>>(e);
+    else select_kernel<16><<<(unsigned)heads, SELECT_THREADS, 0, st>>>(e);
     const int rc2 = abi::cuda_check("evict launch");
     if (rc2) return rc2;
     // at most min(budget, slots beyond it) rows of a head move
