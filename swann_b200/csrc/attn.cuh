@@ -97,12 +97,16 @@ struct Cache {
         const int64_t n = lengths[b];
         return (int)max((int64_t)0, min(n, capacity()));
     }
-    // element offset of a slot's row in a pool, for head 0; -1 where the table
-    // names no page of the pool
+    // the page of a slot; -1 where the table names none of the pool's
+    __device__ __forceinline__ int page(int b, int slot) const {
+        const int p = table[(int64_t)b * table_stride + (slot >> shift)];
+        return (unsigned)p < (unsigned)pages ? p : -1;
+    }
+    // element offset of a slot's row in a pool, for head 0; -1 without a page
     __device__ __forceinline__ int64_t row(int b, int slot) const {
-        const int page = table[(int64_t)b * table_stride + (slot >> shift)];
-        if ((unsigned)page >= (unsigned)pages) return -1;
-        return page * page_stride + (int64_t)(slot & ((1 << shift) - 1)) * row_stride;
+        const int p = page(b, slot);
+        if (p < 0) return -1;
+        return p * page_stride + (int64_t)(slot & ((1 << shift) - 1)) * row_stride;
     }
 };
 

@@ -9,18 +9,20 @@
 // A CTA owns two tiles of 128 query rows that share a key head: row r of a tile is
 // token r / heads, head r % heads, so the heads of a group read each block of keys
 // once.  It walks the blocks of 128 keys that any of its rows sees:
-//   warps 8..11   producers: K and V rows by cp.async into a ring of 128-byte
-//                 swizzled tiles, one row address a lane.  Rows that no page holds
-//                 or that lie past the end are filled with zeros, so what is in
-//                 memory there reaches no product;
-//   warp 12       issues tcgen05.mma: S = Q K^T (both K-major) into the tile's 128
+//   warps 9..11   producers: K and V into a ring of 128-byte swizzled tiles, 32
+//                 rows a warp at a time.  Where all 32 are seen by some row and lie
+//                 in pages of at least 8 rows, TMA brings them, a box a page; else
+//                 cp.async, one row address a lane, rows that no page holds or no
+//                 query sees filled with zeros, so what is in memory there reaches
+//                 no product.  (cp.async alone kept the tensor pipe waiting: 332 us
+//                 against 199 for 2049 tokens over 8193 slots, 32 heads of 128);
+//   warp 8        issues tcgen05.mma: S = Q K^T (both K-major) into the tile's 128
 //                 TMEM columns, O += P V with P read from TMEM and V as it lies
 //                 (MN-major);
-//   warps 0..3 and 4..7  softmax of tile 0 and 1: a thread is a row.  It reads S
-//                 twice (maximum, then weights: holding 128 values a thread would
-//                 not leave registers for two tiles), writes the weights, rounded
-//                 to the cache's 16 bits, over the S it has read, and keeps the
-//                 row's sum in 32 bits, before that rounding.
+//   warps 0..3 and 4..7  softmax of tile 0 and 1: a thread is a row and holds its
+//                 128 logits (384 threads leave it 168 registers).  It writes the
+//                 weights, rounded to the cache's 16 bits, over the logits' columns
+//                 and keeps the row's sum in 32 bits, before that rounding.
 // The running maximum that the exponentials are taken against is only raised when
 // a row's maximum has passed it by 2^8 (weights stay below 2^8 and sums in range);
 // only then is O rescaled in TMEM, which the first blocks of a row need and later
@@ -30,6 +32,9 @@
 // after the product that reads the weights lying in the same columns.  All waits
 // are bounded; if one runs out the CTA's rows are NaN and the status word is set.
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include "attn.cuh"
 #include "tcgen05.cuh"
 
@@ -38,10 +43,10 @@ namespace attn {
 namespace pre {
 
 constexpr int TILE = 128;                   // rows of a query tile, keys of a block
-constexpr int THREADS = 512;
-constexpr int PRODUCER0 = 256, PRODUCERS = 128;
-constexpr int MMA_WARP = 12;
-constexpr int LAG = 2;                      // copies of a producer in flight behind the one being issued
+constexpr int THREADS = 384;
+constexpr int MMA_WARP = 8, PRODUCER0 = 9, PRODUCERS = 3;   // warps
+constexpr int PIECES = 4;                   // of 32 rows, of a tile
+constexpr int LAG = 2;                      // pieces of a warp in flight behind the one being issued
 constexpr float RAISE = 8.f;                // log2 of how far a maximum may pass the one in use
 
 struct Prefill {
@@ -51,9 +56,10 @@ struct Prefill {
     const int32_t* starts;
     int64_t tokens;
     int q_heads, group, head_tiles, tile_heads, tile_tokens;
-    float scale2;               // |scale| * log2(e)
+    float scale2;               // |scale| * log2(e), above 0
     int flip;                   // scale below 0: the queries' signs are turned instead
     int window, sinks;
+    int tma;                    // the maps hold: rows of a box, 0 where there are none
     void* out;
     float* lse;
     int32_t* status;
@@ -139,15 +145,15 @@ __device__ __forceinline__ void tmem_arrived(uint32_t (&r)[32]) {
                  :
                  : "memory");
 }
-__device__ __forceinline__ void tmem_put32(uint32_t a, const uint32_t (&r)[32]) {
+// 16 columns, arrived
+__device__ __forceinline__ void tmem_get16(uint32_t a, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
-        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
-        "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-        "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(a)
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(a)
         : "memory");
 }
 __device__ __forceinline__ void tmem_put16(uint32_t a, const uint32_t (&r)[16]) {
@@ -158,21 +164,61 @@ __device__ __forceinline__ void tmem_put16(uint32_t a, const uint32_t (&r)[16]) 
         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(a)
         : "memory");
 }
+// rows of one page and head into a panel (box: 64 dimensions x some rows)
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int row, int head, int page,
+                                        uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(head), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// two fp32 values an instruction, each rounded on its own
+__device__ __forceinline__ unsigned long long pair(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 halves(unsigned long long v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 
 // the low x bits of a word
 __device__ __forceinline__ uint32_t low_bits(int x) { return x >= 32 ? 0xffffffffu : x <= 0 ? 0u : (1u << x) - 1u; }
 
-// What the CTA's roles agree on.  A block's keys have virtual places u: the first
-// tokens, then everything from slot `lo` on.
+// What the CTA's roles agree on.  Keys have places u, blocks of 128 of them: place
+// u is slot base + u, base a multiple of 128 so that places keep the slots'
+// alignment to pages.  With a window the first slot seen is lo and base lies at
+// least as many places below it as there are first tokens to see: those take the
+// places u < first, and the places between hold nothing.
 struct Job {
     int b, g, head0, heads;
     int64_t token0;             // of the batch: first token of tile 0
     int pos0;                   // its slot
     int live;                   // tokens of the CTA that exist
-    int first, lo, n, blocks;
-    __device__ __forceinline__ int slot(int u) const { return u < first ? u : lo + (u - first); }
+    int first, lo, base, n, blocks;
+    __device__ __forceinline__ int slot(int u) const { return u < first ? u : base + u; }
+    __device__ __forceinline__ bool holds(int u) const { return u < n && (u < first || base + u >= lo); }
 };
 
 __device__ __forceinline__ bool find_job(const Prefill& P, Job& J) {
@@ -221,7 +267,8 @@ __device__ __forceinline__ bool find_job(const Prefill& P, Job& J) {
     const int end = (int)max((int64_t)0, min((int64_t)J.pos0 + J.live, P.c.capacity()));
     J.lo = P.window > 0 ? min(max(0, J.pos0 - P.window + 1), end) : 0;
     J.first = min(P.sinks, J.lo);
-    J.n = J.first + end - J.lo;
+    J.base = (J.lo - J.first) / TILE * TILE;
+    J.n = end - J.base;
     J.blocks = (J.n + TILE - 1) / TILE;
     return true;
 }
@@ -237,14 +284,16 @@ __device__ __forceinline__ Span span_of(const Prefill& P, const Job& J, int t) {
     s.pos = J.pos0 + t * P.tile_tokens;
     s.a = s.z = 0;
     if (s.tokens == 0) return s;
-    const int ub = min(J.n, J.first + s.pos + s.tokens - J.lo);       // end of what its last token sees
+    const int ub = min(J.n, s.pos + s.tokens - J.base);               // end of what its last token sees
     s.z = (max(0, ub) + TILE - 1) / TILE;
-    if (P.window > 0 && P.sinks == 0 && s.z > 1 && J.slot(TILE - 1) <= s.pos - P.window) s.a = 1;
+    if (P.window > 0 && P.sinks == 0 && s.z > 1 && J.base + TILE - 1 <= s.pos - P.window) s.a = 1;
     return s;
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_constant__ Prefill P) {
+__global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_constant__ Prefill P,
+                                                             const __grid_constant__ CUtensorMap tmk,
+                                                             const __grid_constant__ CUtensorMap tmv) {
     using Ly = Layout<D>;
     constexpr int SLOTS = Ly::SLOTS;
     constexpr int CH = D / 8;
@@ -268,10 +317,10 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     if (threadIdx.x == 0) {
         *s_abort = (smem_u32(sm) & 1023u) ? 2 : 0;
         for (int s = 0; s < SLOTS; ++s) {
-            mbar_init(&full[s], PRODUCERS);
+            mbar_init(&full[s], PIECES * 32);
             mbar_init(&empty[s], 1);
         }
-        mbar_init(qbar, PRODUCERS);
+        mbar_init(qbar, 2 * PIECES * 32);
         for (int t = 0; t < 2; ++t) {
             mbar_init(&sbar[t], 2);       // the product's commit and the issuing thread
             mbar_init(&pbar[t], TILE);
@@ -289,32 +338,37 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     const uint32_t tmem = s_tmem;
     const uint32_t base = smem_u32(sm);
 
-    if (warp >= PRODUCER0 / 32 && warp < MMA_WARP) {
+    if (warp >= PRODUCER0) {
         // ---------------- producers
-        const int w = warp - PRODUCER0 / 32;
+        const int w = warp - PRODUCER0;
         const T* q = static_cast<const T*>(P.q);
-        for (int t = 0; t < 2; ++t) {
-            const int r = w * 32 + lane, tok = r / J.heads;
-            const bool real = tok < sp[t].tokens;
-            const int64_t off = real ? (J.token0 + t * P.tile_tokens + tok) * P.q_token_stride +
-                                           (int64_t)(J.head0 + r % J.heads) * P.q_head_stride
-                                     : -1;
+        // 32 rows of a tile, one row address a lane, -1 for a row of zeros
+        auto copy = [&](uint32_t dst, int piece, const T* src, int64_t off) {
 #pragma unroll
             for (int it = 0; it < CH; ++it) {
                 const int rr = (it * 32 + lane) / CH, c = (it * 32 + lane) % CH;
                 const int64_t o = __shfl_sync(FULL, (long long)off, rr);
-                cp_async16_or_zero(base + Ly::Q + t * Ly::TILEB + place(w * 32 + rr, c), q + (o >= 0 ? o + c * 8 : 0), o >= 0);
+                cp_async16_or_zero(dst + place(piece * 32 + rr, c), src + (o >= 0 ? o + c * 8 : 0), o >= 0);
             }
+        };
+        int copies = 0;
+        for (int i = w; i < 2 * PIECES; i += PRODUCERS, ++copies) {
+            const int t = i / PIECES, piece = i % PIECES;
+            const int r = piece * 32 + lane, tok = r / J.heads;
+            const int64_t off = tok < sp[t].tokens ? (J.token0 + t * P.tile_tokens + tok) * P.q_token_stride +
+                                                         (int64_t)(J.head0 + r % J.heads) * P.q_head_stride
+                                                   : -1;
+            copy(base + Ly::Q + t * Ly::TILEB, piece, q, off);
         }
         cp_async_commit();
         cp_async_wait<0>();
         if (P.flip) {
             // each thread turns the chunks that it copied itself
-            for (int t = 0; t < 2; ++t)
+            for (int i = w; i < 2 * PIECES; i += PRODUCERS)
 #pragma unroll
                 for (int it = 0; it < CH; ++it) {
                     const int rr = (it * 32 + lane) / CH, c = (it * 32 + lane) % CH;
-                    uint4* p = reinterpret_cast<uint4*>(sm + Ly::Q + t * Ly::TILEB + place(w * 32 + rr, c));
+                    uint4* p = reinterpret_cast<uint4*>(sm + Ly::Q + (i / PIECES) * Ly::TILEB + place(i % PIECES * 32 + rr, c));
                     uint4 x = *p;
                     x.x ^= 0x80008000u;
                     x.y ^= 0x80008000u;
@@ -324,44 +378,73 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
                 }
         }
         fence_async_smem();
-        mbar_arrive(qbar);
+        for (int i = 0; i < copies; ++i) mbar_arrive(qbar);
 
         const T* kp = static_cast<const T*>(P.c.k) + (int64_t)J.g * P.c.head_stride;
         const T* vp = static_cast<const T*>(P.c.v) + (int64_t)J.g * P.c.head_stride;
-        const int total = 2 * J.blocks;
-        int64_t off = -1;
-        int idx = 0;
-        for (; idx < total && !*s_abort; ++idx) {
-            const int slot = idx % SLOTS;
-            if ((idx & 1) == 0) {
-                const int u = (idx >> 1) * TILE + w * 32 + lane;
-                off = u < J.n ? P.c.row(J.b, J.slot(u)) : -1;
-                const unsigned seen = __ballot_sync(FULL, off >= 0);
-                if (lane == 0) s_seen[((idx >> 1) & 7) * 4 + w] = seen;
-            }
-            if (!mbar_wait(&empty[slot], ((idx / SLOTS) & 1) ^ 1)) {
-                *s_abort = 1;
-                break;
-            }
-            const T* src = (idx & 1) ? vp : kp;
-            const uint32_t dst = base + Ly::RING + slot * Ly::TILEB;
+        // pieces in order: tile K0's four, V0's, K1's, ..; this warp has every third
+        const int total = 2 * J.blocks * PIECES;
+        // the page of this lane's row of piece i, -1 where there is none
+        auto find = [&](int i) -> int {
+            const int u = (i / (2 * PIECES)) * TILE + i % PIECES * 32 + lane;
+            return i < total && J.holds(u) ? P.c.page(J.b, J.slot(u)) : -1;
+        };
+        int waits[LAG], behind = 0;         // ring slots whose copies by cp.async are in flight
+        auto hand_over = [&]() {
+            cp_async_wait<0>();
+            fence_async_smem();
 #pragma unroll
-            for (int it = 0; it < CH; ++it) {
-                const int rr = (it * 32 + lane) / CH, c = (it * 32 + lane) % CH;
-                const int64_t o = __shfl_sync(FULL, (long long)off, rr);
-                cp_async16_or_zero(dst + place(w * 32 + rr, c), src + (o >= 0 ? o + c * 8 : 0), o >= 0);
+            for (int k = 0; k < LAG; ++k)
+                if (k < behind) mbar_arrive(&full[waits[k]]);
+            behind = 0;
+        };
+        int page = find(w);
+        for (int i = w; i < total && !*s_abort; i += PRODUCERS) {
+            const int idx = i / PIECES, piece = i % PIECES, slot = idx % SLOTS;
+            const int u = (idx >> 1) * TILE + piece * 32 + lane, at = J.slot(u) & ((1 << P.c.shift) - 1);
+            const unsigned seen = __ballot_sync(FULL, page >= 0);
+            if ((idx & 1) == 0 && lane == 0) s_seen[((idx >> 1) & 7) * 4 + piece] = seen;
+            const uint32_t phase = ((idx / SLOTS) & 1) ^ 1;
+            if (!__all_sync(FULL, mbar_try_wait(&empty[slot], phase))) {
+                hand_over();                // no room yet: first what is in flight
+                if (!__all_sync(FULL, mbar_wait(&empty[slot], phase))) {
+                    *s_abort = 1;
+                    break;
+                }
             }
+            const uint32_t dst = base + Ly::RING + slot * Ly::TILEB;
+            if (P.tma && seen == FULL && u - lane >= J.first) {
+                if (lane == 0) mbar_expect_tx(&full[slot], 32 * D * 2);
+                else mbar_arrive(&full[slot]);
+                __syncwarp();
+                if ((lane & (P.tma - 1)) == 0) {
+                    const CUtensorMap* map = (idx & 1) ? &tmv : &tmk;
+#pragma unroll
+                    for (int h = 0; h < D / 64; ++h)
+                        tma_box(dst + h * Ly::ROWB + (piece * 32 + lane) * 128, map, h * 64, at, J.g, page, &full[slot]);
+                }
+                page = find(i + PRODUCERS);
+                continue;
+            }
+            copy(dst, piece, (idx & 1) ? vp : kp, page >= 0 ? page * P.c.page_stride + at * P.c.row_stride : -1);
             cp_async_commit();
-            if (idx >= LAG) {
+            page = find(i + PRODUCERS);
+            if (behind == LAG) {
                 cp_async_wait<LAG>();
                 fence_async_smem();
-                mbar_arrive(&full[(idx - LAG) % SLOTS]);
+                mbar_arrive(&full[waits[0]]);
+#pragma unroll
+                for (int k = 1; k < LAG; ++k) waits[k - 1] = waits[k];
+                --behind;
             }
+#pragma unroll
+            for (int k = 0; k < LAG; ++k)
+                if (k == behind) waits[k] = slot;
+            ++behind;
+            if (P.tma) hand_over();         // a boundary's piece: its block waits for it
             __syncwarp();
         }
-        cp_async_wait<0>();
-        fence_async_smem();
-        for (int i = max(0, idx - LAG); i < idx; ++i) mbar_arrive(&full[i % SLOTS]);
+        hand_over();
     } else if (warp == MMA_WARP) {
         // ---------------- MMA issuer
         if (lane == 0) {
@@ -405,7 +488,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
             if (!ok) *s_abort = 1;
         }
         __syncwarp();
-    } else if (warp < PRODUCER0 / 32) {
+    } else {
         // ---------------- softmax: thread r of the tile's warps is row r
         const int t = warp >> 2, r = threadIdx.x & (TILE - 1);
         const Span S = sp[t];
@@ -414,10 +497,11 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         const int pos = S.pos + min(tok, S.tokens - 1);     // rows of no token see what the last one does
         const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t st = tmem + quarter + t * TILE, ot = tmem + quarter + 2 * TILE + t * D;
-        // the row sees the places u < sinks and ua <= u, below ub
-        const int ub = J.first + pos + 1 - J.lo;
-        const int ua = P.window > 0 ? J.first + max(0, pos - P.window + 1 - J.lo) : 0;
-        float m = NEG_INF, l0 = 0.f, l1 = 0.f;
+        // of the places that hold something the row sees u < us and ua <= u, below ub
+        const int ub = pos + 1 - J.base, us = max(J.first, P.sinks - J.base);
+        const int ua = P.window > 0 ? pos - P.window + 1 - J.base : 0;
+        float m = NEG_INF;
+        float2 l[2] = {{0.f, 0.f}, {0.f, 0.f}};
         bool ok = true;
         for (int j = S.a; j < S.z; ++j) {
             const int i = j - S.a, u0 = j * TILE;
@@ -432,38 +516,34 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int u = u0 + c * 32;
-                vis[c] = low_bits(ub - u) & (low_bits(P.sinks - u) | ~low_bits(ua - u)) & s_seen[(j & 7) * 4 + c];
+                vis[c] = low_bits(ub - u) & (low_bits(us - u) | ~low_bits(ua - u)) & s_seen[(j & 7) * 4 + c];
                 whole = whole && vis[c] == 0xffffffffu;
             }
             const bool masked = __any_sync(FULL, !whole);
-            // the row's largest logit
-            float top = NEG_INF;
-            {
-                uint32_t x[2][32];
-                tmem_get32(st, x[0]);
+            uint32_t x[4][32];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    tmem_arrived(x[c & 1]);
-                    if (c < 3) tmem_get32(st + (c + 1) * 32, x[(c + 1) & 1]);
-                    float a[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
-                    if (masked) {
+            for (int c = 0; c < 4; ++c) tmem_get32(st + c * 32, x[c]);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            a[e & 3] = fmaxf(a[e & 3], (vis[c] >> e) & 1u ? __uint_as_float(x[c & 1][e]) : NEG_INF);
-                    } else {
+            for (int c = 0; c < 4; ++c) tmem_arrived(x[c]);
+            if (masked) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) a[e & 3] = fmaxf(a[e & 3], __uint_as_float(x[c & 1][e]));
-                    }
-                    top = fmaxf(top, fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
-                }
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) x[c][e] = (vis[c] >> e) & 1u ? x[c][e] : __float_as_uint(NEG_INF);
             }
-            top = top == NEG_INF ? NEG_INF : top * P.scale2;
+            // the row's largest logit
+            float a[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) a[c] = max3(a[c], __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]));
+            const float top = fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * P.scale2;
             const bool raise = top > m + RAISE || (m == NEG_INF && top != NEG_INF);
             if (__any_sync(FULL, raise)) {
                 const float f = raise && m != NEG_INF ? exp2_fast(m - top) : 1.f;
                 if (raise) m = top;
-                l0 *= f;
-                l1 *= f;
+                l[0] = make_float2(l[0].x * f, l[0].y * f);
+                l[1] = make_float2(l[1].x * f, l[1].y * f);
                 if (i > 0) {
                     ok = mbar_wait(&obar[t], (i - 1) & 1);
                     if (!__all_sync(FULL, ok)) {
@@ -472,43 +552,34 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
                     }
                     tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t x[32];
-                        tmem_get32(ot + c * 32, x);
-                        tmem_arrived(x);
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t z[16];
+                        tmem_get16(ot + c * 16, z);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
-                        tmem_put32(ot + c * 32, x);
+                        for (int e = 0; e < 16; ++e) z[e] = __float_as_uint(__uint_as_float(z[e]) * f);
+                        tmem_put16(ot + c * 16, z);
                     }
                     tmem_stored();
                 }
             }
             const float off = m == NEG_INF ? 0.f : -m;
-            // weights over the logits that were read
-            {
-                uint32_t x[2][32];
-                tmem_get32(st, x[0]);
+            // weights over the logits' columns
+            const unsigned long long s2 = pair(P.scale2, P.scale2), o2 = pair(off, off);
+            unsigned long long l2[2] = {pair(l[0].x, l[0].y), pair(l[1].x, l[1].y)};
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    tmem_arrived(x[c & 1]);
-                    if (c < 3) tmem_get32(st + (c + 1) * 32, x[(c + 1) & 1]);
-                    uint32_t p[16];
+            for (int c = 0; c < 4; ++c) {
+                uint32_t p[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        float y0 = fmaf(__uint_as_float(x[c & 1][2 * e]), P.scale2, off);
-                        float y1 = fmaf(__uint_as_float(x[c & 1][2 * e + 1]), P.scale2, off);
-                        if (masked) {
-                            y0 = (vis[c] >> (2 * e)) & 1u ? y0 : NEG_INF;
-                            y1 = (vis[c] >> (2 * e + 1)) & 1u ? y1 : NEG_INF;
-                        }
-                        const float w0 = exp2_fast(y0), w1 = exp2_fast(y1);
-                        l0 += w0;
-                        l1 += w1;
-                        p[e] = Elem<T>::pack(w0, w1);
-                    }
-                    tmem_put16(st + c * 16, p);
+                for (int e = 0; e < 16; ++e) {
+                    const float2 y = halves(fma2(pair(__uint_as_float(x[c][2 * e]), __uint_as_float(x[c][2 * e + 1])), s2, o2));
+                    const float w0 = exp2_fast(y.x), w1 = exp2_fast(y.y);
+                    l2[e & 1] = add2(l2[e & 1], pair(w0, w1));
+                    p[e] = Elem<T>::pack(w0, w1);
                 }
+                tmem_put16(st + c * 16, p);
             }
+            l[0] = halves(l2[0]);
+            l[1] = halves(l2[1]);
             tmem_stored();
             tc_fence_before();
             mbar_arrive(&pbar[t]);
@@ -519,8 +590,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         ok = __all_sync(FULL, ok);
         if (!ok) *s_abort = 1;
         tc_fence_after();
-        const float l = l0 + l1;
-        const float inv = ok ? (l == 0.f ? 0.f : 1.f / l) : __int_as_float(0x7fffffff);
+        const float sum = (l[0].x + l[0].y) + (l[1].x + l[1].y);
+        const float inv = ok ? (sum == 0.f ? 0.f : 1.f / sum) : __int_as_float(0x7fffffff);
         const int64_t row = (J.token0 + t * P.tile_tokens + tok) * P.q_heads + J.head0 + r % J.heads;
         uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(P.out) + row * D);
 #pragma unroll 1
@@ -544,7 +615,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
                 }
             }
         }
-        if (live) P.lse[row] = !ok ? inv : l == 0.f ? NEG_INF : (m + log2f(l)) * LN2;
+        if (live) P.lse[row] = !ok ? inv : sum == 0.f ? NEG_INF : (m + log2f(sum)) * LN2;
     }
     tc_fence_before();
     __syncthreads();
@@ -555,12 +626,40 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     }
 }
 
+// A pool as a map of boxes of 64 dimensions x `rows` rows of a page and head.
+// Returns whether there is one: strides that a map cannot express are left to
+// cp.async.
+inline bool pool_map(CUtensorMap* m, const void* pool, const Cache& c, int d, bool bf16, int rows) {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    if (!fn) {
+        cudaDriverEntryPointQueryResult q;
+        void* p = nullptr;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return false;
+        fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }
+    if (c.row_stride <= 0 || c.head_stride <= 0 || c.page_stride <= 0) return false;
+    cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)1 << c.shift, (cuuint64_t)c.kv_heads, (cuuint64_t)c.pages};
+    cuuint64_t strides[3] = {(cuuint64_t)c.row_stride * 2, (cuuint64_t)c.head_stride * 2, (cuuint64_t)c.page_stride * 2};
+    cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, step[4] = {1, 1, 1, 1};
+    return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(pool), dims,
+              strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int D>
-int launch(const Prefill& p, int64_t items, cudaStream_t st) {
+int launch(Prefill p, int64_t items, cudaStream_t st) {
     const cudaError_t e = cudaFuncSetAttribute(prefill_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                Layout<D>::TOTAL);
     if (e != cudaSuccess) return abi::cuda_fail(e, "cudaFuncSetAttribute(prefill)");
-    prefill_kernel<T, D><<<(unsigned)items, THREADS, Layout<D>::TOTAL, st>>>(p);
+    // 8 rows are a swizzle period, 32 a piece
+    CUtensorMap mk = {}, mv = {};
+    const int page = 1 << p.c.shift, rows = page < 32 ? page : 32;
+    constexpr bool bf16 = Format<T>::F == 1;
+    if (rows >= 8 && p.c.pages && pool_map(&mk, p.c.k, p.c, D, bf16, rows) && pool_map(&mv, p.c.v, p.c, D, bf16, rows))
+        p.tma = rows;
+    prefill_kernel<T, D><<<(unsigned)items, THREADS, Layout<D>::TOTAL, st>>>(p, mk, mv);
     return abi::cuda_check("prefill launch");
 }
 
@@ -594,7 +693,8 @@ extern "C" int swb_attn_prefill(const void* q, int64_t q_token_stride, int64_t q
     p.head_tiles = (p.group + p.tile_heads - 1) / p.tile_heads;
     p.tile_tokens = pre::TILE / p.tile_heads;
     p.flip = scale < 0.f;
-    p.scale2 = (scale < 0.f ? -scale : scale) * LOG2E;
+    // a scale of 0 is the smallest number instead: logits of 0, and -inf stays what it is
+    p.scale2 = fmaxf((scale < 0.f ? -scale : scale) * LOG2E, 1.2e-38f);
     p.window = window;
     p.sinks = sinks;
     p.out = out;
