@@ -7,33 +7,41 @@
 // layout below keeps the tensor pipe on one tile while another's softmax runs.
 //
 // A CTA owns two tiles of 128 query rows that share a key head: row r of a tile is
-// token r / heads, head r % heads, so the heads of a group read each block of keys
-// once.  It walks the blocks of 128 keys that any of its rows sees:
-//   warps 9..11   producers: K and V into a ring of 128-byte swizzled tiles, 32
-//                 rows a warp at a time.  Where all 32 are seen by some row and lie
+// token r / heads, head r % heads, so the heads of a group read each key once.  It
+// walks steps of 64 keys that any of its rows sees:
+//   warps 9..11   producers: K and V into a ring of 128-byte swizzled tiles, a
+//                 step's a warp.  Where all 64 rows are seen by some query and lie
 //                 in pages of at least 8 rows, TMA brings them, a box a page; else
 //                 cp.async, one row address a lane, rows that no page holds or no
 //                 query sees filled with zeros, so what is in memory there reaches
 //                 no product.  (cp.async alone kept the tensor pipe waiting: 332 us
-//                 against 199 for 2049 tokens over 8193 slots, 32 heads of 128);
-//   warp 8        issues tcgen05.mma: S = Q K^T (both K-major) into the tile's 128
-//                 TMEM columns, O += P V with P read from TMEM and V as it lies
-//                 (MN-major);
-//   warps 0..3 and 4..7  softmax of tile 0 and 1: a thread is a row and holds its
-//                 128 logits (384 threads leave it 168 registers).  It writes the
+//                 against 254 for 2049 tokens over 8193 slots, 32 heads of 128);
+//   warp 8        issues tcgen05.mma: S = Q K^T (both K-major) into one of the
+//                 tile's two buffers of 64 TMEM columns, O += P V with P read from
+//                 TMEM and V as it lies (MN-major).  What it does besides is kept
+//                 short (a wait a stage and a tile, a commit each): the tensor pipe's
+//                 queue is a few products deep;
+//   warps 0..3 and 4..7  softmax of tile 0 and 1: a thread is a row.  It writes the
 //                 weights, rounded to the cache's 16 bits, over the logits' columns
 //                 and keeps the row's sum in 32 bits, before that rounding.
+// With two buffers the next step's logits are there when a softmax ends: with one
+// of 128 keys, which TMEM has room for instead, each tile's softmax and products
+// took turns, and neither pipe was busy for more than half of the time.
+//
 // The running maximum that the exponentials are taken against is only raised when
 // a row's maximum has passed it by 2^8 (weights stay below 2^8 and sums in range);
 // only then is O rescaled in TMEM, which the first blocks of a row need and later
 // ones hardly ever do.
 //
-// MMAs of one thread run in order, so S of the next block may be issued right
-// after the product that reads the weights lying in the same columns.  All waits
+// MMAs of one thread run in order, so the logits of step i + 1 may be issued right
+// after the product that reads step i - 1's weights, which lie in the same columns.
+// All waits
 // are bounded; if one runs out the CTA's rows are NaN and the status word is set.
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
+
+#include <type_traits>
 
 #include "attn.cuh"
 #include "tcgen05.cuh"
@@ -42,11 +50,17 @@ namespace swb {
 namespace attn {
 namespace pre {
 
-constexpr int TILE = 128;                   // rows of a query tile, keys of a block
+constexpr int TILE = 128;                   // rows of a query tile
+constexpr int STEP = 64;                    // keys
 constexpr int THREADS = 384;
 constexpr int MMA_WARP = 8, PRODUCER0 = 9, PRODUCERS = 3;   // warps
-constexpr int PIECES = 4;                   // of 32 rows, of a tile
-constexpr int LAG = 2;                      // pieces of a warp in flight behind the one being issued
+constexpr int SOFTMAX = 4;                  // warps of a tile
+constexpr int SEEN = 32;                    // steps whose rows are on record
+constexpr int LAG = 2;                      // parts of a warp in flight behind the one being issued
+#ifndef SWB_POLY
+#define SWB_POLY 99
+#endif
+constexpr int POLY = SWB_POLY;
 constexpr float RAISE = 8.f;                // log2 of how far a maximum may pass the one in use
 
 struct Prefill {
@@ -67,30 +81,33 @@ struct Prefill {
 
 template <int D>
 struct Layout {
-    static constexpr int ROWB = TILE * 128;                     // a 64-dimension panel of a tile
-    static constexpr int TILEB = TILE * D * 2;
+    static constexpr int QB = TILE * D * 2;                     // a query tile
+    static constexpr int KB = STEP * D * 2;                     // a step's K or V
+    static constexpr int STAGEB = 2 * KB;
     static constexpr int SLOTS = D == 128 ? 4 : 8;
     static constexpr int Q = 0;                                 // two tiles
-    static constexpr int RING = 2 * TILEB;
-    static constexpr int BARS = RING + SLOTS * TILEB;           // full, empty, q, s[2], p[2], o[2]
-    static constexpr int SEEN = BARS + (2 * SLOTS + 7) * 8;     // uint32 [8][4]
-    static constexpr int TOTAL = SEEN + 8 * 4 * 4;
+    static constexpr int RING = 2 * QB;
+    static constexpr int BARS = RING + SLOTS * STAGEB;          // full, empty, q, s[2][2], p[2][2], o[2][2]
+    static constexpr int SEENB = BARS + (2 * SLOTS + 13) * 8;   // uint32 [SEEN][2], on an 8-byte boundary
+    static constexpr int TOTAL = SEENB + SEEN * 2 * 4;
 };
 
-// chunk c (16 bytes) of row r of a tile made of 64-dimension panels
+// chunk c (16 bytes) of row r of a tile made of panels of 64 dimensions
+template <int ROWS>
 __device__ __forceinline__ uint32_t place(int r, int c) {
-    return (uint32_t)((c >> 3) * (TILE * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+    return (uint32_t)((c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-// V as the second operand: 64 dimensions x 8 keys in 1024 bytes, the next 8 keys
-// 1024 bytes on, the next 64 dimensions a panel on
-__device__ __forceinline__ uint64_t desc_v(uint32_t a) {
-    return ((uint64_t)(a >> 4) & 0x3FFFull) | ((uint64_t)(TILE * 128 / 16) << 16) | (64ull << 32) | (1ull << 46) |
-           (2ull << 61);
-}
-__device__ __forceinline__ uint64_t desc_k(uint32_t a) {
-    return ((uint64_t)(a >> 4) & 0x3FFFull) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
+// Operand descriptors: the high word is the same for all (version, 128-byte
+// swizzle, 1024 bytes from 8 rows to the next), the low word is the address / 16 and,
+// for V (which lies with its dimensions contiguous: 64 of them x 8 keys in 1024
+// bytes), the bytes from a panel to the next / 16.
+constexpr uint32_t DESC_HI = 64u | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t a) { return (a >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_v(uint32_t a) { return (a >> 4) | ((uint32_t)(STEP * 128 / 16) << 16); }
+
+// A stage of the ring holds what is multiplied next to each other: stage q has K of
+// step q and V of step q - 2, one after the other.
 
 template <typename T>
 struct Format;
@@ -108,19 +125,26 @@ __host__ __device__ constexpr uint32_t instr(int n, bool b_mn_major) {
            (uint32_t(n >> 3) << 17) | (uint32_t(TILE >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 x, {%1, %4};\n\tmov.b64 y, {%2, %4};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(DESC_HI), "r"(acc)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 y, {%2, %4};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(DESC_HI), "r"(acc)
         : "memory");
+}
+// one lane of a converged warp, in a form that the compiler knows to be one
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
 }
 
 // 32 columns of this thread's TMEM lane; the values are there after tmem_arrived
@@ -174,6 +198,11 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
         : "memory");
 }
 __device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// one arrival for a warp, after all of its lanes
+__device__ __forceinline__ void arrive_warp(uint64_t* bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // two fp32 values an instruction, each rounded on its own
@@ -197,17 +226,38 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+// 2^x of a pair without the special-function unit, for x below 2^22 and not NaN
+// (below -126 as -126): x = n + f with n the nearest integer, found by adding
+// 1.5 * 2^23, and 2^f by the polynomial of degree 4 whose largest relative error
+// on [-1/2, 1/2] is least (2.6e-6; Remez exchange), far below the 16 bits that a
+// weight is rounded to.  n goes into the exponent by an integer addition.
+__device__ __forceinline__ float2 exp2_poly(unsigned long long x) {
+    const float2 lo = halves(x);
+    const unsigned long long y = pair(fmaxf(lo.x, -126.f), fmaxf(lo.y, -126.f));
+    const unsigned long long big = pair(12582912.f, 12582912.f), neg = pair(-12582912.f, -12582912.f);
+    const unsigned long long t = add2(y, big), n = add2(t, neg);
+    const unsigned long long f = fma2(n, pair(-1.f, -1.f), y);
+    unsigned long long p = pair(0.009570102207362652f, 0.009570102207362652f);
+    p = fma2(p, f, pair(0.05591785907745361f, 0.05591785907745361f));
+    p = fma2(p, f, pair(0.240247443318367f, 0.240247443318367f));
+    p = fma2(p, f, pair(0.6931217908859253f, 0.6931217908859253f));
+    p = fma2(p, f, pair(0.9999992847442627f, 0.9999992847442627f));
+    const float2 q = halves(p), k = halves(t);
+    return make_float2(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(k.x) << 23)),
+                       __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(k.y) << 23)));
+}
+// NaN if one of them is
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 
 // the low x bits of a word
 __device__ __forceinline__ uint32_t low_bits(int x) { return x >= 32 ? 0xffffffffu : x <= 0 ? 0u : (1u << x) - 1u; }
 
-// What the CTA's roles agree on.  Keys have places u, blocks of 128 of them: place
-// u is slot base + u, base a multiple of 128 so that places keep the slots'
+// What the CTA's roles agree on.  Keys have places u, steps of 64 of them: place
+// u is slot base + u, base a multiple of 64 so that places keep the slots'
 // alignment to pages.  With a window the first slot seen is lo and base lies at
 // least as many places below it as there are first tokens to see: those take the
 // places u < first, and the places between hold nothing.
@@ -216,7 +266,7 @@ struct Job {
     int64_t token0;             // of the batch: first token of tile 0
     int pos0;                   // its slot
     int live;                   // tokens of the CTA that exist
-    int first, lo, base, n, blocks;
+    int first, lo, base, n, steps;
     __device__ __forceinline__ int slot(int u) const { return u < first ? u : base + u; }
     __device__ __forceinline__ bool holds(int u) const { return u < n && (u < first || base + u >= lo); }
 };
@@ -267,26 +317,30 @@ __device__ __forceinline__ bool find_job(const Prefill& P, Job& J) {
     const int end = (int)max((int64_t)0, min((int64_t)J.pos0 + J.live, P.c.capacity()));
     J.lo = P.window > 0 ? min(max(0, J.pos0 - P.window + 1), end) : 0;
     J.first = min(P.sinks, J.lo);
-    J.base = (J.lo - J.first) / TILE * TILE;
+    J.base = (J.lo - J.first) / STEP * STEP;
     J.n = end - J.base;
-    J.blocks = (J.n + TILE - 1) / TILE;
+    J.steps = (J.n + STEP - 1) / STEP;
     return true;
 }
 
-// the blocks a..z-1 that tile t's rows see (a is 0 or 1: its tokens begin at most
-// 128 slots after the CTA's first)
+// the steps a..z-1 that tile t's rows see
 struct Span {
     int tokens, pos, a, z;
+    int f0, f1;                 // steps f0..f1-1: every row sees every place that holds something
 };
 __device__ __forceinline__ Span span_of(const Prefill& P, const Job& J, int t) {
     Span s;
     s.tokens = max(0, min(P.tile_tokens, J.live - t * P.tile_tokens));
     s.pos = J.pos0 + t * P.tile_tokens;
-    s.a = s.z = 0;
+    s.a = s.z = s.f0 = s.f1 = 0;
     if (s.tokens == 0) return s;
     const int ub = min(J.n, s.pos + s.tokens - J.base);               // end of what its last token sees
-    s.z = (max(0, ub) + TILE - 1) / TILE;
-    if (P.window > 0 && P.sinks == 0 && s.z > 1 && J.base + TILE - 1 <= s.pos - P.window) s.a = 1;
+    s.z = (max(0, ub) + STEP - 1) / STEP;
+    // what its first token sees begins here, but for first tokens
+    if (P.window > 0 && P.sinks == 0) s.a = min(s.z, max(0, s.pos - P.window + 1 - J.base) / STEP);
+    // from where its last token's window has begun, to what its first token sees
+    s.f0 = P.window > 0 ? (max(0, s.pos + s.tokens - P.window - J.base) + STEP - 1) / STEP : 0;
+    s.f1 = max(0, s.pos + 1 - J.base) / STEP;
     return s;
 }
 
@@ -301,10 +355,10 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     uint64_t* full = reinterpret_cast<uint64_t*>(sm + Ly::BARS);
     uint64_t* empty = full + SLOTS;
     uint64_t* qbar = empty + SLOTS;
-    uint64_t* sbar = qbar + 1;
-    uint64_t* pbar = sbar + 2;
-    uint64_t* obar = pbar + 2;
-    volatile uint32_t* s_seen = reinterpret_cast<volatile uint32_t*>(sm + Ly::SEEN);
+    uint64_t* sbar = qbar + 1;           // [tile][buffer]
+    uint64_t* pbar = sbar + 4;
+    uint64_t* obar = pbar + 4;
+    volatile uint32_t* s_seen = reinterpret_cast<volatile uint32_t*>(sm + Ly::SEENB);
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort_store;
     volatile int* s_abort = &s_abort_store;
@@ -317,14 +371,16 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     if (threadIdx.x == 0) {
         *s_abort = (smem_u32(sm) & 1023u) ? 2 : 0;
         for (int s = 0; s < SLOTS; ++s) {
-            mbar_init(&full[s], PIECES * 32);
+            mbar_init(&full[s], 2);               // K and V
             mbar_init(&empty[s], 1);
         }
-        mbar_init(qbar, 2 * PIECES * 32);
+        mbar_init(qbar, PRODUCERS);
         for (int t = 0; t < 2; ++t) {
-            mbar_init(&sbar[t], 2);       // the product's commit and the issuing thread
-            mbar_init(&pbar[t], TILE);
-            mbar_init(&obar[t], 1);
+            for (int k = 0; k < 2; ++k) {
+                mbar_init(&sbar[2 * t + k], 2);       // the product's commit and the issuing thread
+                mbar_init(&pbar[2 * t + k], SOFTMAX);
+                mbar_init(&obar[2 * t + k], 1);   // the product of the last step but one, and of the last
+            }
         }
         fence_mbar_init();
     }
@@ -342,33 +398,33 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         // ---------------- producers
         const int w = warp - PRODUCER0;
         const T* q = static_cast<const T*>(P.q);
-        // 32 rows of a tile, one row address a lane, -1 for a row of zeros
-        auto copy = [&](uint32_t dst, int piece, const T* src, int64_t off) {
+        // 32 rows, one row address a lane, -1 for a row of zeros
+        auto copy = [&](auto at, const T* src, int64_t off) {
 #pragma unroll
             for (int it = 0; it < CH; ++it) {
                 const int rr = (it * 32 + lane) / CH, c = (it * 32 + lane) % CH;
                 const int64_t o = __shfl_sync(FULL, (long long)off, rr);
-                cp_async16_or_zero(dst + place(piece * 32 + rr, c), src + (o >= 0 ? o + c * 8 : 0), o >= 0);
+                cp_async16_or_zero(at(rr, c), src + (o >= 0 ? o + c * 8 : 0), o >= 0);
             }
         };
-        int copies = 0;
-        for (int i = w; i < 2 * PIECES; i += PRODUCERS, ++copies) {
-            const int t = i / PIECES, piece = i % PIECES;
+        constexpr int QPIECES = TILE / 32;
+        for (int i = w; i < 2 * QPIECES; i += PRODUCERS) {
+            const int t = i / QPIECES, piece = i % QPIECES;
             const int r = piece * 32 + lane, tok = r / J.heads;
             const int64_t off = tok < sp[t].tokens ? (J.token0 + t * P.tile_tokens + tok) * P.q_token_stride +
                                                          (int64_t)(J.head0 + r % J.heads) * P.q_head_stride
                                                    : -1;
-            copy(base + Ly::Q + t * Ly::TILEB, piece, q, off);
+            copy([&](int rr, int c) { return base + Ly::Q + t * Ly::QB + place<TILE>(piece * 32 + rr, c); }, q, off);
         }
         cp_async_commit();
         cp_async_wait<0>();
         if (P.flip) {
             // each thread turns the chunks that it copied itself
-            for (int i = w; i < 2 * PIECES; i += PRODUCERS)
+            for (int i = w; i < 2 * QPIECES; i += PRODUCERS)
 #pragma unroll
                 for (int it = 0; it < CH; ++it) {
                     const int rr = (it * 32 + lane) / CH, c = (it * 32 + lane) % CH;
-                    uint4* p = reinterpret_cast<uint4*>(sm + Ly::Q + (i / PIECES) * Ly::TILEB + place(i % PIECES * 32 + rr, c));
+                    uint4* p = reinterpret_cast<uint4*>(sm + Ly::Q + (i / QPIECES) * Ly::QB + place<TILE>(i % QPIECES * 32 + rr, c));
                     uint4 x = *p;
                     x.x ^= 0x80008000u;
                     x.y ^= 0x80008000u;
@@ -378,33 +434,46 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
                 }
         }
         fence_async_smem();
-        for (int i = 0; i < copies; ++i) mbar_arrive(qbar);
+        arrive_warp(qbar);
 
         const T* kp = static_cast<const T*>(P.c.k) + (int64_t)J.g * P.c.head_stride;
         const T* vp = static_cast<const T*>(P.c.v) + (int64_t)J.g * P.c.head_stride;
-        // pieces in order: tile K0's four, V0's, K1's, ..; this warp has every third
-        const int total = 2 * J.blocks * PIECES;
-        // the page of this lane's row of piece i, -1 where there is none
-        auto find = [&](int i) -> int {
-            const int u = (i / (2 * PIECES)) * TILE + i % PIECES * 32 + lane;
-            return i < total && J.holds(u) ? P.c.page(J.b, J.slot(u)) : -1;
+        // parts in order: K and V of stage 0, of stage 1, ..; this warp has every third
+        const int total = J.steps ? 2 * (J.steps + 2) : 0;
+        // the step of part i, -1 where its stage has none
+        auto step_of = [&](int i) {
+            const int s = (i & 1) ? (i >> 1) - 2 : (i >> 1);
+            return s < J.steps ? s : -1;
         };
+        // the pages of this lane's rows of part i (lane and lane + 32), -1 where there is none
+        auto find = [&](int i) -> int2 {
+            const int s = step_of(i), u = s * STEP + lane;
+            const bool in = i < total && s >= 0;
+            return make_int2(in && J.holds(u) ? P.c.page(J.b, J.slot(u)) : -1,
+                             in && J.holds(u + 32) ? P.c.page(J.b, J.slot(u + 32)) : -1);
+        };
+        const int in_page = (1 << P.c.shift) - 1;
         int waits[LAG], behind = 0;         // ring slots whose copies by cp.async are in flight
         auto hand_over = [&]() {
             cp_async_wait<0>();
             fence_async_smem();
 #pragma unroll
             for (int k = 0; k < LAG; ++k)
-                if (k < behind) mbar_arrive(&full[waits[k]]);
+                if (k < behind) arrive_warp(&full[waits[k]]);
             behind = 0;
         };
-        int page = find(w);
+        int2 page = find(w);
         for (int i = w; i < total && !*s_abort; i += PRODUCERS) {
-            const int idx = i / PIECES, piece = i % PIECES, slot = idx % SLOTS;
-            const int u = (idx >> 1) * TILE + piece * 32 + lane, at = J.slot(u) & ((1 << P.c.shift) - 1);
-            const unsigned seen = __ballot_sync(FULL, page >= 0);
-            if ((idx & 1) == 0 && lane == 0) s_seen[((idx >> 1) & 7) * 4 + piece] = seen;
-            const uint32_t phase = ((idx / SLOTS) & 1) ^ 1;
+            const int stage = i >> 1, slot = stage % SLOTS, step = step_of(i);
+            const bool is_v = i & 1;
+            const int2 mine = page;
+            page = find(i + PRODUCERS);
+            const unsigned seen0 = __ballot_sync(FULL, mine.x >= 0), seen1 = __ballot_sync(FULL, mine.y >= 0);
+            if (!is_v && lane == 0) {
+                s_seen[(stage % SEEN) * 2] = seen0;
+                s_seen[(stage % SEEN) * 2 + 1] = seen1;
+            }
+            const uint32_t phase = ((stage / SLOTS) & 1) ^ 1;
             if (!__all_sync(FULL, mbar_try_wait(&empty[slot], phase))) {
                 hand_over();                // no room yet: first what is in flight
                 if (!__all_sync(FULL, mbar_wait(&empty[slot], phase))) {
@@ -412,27 +481,38 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
                     break;
                 }
             }
-            const uint32_t dst = base + Ly::RING + slot * Ly::TILEB;
-            if (P.tma && seen == FULL && u - lane >= J.first) {
-                if (lane == 0) mbar_expect_tx(&full[slot], 32 * D * 2);
-                else mbar_arrive(&full[slot]);
-                __syncwarp();
-                if ((lane & (P.tma - 1)) == 0) {
-                    const CUtensorMap* map = (idx & 1) ? &tmv : &tmk;
-#pragma unroll
-                    for (int h = 0; h < D / 64; ++h)
-                        tma_box(dst + h * Ly::ROWB + (piece * 32 + lane) * 128, map, h * 64, at, J.g, page, &full[slot]);
-                }
-                page = find(i + PRODUCERS);
+            if (step < 0) {
+                arrive_warp(&full[slot]);
                 continue;
             }
-            copy(dst, piece, (idx & 1) ? vp : kp, page >= 0 ? page * P.c.page_stride + at * P.c.row_stride : -1);
+            const uint32_t dst = base + Ly::RING + slot * Ly::STAGEB + (is_v ? Ly::KB : 0);
+            const int u = step * STEP + lane;
+            if (P.tma && (seen0 & seen1) == FULL && step * STEP >= J.first) {
+                if (lane == 0) mbar_expect_tx(&full[slot], Ly::KB);
+                __syncwarp();
+                // a lane a box: rows from the lane's own on, a panel of 64 dimensions
+                const CUtensorMap* map = is_v ? &tmv : &tmk;
+                if ((lane & (P.tma - 1)) == 0) {
+                    const int at = (J.base + u) & in_page, at1 = (J.base + u + 32) & in_page;
+#pragma unroll
+                    for (int h = 0; h < D / 64; ++h) {
+                        tma_box(dst + h * (STEP * 128) + lane * 128, map, h * 64, at, J.g, mine.x, &full[slot]);
+                        tma_box(dst + h * (STEP * 128) + (lane + 32) * 128, map, h * 64, at1, J.g, mine.y, &full[slot]);
+                    }
+                }
+                continue;
+            }
+            const T* src = is_v ? vp : kp;
+            auto row = [&](int pg, int place_) -> int64_t {
+                return pg >= 0 ? pg * P.c.page_stride + (int64_t)(J.slot(place_) & in_page) * P.c.row_stride : -1;
+            };
+            copy([&](int rr, int c) { return dst + place<STEP>(rr, c); }, src, row(mine.x, u));
+            copy([&](int rr, int c) { return dst + place<STEP>(32 + rr, c); }, src, row(mine.y, u + 32));
             cp_async_commit();
-            page = find(i + PRODUCERS);
             if (behind == LAG) {
                 cp_async_wait<LAG>();
                 fence_async_smem();
-                mbar_arrive(&full[waits[0]]);
+                arrive_warp(&full[waits[0]]);
 #pragma unroll
                 for (int k = 1; k < LAG; ++k) waits[k - 1] = waits[k];
                 --behind;
@@ -441,62 +521,64 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
             for (int k = 0; k < LAG; ++k)
                 if (k == behind) waits[k] = slot;
             ++behind;
-            if (P.tma) hand_over();         // a boundary's piece: its block waits for it
+            if (P.tma) hand_over();         // a boundary's rows: their step waits for them
             __syncwarp();
         }
         hand_over();
     } else if (warp == MMA_WARP) {
         // ---------------- MMA issuer
-        if (lane == 0) {
-            constexpr uint32_t IS = instr<T>(TILE, false), IO = instr<T>(D, true);
+        const uint32_t tm = __shfl_sync(FULL, tmem, 0);
+        if (elect_one()) {
+            constexpr uint32_t IS = instr<T>(STEP, false), IO = instr<T>(D, true);
+            const uint32_t q0 = desc_k(base + Ly::Q), k0 = desc_k(base + Ly::RING), v0 = desc_v(base + Ly::RING + Ly::KB);
             bool ok = mbar_wait(qbar, 0);
-            for (int j = 0; ok && j <= J.blocks; ++j) {
-                const int ki = 2 * j, vi = 2 * j - 1;
-                if (j > 0) ok = ok && mbar_wait(&full[vi % SLOTS], (vi / SLOTS) & 1);
-                if (j < J.blocks) ok = ok && mbar_wait(&full[ki % SLOTS], (ki / SLOTS) & 1);
+            // stage q: each tile's product with step q - 2's weights, then its logits of step q
+            for (int q = 0; ok && q < J.steps + 2 && J.steps; ++q) {
+                const int slot = q % SLOTS;
+                ok = mbar_wait(&full[slot], (q / SLOTS) & 1);
                 if (!ok) break;
-                tc_fence_after();
-                const uint32_t ks = base + Ly::RING + (ki % SLOTS) * Ly::TILEB;
-                const uint32_t vs = base + Ly::RING + (vi % SLOTS) * Ly::TILEB;
+                const uint32_t kd = k0 + slot * (Ly::STAGEB / 16), vd = v0 + slot * (Ly::STAGEB / 16);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    const uint32_t st = tmem + t * TILE, ot = tmem + 2 * TILE + t * D;
-                    if (j > sp[t].a && j <= sp[t].z) {
-                        ok = ok && mbar_wait(&pbar[t], (j - 1 - sp[t].a) & 1);
+                    const int n = q - 2 - sp[t].a, buf = n & 1;       // of the tile's own steps; n + 2 has the same buffer
+                    const uint32_t st = tm + t * TILE + buf * STEP, ot = tm + 2 * TILE + t * D;
+                    const bool more = n + 2 >= 0 && q < sp[t].z;
+                    if (n >= 0 && q - 2 < sp[t].z) {
+                        ok = mbar_wait(&pbar[2 * t + buf], (n >> 1) & 1);
                         if (!ok) break;
                         tc_fence_after();
+                        mma_ts(ot, st, vd, IO, n > 0 ? 1u : 0u);
 #pragma unroll
-                        for (int k = 0; k < TILE / 16; ++k)
-                            mma_ts(ot, st + k * 8, desc_v(vs + k * 2048), IO, (j - 1 > sp[t].a || k > 0) ? 1u : 0u);
-                        umma_commit(&obar[t]);
+                        for (int k = 1; k < STEP / 16; ++k) mma_ts(ot, st + k * 8, vd + k * 128, IO, 1u);
+                        // done when the logits' commit says so, or at the last two steps its own
+                        if (!more) umma_commit(&obar[2 * t + (q - 2 == sp[t].z - 1)]);
                     }
-                    if (j >= sp[t].a && j < sp[t].z) {
-                        const uint32_t qs = base + Ly::Q + t * Ly::TILEB;
+                    if (more) {
+                        tc_fence_after();
+                        const uint32_t qd = q0 + t * (Ly::QB / 16);
+                        mma_ss(st, qd, kd, IS, 0u);
 #pragma unroll
-                        for (int k = 0; k < D / 16; ++k) {
-                            const uint32_t o = (k >> 2) * Ly::ROWB + (k & 3) * 32;
-                            mma_ss(st, desc_k(qs + o), desc_k(ks + o), IS, k > 0 ? 1u : 0u);
-                        }
-                        umma_commit(&sbar[t]);
-                        mbar_arrive(&sbar[t]);
+                        for (int k = 1; k < D / 16; ++k)
+                            mma_ss(st, qd + (k >> 2) * (TILE * 8) + (k & 3) * 2, kd + (k >> 2) * (STEP * 8) + (k & 3) * 2, IS, 1u);
+                        umma_commit(&sbar[2 * t + buf]);
+                        mbar_arrive(&sbar[2 * t + buf]);
                     }
                 }
                 if (!ok) break;
-                if (j > 0) umma_commit(&empty[vi % SLOTS]);
-                if (j < J.blocks) umma_commit(&empty[ki % SLOTS]);
+                umma_commit(&empty[slot]);
             }
             if (!ok) *s_abort = 1;
         }
         __syncwarp();
     } else {
-        // ---------------- softmax: thread r of the tile's warps is row r
-        const int t = warp >> 2, r = threadIdx.x & (TILE - 1);
+        // ---------------- softmax: a thread is a row
+        const int t = warp / SOFTMAX, r = threadIdx.x & (TILE - 1);
         const Span S = sp[t];
         const int tok = r / J.heads;
         const bool live = tok < S.tokens;
         const int pos = S.pos + min(tok, S.tokens - 1);     // rows of no token see what the last one does
         const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t st = tmem + quarter + t * TILE, ot = tmem + quarter + 2 * TILE + t * D;
+        const uint32_t ot = tmem + quarter + 2 * TILE + t * D;
         // of the places that hold something the row sees u < us and ua <= u, below ub
         const int ub = pos + 1 - J.base, us = max(J.first, P.sinks - J.base);
         const int ua = P.window > 0 ? pos - P.window + 1 - J.base : 0;
@@ -504,40 +586,39 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         float2 l[2] = {{0.f, 0.f}, {0.f, 0.f}};
         bool ok = true;
         for (int j = S.a; j < S.z; ++j) {
-            const int i = j - S.a, u0 = j * TILE;
-            ok = ok && !*s_abort && mbar_wait(&sbar[t], i & 1);
+            const int i = j - S.a, u0 = j * STEP, buf = i & 1;
+            const uint32_t st = tmem + quarter + t * TILE + buf * STEP;
+            ok = ok && !*s_abort && mbar_wait(&sbar[2 * t + buf], (i >> 1) & 1);
             if (!__all_sync(FULL, ok)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
-            uint32_t vis[4];
-            bool whole = true;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int u = u0 + c * 32;
-                vis[c] = low_bits(ub - u) & (low_bits(us - u) | ~low_bits(ua - u)) & s_seen[(j & 7) * 4 + c];
-                whole = whole && vis[c] == 0xffffffffu;
-            }
-            const bool masked = __any_sync(FULL, !whole);
-            uint32_t x[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_get32(st + c * 32, x[c]);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_arrived(x[c]);
+            // the row's logits, and the largest of them
+            uint32_t x[2][32];
+            tmem_get32(st, x[0]);
+            tmem_get32(st + 32, x[1]);
+            const uint2 seen = *reinterpret_cast<const uint2*>(const_cast<const uint32_t*>(s_seen) + (j % SEEN) * 2);
+            const bool masked = j < S.f0 || j >= S.f1 || (seen.x & seen.y) != 0xffffffffu;
+            tmem_arrived(x[0]);
+            tmem_arrived(x[1]);
             if (masked) {
+                const uint32_t sw[2] = {seen.x, seen.y};
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int c = 0; c < 2; ++c) {
+                    const int u = u0 + c * 32;
+                    const uint32_t vis = low_bits(ub - u) & (low_bits(us - u) | ~low_bits(ua - u)) & sw[c];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) x[c][e] = (vis[c] >> e) & 1u ? x[c][e] : __float_as_uint(NEG_INF);
+                    for (int e = 0; e < 32; ++e) x[c][e] = (vis >> e) & 1u ? x[c][e] : __float_as_uint(NEG_INF);
+                }
             }
-            // the row's largest logit
             float a[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
+            for (int e = 0; e < 16; ++e)
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) a[c] = max3(a[c], __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]));
-            const float top = fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])) * P.scale2;
+                for (int c = 0; c < 2; ++c)
+                    a[2 * c + (e & 1)] = max3(a[2 * c + (e & 1)], __uint_as_float(x[c][2 * e]), __uint_as_float(x[c][2 * e + 1]));
+            const float top = max3(max3(a[0], a[1], a[2]), a[3], a[3]) * P.scale2;
             const bool raise = top > m + RAISE || (m == NEG_INF && top != NEG_INF);
             if (__any_sync(FULL, raise)) {
                 const float f = raise && m != NEG_INF ? exp2_fast(m - top) : 1.f;
@@ -545,7 +626,9 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
                 l[0] = make_float2(l[0].x * f, l[0].y * f);
                 l[1] = make_float2(l[1].x * f, l[1].y * f);
                 if (i > 0) {
-                    ok = mbar_wait(&obar[t], (i - 1) & 1);
+                    // the product of step i - 1 is done when the next logits are there, or at the
+                    // last step when its own commit says so
+                    ok = j + 1 < S.z ? mbar_wait(&sbar[2 * t + (buf ^ 1)], ((i + 1) >> 1) & 1) : mbar_wait(&obar[2 * t], 0);
                     if (!__all_sync(FULL, ok)) {
                         ok = false;
                         break;
@@ -563,30 +646,45 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
                 }
             }
             const float off = m == NEG_INF ? 0.f : -m;
-            // weights over the logits' columns
+            // weights over the logits' columns.  The special-function unit gives 4 values a
+            // cycle and scheduler, which would take as long as both products: every
+            // POLY-th pair is computed on the FMA pipe instead, but for masked logits and
+            // those that are not finite, which the polynomial does not know
             const unsigned long long s2 = pair(P.scale2, P.scale2), o2 = pair(off, off);
             unsigned long long l2[2] = {pair(l[0].x, l[0].y), pair(l[1].x, l[1].y)};
+            auto weigh = [&](auto careful) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t p[16];
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t p[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float2 y = halves(fma2(pair(__uint_as_float(x[c][2 * e]), __uint_as_float(x[c][2 * e + 1])), s2, o2));
-                    const float w0 = exp2_fast(y.x), w1 = exp2_fast(y.y);
-                    l2[e & 1] = add2(l2[e & 1], pair(w0, w1));
-                    p[e] = Elem<T>::pack(w0, w1);
+                    for (int e = 0; e < 16; ++e) {
+                        const unsigned long long y2 =
+                            fma2(pair(__uint_as_float(x[c][2 * e]), __uint_as_float(x[c][2 * e + 1])), s2, o2);
+                        float2 w;
+                        if (!decltype(careful)::value && e % POLY == POLY - 1) {
+                            w = exp2_poly(y2);
+                        } else {
+                            const float2 y = halves(y2);
+                            w = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+                        }
+                        l2[e & 1] = add2(l2[e & 1], pair(w.x, w.y));
+                        p[e] = Elem<T>::pack(w.x, w.y);
+                    }
+                    tmem_put16(st + c * 16, p);
                 }
-                tmem_put16(st + c * 16, p);
-            }
+            };
+            const bool plain = !masked && fabsf(top) < __int_as_float(0x7f800000) && m != NEG_INF;
+            if (__all_sync(FULL, plain)) weigh(std::false_type());
+            else weigh(std::true_type());
             l[0] = halves(l2[0]);
             l[1] = halves(l2[1]);
             tmem_stored();
             tc_fence_before();
-            mbar_arrive(&pbar[t]);
+            arrive_warp(&pbar[2 * t + buf]);
         }
         // ---- the rows
-        const int blocks = S.z - S.a;
-        if (blocks > 0) ok = ok && !*s_abort && mbar_wait(&obar[t], (blocks - 1) & 1);
+        const int steps = S.z - S.a;
+        if (steps > 0) ok = ok && !*s_abort && mbar_wait(&obar[2 * t + 1], 0);
         ok = __all_sync(FULL, ok);
         if (!ok) *s_abort = 1;
         tc_fence_after();
@@ -595,23 +693,22 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         const int64_t row = (J.token0 + t * P.tile_tokens + tok) * P.q_heads + J.head0 + r % J.heads;
         uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(P.out) + row * D);
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-            uint32_t x[32];
-            if (blocks > 0) {
-                tmem_get32(ot + c * 32, x);
-                tmem_arrived(x);
+        for (int c = 0; c < D / 16; ++c) {
+            uint32_t z[16];
+            if (steps > 0) {
+                tmem_get16(ot + c * 16, z);
             } else {
 #pragma unroll
-                for (int e = 0; e < 32; ++e) x[e] = 0u;
+                for (int e = 0; e < 16; ++e) z[e] = 0u;
             }
             if (live) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+                for (int e = 0; e < 2; ++e) {
                     uint32_t p[4];
 #pragma unroll
                     for (int y = 0; y < 4; ++y)
-                        p[y] = Elem<T>::pack(__uint_as_float(x[8 * e + 2 * y]) * inv, __uint_as_float(x[8 * e + 2 * y + 1]) * inv);
-                    out[c * 4 + e] = make_uint4(p[0], p[1], p[2], p[3]);
+                        p[y] = Elem<T>::pack(__uint_as_float(z[8 * e + 2 * y]) * inv, __uint_as_float(z[8 * e + 2 * y + 1]) * inv);
+                    out[c * 2 + e] = make_uint4(p[0], p[1], p[2], p[3]);
                 }
             }
         }
