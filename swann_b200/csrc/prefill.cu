@@ -41,8 +41,6 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
-#include <type_traits>
-
 #include "attn.cuh"
 #include "tcgen05.cuh"
 
@@ -57,10 +55,6 @@ constexpr int MMA_WARP = 8, PRODUCER0 = 9, PRODUCERS = 3;   // warps
 constexpr int SOFTMAX = 4;                  // warps of a tile
 constexpr int SEEN = 32;                    // steps whose rows are on record
 constexpr int LAG = 2;                      // parts of a warp in flight behind the one being issued
-#ifndef SWB_POLY
-#define SWB_POLY 99
-#endif
-constexpr int POLY = SWB_POLY;
 constexpr float RAISE = 8.f;                // log2 of how far a maximum may pass the one in use
 
 struct Prefill {
@@ -74,6 +68,7 @@ struct Prefill {
     int flip;                   // scale below 0: the queries' signs are turned instead
     int window, sinks;
     int tma;                    // the maps hold: rows of a box, 0 where there are none
+    int64_t items;              // at most so many
     void* out;
     float* lse;
     int32_t* status;
@@ -87,9 +82,10 @@ struct Layout {
     static constexpr int SLOTS = D == 128 ? 4 : 8;
     static constexpr int Q = 0;                                 // two tiles
     static constexpr int RING = 2 * QB;
-    static constexpr int BARS = RING + SLOTS * STAGEB;          // full, empty, q, s[2][2], p[2][2], o[2][2]
-    static constexpr int SEENB = BARS + (2 * SLOTS + 13) * 8;   // uint32 [SEEN][2], on an 8-byte boundary
-    static constexpr int TOTAL = SEENB + SEEN * 2 * 4;
+    static constexpr int BARS = RING + SLOTS * STAGEB;          // full, empty, q, q let go, s[2][2], p[2][2], o[2][2]
+    static constexpr int SEENB = BARS + (2 * SLOTS + 14) * 8;   // uint32 [SEEN][2], on an 8-byte boundary
+    static constexpr int OUT = (SEENB + SEEN * 2 * 4 + 15) / 16 * 16;   // a warp's 32 rows of 64 dimensions, on their way out
+    static constexpr int TOTAL = OUT + 2 * SOFTMAX * 32 * 128;
 };
 
 // chunk c (16 bytes) of row r of a tile made of panels of 64 dimensions
@@ -226,31 +222,24 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// 2^x of a pair without the special-function unit, for x below 2^22 and not NaN
-// (below -126 as -126): x = n + f with n the nearest integer, found by adding
-// 1.5 * 2^23, and 2^f by the polynomial of degree 4 whose largest relative error
-// on [-1/2, 1/2] is least (2.6e-6; Remez exchange), far below the 16 bits that a
-// weight is rounded to.  n goes into the exponent by an integer addition.
-__device__ __forceinline__ float2 exp2_poly(unsigned long long x) {
-    const float2 lo = halves(x);
-    const unsigned long long y = pair(fmaxf(lo.x, -126.f), fmaxf(lo.y, -126.f));
-    const unsigned long long big = pair(12582912.f, 12582912.f), neg = pair(-12582912.f, -12582912.f);
-    const unsigned long long t = add2(y, big), n = add2(t, neg);
-    const unsigned long long f = fma2(n, pair(-1.f, -1.f), y);
-    unsigned long long p = pair(0.009570102207362652f, 0.009570102207362652f);
-    p = fma2(p, f, pair(0.05591785907745361f, 0.05591785907745361f));
-    p = fma2(p, f, pair(0.240247443318367f, 0.240247443318367f));
-    p = fma2(p, f, pair(0.6931217908859253f, 0.6931217908859253f));
-    p = fma2(p, f, pair(0.9999992847442627f, 0.9999992847442627f));
-    const float2 q = halves(p), k = halves(t);
-    return make_float2(__uint_as_float(__float_as_uint(q.x) + (__float_as_uint(k.x) << 23)),
-                       __uint_as_float(__float_as_uint(q.y) + (__float_as_uint(k.y) << 23)));
-}
-// NaN if one of them is
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
+}
+
+// mbar_wait with nothing on the way of a phase that is complete: the clock is only
+// read after many tries
+__device__ __forceinline__ bool await(uint64_t* bar, uint32_t parity) {
+    long long t0 = 0;
+    for (uint32_t n = 1; !mbar_try_wait(bar, parity); ++n) {
+        if ((n & 255u) == 0) {
+            const long long t = clock64();
+            if (t0 == 0) t0 = t;
+            else if (t - t0 > (1ll << 32)) return false;
+        }
+    }
+    return true;
 }
 
 // the low x bits of a word
@@ -271,9 +260,10 @@ struct Job {
     __device__ __forceinline__ bool holds(int u) const { return u < n && (u < first || base + u >= lo); }
 };
 
-__device__ __forceinline__ bool find_job(const Prefill& P, Job& J) {
+// item `item` of all; false past the last
+__device__ __forceinline__ bool find_job(const Prefill& P, int64_t item, Job& J) {
+    if (item >= P.items) return false;
     const int lane = threadIdx.x & 31;
-    int64_t item = blockIdx.x;
     const int ht = (int)(item % P.head_tiles);
     item /= P.head_tiles;
     J.g = (int)(item % P.c.kv_heads);
@@ -355,7 +345,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     uint64_t* full = reinterpret_cast<uint64_t*>(sm + Ly::BARS);
     uint64_t* empty = full + SLOTS;
     uint64_t* qbar = empty + SLOTS;
-    uint64_t* sbar = qbar + 1;           // [tile][buffer]
+    uint64_t* sbar = qbar + 2;           // [tile][buffer]
     uint64_t* pbar = sbar + 4;
     uint64_t* obar = pbar + 4;
     volatile uint32_t* s_seen = reinterpret_cast<volatile uint32_t*>(sm + Ly::SEENB);
@@ -364,17 +354,14 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     volatile int* s_abort = &s_abort_store;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    Job J;
-    if (!find_job(P, J)) return;
-    const Span sp[2] = {span_of(P, J, 0), span_of(P, J, 1)};
-
     if (threadIdx.x == 0) {
         *s_abort = (smem_u32(sm) & 1023u) ? 2 : 0;
         for (int s = 0; s < SLOTS; ++s) {
             mbar_init(&full[s], 2);               // K and V
             mbar_init(&empty[s], 1);
         }
-        mbar_init(qbar, PRODUCERS);
+        mbar_init(&qbar[0], PRODUCERS);
+        mbar_init(&qbar[1], 1);
         for (int t = 0; t < 2; ++t) {
             for (int k = 0; k < 2; ++k) {
                 mbar_init(&sbar[2 * t + k], 2);       // the product's commit and the issuing thread
@@ -394,6 +381,9 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     const uint32_t tmem = s_tmem;
     const uint32_t base = smem_u32(sm);
 
+    // Every role walks the same jobs.  Barriers are not begun anew with one: stages,
+    // steps and jobs are counted on.
+    int stage0 = 0, jobs = 0;             // stages and jobs with keys before this job
     if (warp >= PRODUCER0) {
         // ---------------- producers
         const int w = warp - PRODUCER0;
@@ -408,6 +398,14 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
             }
         };
         constexpr int QPIECES = TILE / 32;
+        Job J;
+        for (int64_t item = blockIdx.x; !*s_abort && find_job(P, item, J); item += gridDim.x) {
+        if (J.steps == 0) continue;
+        const Span sp[2] = {span_of(P, J, 0), span_of(P, J, 1)};
+        if (!__all_sync(FULL, await(&qbar[1], (jobs & 1) ^ 1))) {
+            *s_abort = 1;
+            break;
+        }
         for (int i = w; i < 2 * QPIECES; i += PRODUCERS) {
             const int t = i / QPIECES, piece = i % QPIECES;
             const int r = piece * 32 + lane, tok = r / J.heads;
@@ -434,12 +432,12 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
                 }
         }
         fence_async_smem();
-        arrive_warp(qbar);
+        arrive_warp(&qbar[0]);
 
         const T* kp = static_cast<const T*>(P.c.k) + (int64_t)J.g * P.c.head_stride;
         const T* vp = static_cast<const T*>(P.c.v) + (int64_t)J.g * P.c.head_stride;
         // parts in order: K and V of stage 0, of stage 1, ..; this warp has every third
-        const int total = J.steps ? 2 * (J.steps + 2) : 0;
+        const int total = 2 * (J.steps + 2);
         // the step of part i, -1 where its stage has none
         auto step_of = [&](int i) {
             const int s = (i & 1) ? (i >> 1) - 2 : (i >> 1);
@@ -464,7 +462,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         };
         int2 page = find(w);
         for (int i = w; i < total && !*s_abort; i += PRODUCERS) {
-            const int stage = i >> 1, slot = stage % SLOTS, step = step_of(i);
+            const int stage = stage0 + (i >> 1), slot = stage % SLOTS, step = step_of(i);
             const bool is_v = i & 1;
             const int2 mine = page;
             page = find(i + PRODUCERS);
@@ -476,7 +474,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
             const uint32_t phase = ((stage / SLOTS) & 1) ^ 1;
             if (!__all_sync(FULL, mbar_try_wait(&empty[slot], phase))) {
                 hand_over();                // no room yet: first what is in flight
-                if (!__all_sync(FULL, mbar_wait(&empty[slot], phase))) {
+                if (!__all_sync(FULL, await(&empty[slot], phase))) {
                     *s_abort = 1;
                     break;
                 }
@@ -525,26 +523,35 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
             __syncwarp();
         }
         hand_over();
+        stage0 += J.steps + 2;
+        ++jobs;
+        }
     } else if (warp == MMA_WARP) {
         // ---------------- MMA issuer
         const uint32_t tm = __shfl_sync(FULL, tmem, 0);
+        int done[2] = {0, 0};             // a tile's steps before this job
+        Job J;
+        for (int64_t item = blockIdx.x; !*s_abort && find_job(P, item, J); item += gridDim.x) {
+        if (J.steps == 0) continue;
+        const Span sp[2] = {span_of(P, J, 0), span_of(P, J, 1)};
         if (elect_one()) {
             constexpr uint32_t IS = instr<T>(STEP, false), IO = instr<T>(D, true);
             const uint32_t q0 = desc_k(base + Ly::Q), k0 = desc_k(base + Ly::RING), v0 = desc_v(base + Ly::RING + Ly::KB);
-            bool ok = mbar_wait(qbar, 0);
+            bool ok = await(&qbar[0], jobs & 1);
             // stage q: each tile's product with step q - 2's weights, then its logits of step q
-            for (int q = 0; ok && q < J.steps + 2 && J.steps; ++q) {
-                const int slot = q % SLOTS;
-                ok = mbar_wait(&full[slot], (q / SLOTS) & 1);
+            for (int q = 0; ok && q < J.steps + 2; ++q) {
+                const int slot = (stage0 + q) % SLOTS;
+                ok = await(&full[slot], ((stage0 + q) / SLOTS) & 1);
                 if (!ok) break;
                 const uint32_t kd = k0 + slot * (Ly::STAGEB / 16), vd = v0 + slot * (Ly::STAGEB / 16);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    const int n = q - 2 - sp[t].a, buf = n & 1;       // of the tile's own steps; n + 2 has the same buffer
+                    // of the tile's own steps, in this job and in all; n + 2 has the same buffer
+                    const int n = q - 2 - sp[t].a, all = done[t] + n, buf = all & 1;
                     const uint32_t st = tm + t * TILE + buf * STEP, ot = tm + 2 * TILE + t * D;
                     const bool more = n + 2 >= 0 && q < sp[t].z;
                     if (n >= 0 && q - 2 < sp[t].z) {
-                        ok = mbar_wait(&pbar[2 * t + buf], (n >> 1) & 1);
+                        ok = await(&pbar[2 * t + buf], (all >> 1) & 1);
                         if (!ok) break;
                         tc_fence_after();
                         mma_ts(ot, st, vd, IO, n > 0 ? 1u : 0u);
@@ -566,14 +573,25 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
                 }
                 if (!ok) break;
                 umma_commit(&empty[slot]);
+                if (q == J.steps - 1) umma_commit(&qbar[1]);
             }
             if (!ok) *s_abort = 1;
         }
         __syncwarp();
+        stage0 += J.steps + 2;
+        ++jobs;
+        done[0] += sp[0].z - sp[0].a;
+        done[1] += sp[1].z - sp[1].a;
+        }
     } else {
         // ---------------- softmax: a thread is a row
         const int t = warp / SOFTMAX, r = threadIdx.x & (TILE - 1);
-        const Span S = sp[t];
+        // (after a wait that gave up these go on, to NaN)
+        int done = 0, ends = 0, pairs = 0;    // the tile's steps, its jobs with a step, and with two, before this job
+        Job J, next;
+        bool more = find_job(P, blockIdx.x, J);
+        for (int64_t item = blockIdx.x; more; J = next) {
+        const Span S = span_of(P, J, t);
         const int tok = r / J.heads;
         const bool live = tok < S.tokens;
         const int pos = S.pos + min(tok, S.tokens - 1);     // rows of no token see what the last one does
@@ -586,9 +604,9 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         float2 l[2] = {{0.f, 0.f}, {0.f, 0.f}};
         bool ok = true;
         for (int j = S.a; j < S.z; ++j) {
-            const int i = j - S.a, u0 = j * STEP, buf = i & 1;
+            const int i = j - S.a, all = done + i, u0 = j * STEP, buf = all & 1;
             const uint32_t st = tmem + quarter + t * TILE + buf * STEP;
-            ok = ok && !*s_abort && mbar_wait(&sbar[2 * t + buf], (i >> 1) & 1);
+            ok = ok && !*s_abort && await(&sbar[2 * t + buf], (all >> 1) & 1);
             if (!__all_sync(FULL, ok)) {
                 ok = false;
                 break;
@@ -598,7 +616,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
             uint32_t x[2][32];
             tmem_get32(st, x[0]);
             tmem_get32(st + 32, x[1]);
-            const uint2 seen = *reinterpret_cast<const uint2*>(const_cast<const uint32_t*>(s_seen) + (j % SEEN) * 2);
+            const uint2 seen = *reinterpret_cast<const uint2*>(const_cast<const uint32_t*>(s_seen) + ((stage0 + j) % SEEN) * 2);
             const bool masked = j < S.f0 || j >= S.f1 || (seen.x & seen.y) != 0xffffffffu;
             tmem_arrived(x[0]);
             tmem_arrived(x[1]);
@@ -628,7 +646,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
                 if (i > 0) {
                     // the product of step i - 1 is done when the next logits are there, or at the
                     // last step when its own commit says so
-                    ok = j + 1 < S.z ? mbar_wait(&sbar[2 * t + (buf ^ 1)], ((i + 1) >> 1) & 1) : mbar_wait(&obar[2 * t], 0);
+                    ok = j + 1 < S.z ? await(&sbar[2 * t + (buf ^ 1)], ((all + 1) >> 1) & 1)
+                                     : await(&obar[2 * t], pairs & 1);
                     if (!__all_sync(FULL, ok)) {
                         ok = false;
                         break;
@@ -646,36 +665,21 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
                 }
             }
             const float off = m == NEG_INF ? 0.f : -m;
-            // weights over the logits' columns.  The special-function unit gives 4 values a
-            // cycle and scheduler, which would take as long as both products: every
-            // POLY-th pair is computed on the FMA pipe instead, but for masked logits and
-            // those that are not finite, which the polynomial does not know
+            // weights over the logits' columns
             const unsigned long long s2 = pair(P.scale2, P.scale2), o2 = pair(off, off);
             unsigned long long l2[2] = {pair(l[0].x, l[0].y), pair(l[1].x, l[1].y)};
-            auto weigh = [&](auto careful) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t p[16];
+            for (int c = 0; c < 2; ++c) {
+                uint32_t p[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const unsigned long long y2 =
-                            fma2(pair(__uint_as_float(x[c][2 * e]), __uint_as_float(x[c][2 * e + 1])), s2, o2);
-                        float2 w;
-                        if (!decltype(careful)::value && e % POLY == POLY - 1) {
-                            w = exp2_poly(y2);
-                        } else {
-                            const float2 y = halves(y2);
-                            w = make_float2(exp2_fast(y.x), exp2_fast(y.y));
-                        }
-                        l2[e & 1] = add2(l2[e & 1], pair(w.x, w.y));
-                        p[e] = Elem<T>::pack(w.x, w.y);
-                    }
-                    tmem_put16(st + c * 16, p);
+                for (int e = 0; e < 16; ++e) {
+                    const float2 y = halves(fma2(pair(__uint_as_float(x[c][2 * e]), __uint_as_float(x[c][2 * e + 1])), s2, o2));
+                    const float w0 = exp2_fast(y.x), w1 = exp2_fast(y.y);
+                    l2[e & 1] = add2(l2[e & 1], pair(w0, w1));
+                    p[e] = Elem<T>::pack(w0, w1);
                 }
-            };
-            const bool plain = !masked && fabsf(top) < __int_as_float(0x7f800000) && m != NEG_INF;
-            if (__all_sync(FULL, plain)) weigh(std::false_type());
-            else weigh(std::true_type());
+                tmem_put16(st + c * 16, p);
+            }
             l[0] = halves(l2[0]);
             l[1] = halves(l2[1]);
             tmem_stored();
@@ -684,35 +688,55 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         }
         // ---- the rows
         const int steps = S.z - S.a;
-        if (steps > 0) ok = ok && !*s_abort && mbar_wait(&obar[2 * t + 1], 0);
+        item += gridDim.x;
+        more = find_job(P, item, next);       // while the last product runs
+        if (steps > 0) ok = ok && !*s_abort && await(&obar[2 * t + 1], ends & 1);
         ok = __all_sync(FULL, ok);
         if (!ok) *s_abort = 1;
         tc_fence_after();
         const float sum = (l[0].x + l[0].y) + (l[1].x + l[1].y);
         const float inv = ok ? (sum == 0.f ? 0.f : 1.f / sum) : __int_as_float(0x7fffffff);
         const int64_t row = (J.token0 + t * P.tile_tokens + tok) * P.q_heads + J.head0 + r % J.heads;
-        uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(P.out) + row * D);
-#pragma unroll 1
-        for (int c = 0; c < D / 16; ++c) {
-            uint32_t z[16];
+        // through shared memory, so that a store writes whole 128-byte lines: 64 dimensions of
+        // 32 rows at a time, chunks placed so that neither side meets in a bank
+        char* box = sm + Ly::OUT + warp * (32 * 128);
+#pragma unroll
+        for (int h = 0; h < D / 64; ++h) {
+            uint32_t z[2][32];
             if (steps > 0) {
-                tmem_get16(ot + c * 16, z);
+                tmem_get32(ot + h * 64, z[0]);
+                tmem_get32(ot + h * 64 + 32, z[1]);
+                tmem_arrived(z[0]);
+                tmem_arrived(z[1]);
             } else {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) z[e] = 0u;
+                for (int e = 0; e < 32; ++e) z[0][e] = z[1][e] = 0u;
             }
-            if (live) {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    uint32_t p[4];
+            for (int c = 0; c < 8; ++c) {
+                uint32_t p[4];
 #pragma unroll
-                    for (int y = 0; y < 4; ++y)
-                        p[y] = Elem<T>::pack(__uint_as_float(z[8 * e + 2 * y]) * inv, __uint_as_float(z[8 * e + 2 * y + 1]) * inv);
-                    out[c * 2 + e] = make_uint4(p[0], p[1], p[2], p[3]);
-                }
+                for (int y = 0; y < 4; ++y)
+                    p[y] = Elem<T>::pack(__uint_as_float(z[c >> 2][(c & 3) * 8 + 2 * y]) * inv,
+                                         __uint_as_float(z[c >> 2][(c & 3) * 8 + 2 * y + 1]) * inv);
+                *reinterpret_cast<uint4*>(box + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(p[0], p[1], p[2], p[3]);
             }
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int rr = i * 4 + (lane >> 3), c = lane & 7;
+                const int64_t to = __shfl_sync(FULL, (long long)(live ? row : -1), rr);
+                const uint4 y = *reinterpret_cast<const uint4*>(box + rr * 128 + ((c ^ (rr & 7)) << 4));
+                if (to >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(P.out) + to * D + h * 64 + c * 8) = y;
+            }
+            __syncwarp();
         }
         if (live) P.lse[row] = !ok ? inv : sum == 0.f ? NEG_INF : (m + log2f(sum)) * LN2;
+        if (J.steps) stage0 += J.steps + 2;
+        done += steps;
+        ends += steps > 0;
+        pairs += steps > 1;
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -756,7 +780,9 @@ int launch(Prefill p, int64_t items, cudaStream_t st) {
     constexpr bool bf16 = Format<T>::F == 1;
     if (rows >= 8 && p.c.pages && pool_map(&mk, p.c.k, p.c, D, bf16, rows) && pool_map(&mv, p.c.v, p.c, D, bf16, rows))
         p.tma = rows;
-    prefill_kernel<T, D><<<(unsigned)items, THREADS, Layout<D>::TOTAL, st>>>(p, mk, mv);
+    p.items = items;
+    const int64_t sms = abi::num_sms();
+    prefill_kernel<T, D><<<(unsigned)(items < sms ? items : sms), THREADS, Layout<D>::TOTAL, st>>>(p, mk, mv);
     return abi::cuda_check("prefill launch");
 }
 
