@@ -68,7 +68,7 @@ struct Prefill {
     int flip;                   // scale below 0: the queries' signs are turned instead
     int window, sinks;
     int tma;                    // the maps hold: rows of a box, 0 where there are none
-    int64_t items;              // at most so many
+    int items;                  // at most so many
     void* out;
     float* lse;
     int32_t* status;
@@ -261,22 +261,24 @@ struct Job {
 };
 
 // item `item` of all; false past the last
-__device__ __forceinline__ bool find_job(const Prefill& P, int64_t item, Job& J) {
+__device__ __forceinline__ bool find_job(const Prefill& P, int item, Job& J) {
     if (item >= P.items) return false;
     const int lane = threadIdx.x & 31;
-    const int ht = (int)(item % P.head_tiles);
-    item /= P.head_tiles;
-    J.g = (int)(item % P.c.kv_heads);
-    int64_t left = item / P.c.kv_heads;
+    int left = item / P.head_tiles;
+    const int ht = item - left * P.head_tiles;
+    J.g = left % P.c.kv_heads;
+    left /= P.c.kv_heads;
     const int step = 2 * P.tile_tokens;
     // the sequences' tiles end to end, 32 sequences at a time
-    int b = -1, tiles = 0;
+    int b = -1, tiles = 0, s0 = 0, ntok = 0, length = 0;
     for (int b0 = 0; b0 < P.c.seqs; b0 += 32) {
         const int mine = b0 + lane;
-        int t = 0;
+        int t = 0, from = 0, n = 0, held = 0;
         if (mine < P.c.seqs) {
-            const int64_t n = clamp_start(P.starts, mine + 1, P.tokens) - clamp_start(P.starts, mine, P.tokens);
-            t = n > 0 ? (int)((n + step - 1) / step) : 0;
+            from = (int)clamp_start(P.starts, mine, P.tokens);
+            n = (int)clamp_start(P.starts, mine + 1, P.tokens) - from;
+            held = P.c.lengths[mine];
+            t = n > 0 ? (n + step - 1) / step : 0;
         }
         int sum = t;
 #pragma unroll
@@ -290,20 +292,21 @@ __device__ __forceinline__ bool find_job(const Prefill& P, int64_t item, Job& J)
             b = b0 + src;
             tiles = __shfl_sync(FULL, t, src);
             left -= __shfl_sync(FULL, sum, src) - tiles;
+            s0 = __shfl_sync(FULL, from, src);
+            ntok = __shfl_sync(FULL, n, src);
+            length = __shfl_sync(FULL, held, src);
             break;
         }
         left -= __shfl_sync(FULL, sum, 31);
     }
     if (b < 0) return false;
-    const int64_t s0 = clamp_start(P.starts, b, P.tokens);
-    const int ntok = (int)(clamp_start(P.starts, b + 1, P.tokens) - s0);
-    const int tile = tiles - 1 - (int)left;          // the longest rows first
+    const int tile = tiles - 1 - left;               // the longest rows first
     J.b = b;
     J.heads = min(P.tile_heads, P.group - ht * P.tile_heads);
     J.head0 = J.g * P.group + ht * P.tile_heads;
-    J.token0 = s0 + (int64_t)tile * step;
+    J.token0 = s0 + tile * step;
     J.live = min(step, ntok - tile * step);
-    J.pos0 = P.c.lengths[b] - ntok + tile * step;
+    J.pos0 = length - ntok + tile * step;
     const int end = (int)max((int64_t)0, min((int64_t)J.pos0 + J.live, P.c.capacity()));
     J.lo = P.window > 0 ? min(max(0, J.pos0 - P.window + 1), end) : 0;
     J.first = min(P.sinks, J.lo);
@@ -399,7 +402,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         };
         constexpr int QPIECES = TILE / 32;
         Job J;
-        for (int64_t item = blockIdx.x; !*s_abort && find_job(P, item, J); item += gridDim.x) {
+        for (int item = blockIdx.x; !*s_abort && find_job(P, item, J); item += gridDim.x) {
         if (J.steps == 0) continue;
         const Span sp[2] = {span_of(P, J, 0), span_of(P, J, 1)};
         if (!__all_sync(FULL, await(&qbar[1], (jobs & 1) ^ 1))) {
@@ -531,7 +534,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         const uint32_t tm = __shfl_sync(FULL, tmem, 0);
         int done[2] = {0, 0};             // a tile's steps before this job
         Job J;
-        for (int64_t item = blockIdx.x; !*s_abort && find_job(P, item, J); item += gridDim.x) {
+        for (int item = blockIdx.x; !*s_abort && find_job(P, item, J); item += gridDim.x) {
         if (J.steps == 0) continue;
         const Span sp[2] = {span_of(P, J, 0), span_of(P, J, 1)};
         if (elect_one()) {
@@ -590,7 +593,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         int done = 0, ends = 0, pairs = 0;    // the tile's steps, its jobs with a step, and with two, before this job
         Job J, next;
         bool more = find_job(P, blockIdx.x, J);
-        for (int64_t item = blockIdx.x; more; J = next) {
+        for (int item = blockIdx.x; more; J = next) {
         const Span S = span_of(P, J, t);
         const int tok = r / J.heads;
         const bool live = tok < S.tokens;
@@ -780,7 +783,7 @@ int launch(Prefill p, int64_t items, cudaStream_t st) {
     constexpr bool bf16 = Format<T>::F == 1;
     if (rows >= 8 && p.c.pages && pool_map(&mk, p.c.k, p.c, D, bf16, rows) && pool_map(&mv, p.c.v, p.c, D, bf16, rows))
         p.tma = rows;
-    p.items = items;
+    p.items = (int)items;
     const int64_t sms = abi::num_sms();
     prefill_kernel<T, D><<<(unsigned)(items < sms ? items : sms), THREADS, Layout<D>::TOTAL, st>>>(p, mk, mv);
     return abi::cuda_check("prefill launch");
@@ -826,7 +829,7 @@ extern "C" int swb_attn_prefill(const void* q, int64_t q_token_stride, int64_t q
     // every sequence may end in a tile that is not full
     const int64_t step = 2 * p.tile_tokens;
     const int64_t items = ((tokens + step - 1) / step + p.c.seqs) * p.c.kv_heads * p.head_tiles;
-    if (items >= ((int64_t)1 << 31)) return abi::fail(SWB_ERR_ARG, "too many tokens in one call");
+    if (items >= ((int64_t)1 << 30) || tokens >= ((int64_t)1 << 31) - 256) return abi::fail(SWB_ERR_ARG, "too many tokens in one call");
     cudaStream_t st = (cudaStream_t)stream;
     if (cache->dtype == SWB_F16)
         return cache->head_dim == 64 ? pre::launch<__half, 64>(p, items, st) : pre::launch<__half, 128>(p, items, st);
