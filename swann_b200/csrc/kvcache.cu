@@ -4,9 +4,8 @@
 // eps) * w) and rotated by its position, keys and values written to their slot.
 // One pass: every element is read once and written once, in 32 bits between, so
 // the kernel is bound by those bytes (and, for a few tokens, by its launch).  A
-// 16-byte chunk of a head is a lane's; the lanes of a head sum its squares by
-// shuffles, and a lane gets its rotation partner's chunk from the lane that holds
-// it.
+// lane has two 16-byte chunks of a head, rotation partners; the lanes of a head
+// sum its squares by shuffles.  9721 tokens of 48 heads of 128: 54 us, 4.5 TB/s.
 //
 // swb_kv_evict: per key head, the `budget` slots with the largest accumulated
 // weight stay (first and newest positions before all), and rows that lie beyond
@@ -50,119 +49,145 @@ struct Append {
 };
 
 constexpr int APPEND_THREADS = 128;
-constexpr int APPEND_HEADS = 4;      // heads of a thread, their loads in flight together
+constexpr int APPEND_HEADS = 3;      // heads of a thread, their loads in flight together
+constexpr int APPEND_CTAS = 7;       // an SM: 54 us at 72 registers, 59 at 5 CTAs, 67 unbounded
 
-// A token, and APPEND_HEADS * (128 threads / lanes of a head) of its heads, a
-// CTA: a thread has the same chunk of each of its heads, so the token's place and
-// its rotation are read once.
+template <typename T>
+__device__ __forceinline__ void wide8(const uint4& r, float (&x)[8]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float2 f = Elem<T>::wide(w[e]);
+        x[2 * e] = f.x;
+        x[2 * e + 1] = f.y;
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+    return make_uint4(Elem<T>::pack(x[0], x[1]), Elem<T>::pack(x[2], x[3]), Elem<T>::pack(x[4], x[5]),
+                      Elem<T>::pack(x[6], x[7]));
+}
+
+// A CTA a token, so that its place and its angles are read once.  A thread has the
+// same two 16-byte chunks of each of its heads: of the dimensions that are rotated
+// by halves those that are turned into one another, so nothing is exchanged but the
+// sum of squares.  (A chunk a thread, the partner's by shuffles: 75 us for 9721
+// tokens of 48 heads of 128.)
 template <typename T, int D>
-__global__ void __launch_bounds__(APPEND_THREADS) append_kernel(const __grid_constant__ Append P) {
-    constexpr int LPH = D / 8, HP = APPEND_THREADS / LPH, U = APPEND_HEADS;
+__global__ void __launch_bounds__(APPEND_THREADS, APPEND_CTAS) append_kernel(const __grid_constant__ Append P) {
+    constexpr int LPH = D / 16, HP = APPEND_THREADS / LPH, U = APPEND_HEADS;
     const int heads = P.q_heads + 2 * P.c.kv_heads, keys = P.q_heads, values = P.q_heads + P.c.kv_heads;
     const int64_t tok = blockIdx.x;
-    const int c = threadIdx.x % LPH;
-    const int h0 = blockIdx.y * (HP * U) + threadIdx.x / LPH;
+    const int idx = threadIdx.x % LPH, hc = P.half / 8;
+    // chunks idx and idx + hc are rotated into one another; the others go two by two
+    const bool halves = idx < hc && !P.interleaved;
+    const int c0 = halves ? idx : 2 * idx, c1 = halves ? idx + hc : 2 * idx + 1;
+    const bool turned = idx < hc;
 
-    uint4 raw[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-        const int h = h0 + i * HP;
-        const T* src = h < keys ? static_cast<const T*>(P.q) + tok * P.q_ts + h * P.q_hs
-                     : h < values ? static_cast<const T*>(P.k) + tok * P.k_ts + (h - keys) * P.k_hs
-                                  : static_cast<const T*>(P.v) + tok * P.v_ts + (h - values) * P.v_hs;
-        raw[i] = h < heads ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0u, 0u, 0u, 0u);
-    }
-
-    // the token's sequence: the last one that starts at or before it
-    int b = 0, hi = P.c.seqs;
-    while (hi - b > 1) {
-        const int mid = (b + hi) >> 1;
-        if (P.starts[mid] <= tok) b = mid;
-        else hi = mid;
-    }
-    const int64_t slot = (int64_t)P.c.lengths[b] - (P.starts[b + 1] - tok);
-    const int64_t pos = P.positions ? (int64_t)P.positions[tok] : slot;
-    const int64_t row = slot >= 0 && slot < P.c.capacity() ? P.c.row(b, (int)slot) : -1;
-
-    // this chunk's rotation: 8 angles (halves) or 4 (neighbours)
-    const int hc = P.half / 8;
-    const bool turned = c < 2 * hc, lower = c < hc;
-    const int partner = turned && !P.interleaved ? (lower ? c + hc : c - hc) : c;
+    int b = 0;
+    int64_t slot = 0, pos = 0, row = 0;
     float co[8], si[8];
-    if (turned) {
-        if (pos >= 0 && pos < P.table_rows) {
-            const int64_t at = pos * P.half + (P.interleaved ? c * 4 : (lower ? c : c - hc) * 8);
-            *reinterpret_cast<float4*>(co) = *reinterpret_cast<const float4*>(P.cos + at);
-            *reinterpret_cast<float4*>(si) = *reinterpret_cast<const float4*>(P.sin + at);
-            if (!P.interleaved) {
-                *reinterpret_cast<float4*>(co + 4) = *reinterpret_cast<const float4*>(P.cos + at + 4);
-                *reinterpret_cast<float4*>(si + 4) = *reinterpret_cast<const float4*>(P.sin + at + 4);
-            }
-        } else {                                            // a position outside the tables gives NaN
+    for (int hb = threadIdx.x / LPH; hb - (int)threadIdx.x / LPH < heads; hb += HP * U) {
+        uint4 raw[U][2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) co[e] = si[e] = __int_as_float(0x7fffffff);
-        }
-    }
-    const int base = (threadIdx.x & 31) / LPH * LPH;
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-        const int h = h0 + i * HP;
-        const bool is_q = h < keys, is_v = h >= values;
-        float x[8];
-        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float2 f = Elem<T>::wide(w[e]);
-            x[2 * e] = f.x;
-            x[2 * e + 1] = f.y;
-            ss += f.x * f.x;
-            ss += f.y * f.y;
-        }
-#pragma unroll
-        for (int s = LPH / 2; s > 0; s >>= 1) ss += __shfl_xor_sync(FULL, ss, s);
-        const T* weight = static_cast<const T*>(is_v ? nullptr : is_q ? P.q_weight : P.k_weight);
-        if (weight) {
-            const float inv = rsqrtf(ss * (1.f / D) + P.eps);
-            const uint4 wr = *reinterpret_cast<const uint4*>(weight + c * 8);
-            const uint32_t v[4] = {wr.x, wr.y, wr.z, wr.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 f = Elem<T>::wide(v[e]);
-                x[2 * e] *= inv * f.x;
-                x[2 * e + 1] *= inv * f.y;
+        for (int i = 0; i < U; ++i) {
+            const int h = hb + i * HP;
+            const T* src = h < keys ? static_cast<const T*>(P.q) + tok * P.q_ts + h * P.q_hs
+                         : h < values ? static_cast<const T*>(P.k) + tok * P.k_ts + (h - keys) * P.k_hs
+                                      : static_cast<const T*>(P.v) + tok * P.v_ts + (h - values) * P.v_hs;
+            raw[i][0] = raw[i][1] = make_uint4(0u, 0u, 0u, 0u);
+            if (h < heads) {
+                raw[i][0] = *reinterpret_cast<const uint4*>(src + c0 * 8);
+                raw[i][1] = *reinterpret_cast<const uint4*>(src + c1 * 8);
             }
         }
-        if (P.interleaved) {
-            if (turned && !is_v) {
+        if (hb < HP) {
+            // the token's sequence: the last one that starts at or before it
+            int hi = P.c.seqs;
+            while (hi - b > 1) {
+                const int mid = (b + hi) >> 1;
+                if (P.starts[mid] <= tok) b = mid;
+                else hi = mid;
+            }
+            slot = (int64_t)P.c.lengths[b] - (P.starts[b + 1] - tok);
+            pos = P.positions ? (int64_t)P.positions[tok] : slot;
+            row = slot >= 0 && slot < P.c.capacity() ? P.c.row(b, (int)slot) : -1;
+            if (turned) {
+                if (pos >= 0 && pos < P.table_rows) {
+                    const float4* pc = reinterpret_cast<const float4*>(P.cos + pos * P.half + idx * 8);
+                    const float4* ps = reinterpret_cast<const float4*>(P.sin + pos * P.half + idx * 8);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float a = x[2 * e], z = x[2 * e + 1];
-                    x[2 * e] = a * co[e] - z * si[e];
-                    x[2 * e + 1] = z * co[e] + a * si[e];
+                    for (int e = 0; e < 2; ++e) {
+                        *reinterpret_cast<float4*>(co + 4 * e) = pc[e];
+                        *reinterpret_cast<float4*>(si + 4 * e) = ps[e];
+                    }
+                } else {                                    // a position outside the tables gives NaN
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) co[e] = si[e] = __int_as_float(0x7fffffff);
                 }
             }
-        } else {
-            float y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = __shfl_sync(FULL, x[e], base + partner);
-            if (turned && !is_v) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = lower ? x[e] * co[e] - y[e] * si[e] : x[e] * co[e] + y[e] * si[e];
-            }
         }
-        if (h >= heads) continue;
-        if (weight || (turned && !is_v))
-            raw[i] = make_uint4(Elem<T>::pack(x[0], x[1]), Elem<T>::pack(x[2], x[3]), Elem<T>::pack(x[4], x[5]),
-                                Elem<T>::pack(x[6], x[7]));
-        if (is_q) {
-            *reinterpret_cast<uint4*>(static_cast<T*>(P.out) + (tok * P.q_heads + h) * D + c * 8) = raw[i];
-        } else if (row >= 0) {
-            const int kh = is_v ? h - values : h - keys;
-            T* pool = static_cast<T*>(const_cast<void*>(is_v ? P.c.v : P.c.k));
-            *reinterpret_cast<uint4*>(pool + row + kh * P.c.head_stride + c * 8) = raw[i];
-            if (P.slot_positions && !is_v && c == 0 && slot < P.width)
-                P.slot_positions[((int64_t)b * P.c.kv_heads + kh) * P.width + slot] = (int32_t)pos;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int h = hb + i * HP;
+            const bool is_q = h < keys, is_v = h >= values;
+            const T* weight = static_cast<const T*>(is_v ? nullptr : is_q ? P.q_weight : P.k_weight);
+            const bool turn = turned && !is_v;
+            float x[8], y[8];
+            wide8<T>(raw[i][0], x);
+            wide8<T>(raw[i][1], y);
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss += x[e] * x[e] + y[e] * y[e];
+#pragma unroll
+            for (int s = LPH / 2; s > 0; s >>= 1) ss += __shfl_xor_sync(FULL, ss, s);
+            if (weight) {
+                const float inv = rsqrtf(ss * (1.f / D) + P.eps);
+                float w0[8], w1[8];
+                wide8<T>(*reinterpret_cast<const uint4*>(weight + c0 * 8), w0);
+                wide8<T>(*reinterpret_cast<const uint4*>(weight + c1 * 8), w1);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] *= inv * w0[e];
+                    y[e] *= inv * w1[e];
+                }
+            }
+            if (turn) {
+                if (P.interleaved) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float a0 = x[2 * e], b0 = x[2 * e + 1], a1 = y[2 * e], b1 = y[2 * e + 1];
+                        x[2 * e] = a0 * co[e] - b0 * si[e];
+                        x[2 * e + 1] = b0 * co[e] + a0 * si[e];
+                        y[2 * e] = a1 * co[e + 4] - b1 * si[e + 4];
+                        y[2 * e + 1] = b1 * co[e + 4] + a1 * si[e + 4];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float a0 = x[e], b0 = y[e];
+                        x[e] = a0 * co[e] - b0 * si[e];
+                        y[e] = b0 * co[e] + a0 * si[e];
+                    }
+                }
+            }
+            if (h >= heads) continue;
+            if (weight || turn) {
+                raw[i][0] = pack8<T>(x);
+                raw[i][1] = pack8<T>(y);
+            }
+            T* dst;
+            if (is_q) {
+                dst = static_cast<T*>(P.out) + (tok * P.q_heads + h) * D;
+            } else {
+                if (row < 0) continue;
+                const int kh = is_v ? h - values : h - keys;
+                dst = static_cast<T*>(const_cast<void*>(is_v ? P.c.v : P.c.k)) + row + kh * P.c.head_stride;
+                if (P.slot_positions && !is_v && idx == 0 && slot < P.width)
+                    P.slot_positions[((int64_t)b * P.c.kv_heads + kh) * P.width + slot] = (int32_t)pos;
+            }
+            *reinterpret_cast<uint4*>(dst + c0 * 8) = raw[i][0];
+            *reinterpret_cast<uint4*>(dst + c1 * 8) = raw[i][1];
         }
     }
 }
@@ -187,6 +212,7 @@ struct Evict {
 constexpr int SELECT_THREADS = 1024;
 constexpr int SELECT_WARPS = SELECT_THREADS / 32;
 constexpr int BINS = 2048;
+constexpr int COPIES = 8;        // of a bin: weights share exponents, so neighbouring lanes would meet in one
 
 // a slot's key: larger stays.  First and newest positions above every weight,
 // then the weights as numbers, NaN below all of them.
@@ -220,7 +246,9 @@ static_assert(SELECT_WARPS == 32, "one lane a warp");
 // read again in each pass
 template <int KEEP>
 __global__ void __launch_bounds__(SELECT_THREADS) select_kernel(const __grid_constant__ Evict P) {
-    __shared__ int s_hist[BINS], s_warp[SELECT_WARPS], s_pick[2];
+    extern __shared__ int4 s_bins[];                       // [BINS][COPIES] counts
+    int* s_hist = reinterpret_cast<int*>(s_bins);
+    __shared__ int s_warp[SELECT_WARPS], s_pick[2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t head = blockIdx.x;                       // sequence * kv_heads + key head
     const int b = (int)(head / P.c.kv_heads);
@@ -232,10 +260,6 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_kernel(const __grid_con
     int32_t* np = P.new_positions + head * P.width;
     const int64_t fresh = (int64_t)P.seen[b] - P.recent;
     if (threadIdx.x == 0 && head % P.c.kv_heads == 0) P.new_lengths[b] = min(n, m);
-    for (int64_t j = min(n, m) + threadIdx.x; j < P.width; j += SELECT_THREADS) {
-        nw[j] = 0.f;
-        np[j] = -1;
-    }
     if (n <= m) {
         for (int j = threadIdx.x; j < n; j += SELECT_THREADS) {
             nw[j] = w[j];
@@ -246,19 +270,30 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_kernel(const __grid_con
     }
     // this warp's slots: 32 at a time from j0 on
     const int steps = (n + SELECT_THREADS - 1) / SELECT_THREADS, j0 = warp * steps * 32 + lane;
-    auto key_at = [&](int i) -> uint32_t {
-        const int j = j0 + i * 32;
-        return j < n ? keep_key(w[j], pos[j], P.sinks, fresh) : 0u;
-    };
+    const int mine = max(0, min(steps, (n - j0 + 31) / 32));      // of this lane
+    auto key_at = [&](int i) -> uint32_t { return keep_key(w[j0 + i * 32], pos[j0 + i * 32], P.sinks, fresh); };
     uint32_t held[KEEP];
+    constexpr int BATCH = KEEP < 8 ? KEEP : 8;             // slots whose loads are in flight together
 #pragma unroll
-    for (int i = 0; i < KEEP; ++i) held[i] = i < steps ? key_at(i) : 0u;
-    // f(step, key, whether there is a slot) for this warp's steps, in order
+    for (int i0 = 0; i0 < KEEP; i0 += BATCH) {
+        float wv[BATCH];
+        int pv[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const bool in = i0 + i < mine;
+            wv[i] = in ? w[j0 + (i0 + i) * 32] : 0.f;
+            pv[i] = in ? pos[j0 + (i0 + i) * 32] : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) held[i0 + i] = keep_key(wv[i], pv[i], P.sinks, fresh);
+    }
+    // f(slot, key) for this lane's slots; every lane takes part in every step, with
+    // whether it has a slot there
     auto each = [&](auto f) {
 #pragma unroll
         for (int i = 0; i < KEEP; ++i)
-            if (i < steps) f(i, held[i], j0 + i * 32 < n);
-        for (int i = KEEP; i < steps; ++i) f(i, key_at(i), j0 + i * 32 < n);
+            if (i < steps) f(j0 + i * 32, held[i], i < mine);
+        for (int i = KEEP; i < steps; ++i) f(j0 + i * 32, i < mine ? key_at(i) : 0u, i < mine);
     };
 
     // the m-th largest key, some bits at a time from the top; `need` of the keys
@@ -269,27 +304,33 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_kernel(const __grid_con
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const uint32_t digit = pass == 2 ? 1023u : 2047u;
-        s_hist[threadIdx.x] = 0;
-        s_hist[threadIdx.x + 1024] = 0;
+#pragma unroll
+        for (int i = 0; i < BINS * COPIES / 4 / SELECT_THREADS; ++i)
+            s_bins[threadIdx.x + i * SELECT_THREADS] = make_int4(0, 0, 0, 0);
         __syncthreads();
         each([&](int, uint32_t key, bool there) {
-            if (there && (key & mask) == prefix) atomicAdd(&s_hist[(key >> shift) & digit], 1);
+            if (there && (key & mask) == prefix) atomicAdd(&s_hist[((key >> shift) & digit) * COPIES + (lane & (COPIES - 1))], 1);
         });
         __syncthreads();
         // bins from the largest down, two a thread: the one that holds the need-th
-        const int hi = s_hist[BINS - 1 - 2 * threadIdx.x], lo = s_hist[BINS - 2 - 2 * threadIdx.x];
-        int sum = hi + lo;
+        int count[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int4 x = s_bins[(BINS - 1 - 2 * threadIdx.x - k) * 2], y = s_bins[(BINS - 1 - 2 * threadIdx.x - k) * 2 + 1];
+            count[k] = (x.x + x.y) + (x.z + x.w) + (y.x + y.y) + (y.z + y.w);
+        }
+        int sum = count[0] + count[1];
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) {
             const int z = __shfl_up_sync(FULL, sum, s);
             if (lane >= s) sum += z;
         }
         int total;
-        const int before = warps_before(__shfl_sync(FULL, sum, 31), s_warp, total) + sum - hi - lo;
-        if (before < need && need <= before + hi + lo) {
-            const bool top = need <= before + hi;
+        const int before = warps_before(__shfl_sync(FULL, sum, 31), s_warp, total) + sum - count[0] - count[1];
+        if (before < need && need <= before + count[0] + count[1]) {
+            const bool top = need <= before + count[0];
             s_pick[0] = BINS - 1 - 2 * threadIdx.x - (top ? 0 : 1);
-            s_pick[1] = need - before - (top ? 0 : hi);
+            s_pick[1] = need - before - (top ? 0 : count[0]);
         }
         __syncthreads();
         prefix |= (uint32_t)s_pick[0] << shift;
@@ -297,61 +338,82 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_kernel(const __grid_con
         need = s_pick[1];
     }
 
-    // in slot order: equal keys to the lowest slots
-    int total, mine = 0;
-    each([&](int, uint32_t key, bool there) { mine += __popc(__ballot_sync(FULL, there && key == prefix)); });
-    const int ties0 = warps_before(mine, s_warp, total);
-    int ties = ties0, free = 0, late = 0;
-    auto keeps = [&](uint32_t key, bool there) -> bool {
-        const unsigned t = __ballot_sync(FULL, there && key == prefix);
-        const bool keep = there && (key > prefix || (key == prefix && ties + __popc(t & lanemask_lt()) < need));
-        ties += __popc(t);
-        return keep;
-    };
-    each([&](int i, uint32_t key, bool there) {
-        const bool keep = keeps(key, there);
-        const int j = j0 + i * 32;
-        free += __popc(__ballot_sync(FULL, j < m && !keep));
-        late += __popc(__ballot_sync(FULL, j >= m && keep));
+    // equal keys stay in the lowest slots: up to the slot of the need-th of them
+    int total, ties = 0;
+    each([&](int, uint32_t key, bool there) { ties += there && key == prefix; });
+    const int before = warps_before((int)__reduce_add_sync(FULL, ties), s_warp, total);
+    if (threadIdx.x == 0) s_pick[0] = 0x7fffffff;
+    __syncthreads();
+    if (total > need) {
+        int seen = before;
+        each([&](int j, uint32_t key, bool there) {
+            const unsigned t = __ballot_sync(FULL, there && key == prefix);
+            if (there && key == prefix && seen + __popc(t & lanemask_lt()) == need - 1) s_pick[0] = j;
+            seen += __popc(t);
+        });
+    }
+    __syncthreads();
+    const int last = s_pick[0];
+    auto keeps = [&](int j, uint32_t key, bool there) { return there && (key > prefix || (key == prefix && j <= last)); };
+    // ranks of the free places and of the rows to move, in slot order
+    int free = 0, late = 0, moved;
+    each([&](int j, uint32_t key, bool there) {
+        const bool keep = keeps(j, key, there);
+        free += there && j < m && !keep;
+        late += j >= m && keep;
     });
-    int moved;
-    free = warps_before(free, s_warp, total);
-    late = warps_before(late, s_warp, moved);
-    ties = ties0;
+    free = warps_before((int)__reduce_add_sync(FULL, free), s_warp, total);
+    late = warps_before((int)__reduce_add_sync(FULL, late), s_warp, moved);
     int32_t* from = P.moves + head * 2 * m;
     int32_t* to = from + m;
-    each([&](int i, uint32_t key, bool there) {
-        const bool keep = keeps(key, there);
-        const int j = j0 + i * 32;
-        const unsigned f = __ballot_sync(FULL, j < m && !keep), l = __ballot_sync(FULL, j >= m && keep);
-        if (j < m && keep) {
-            nw[j] = w[j];
-            np[j] = pos[j];
+    each([&](int j, uint32_t key, bool there) {
+        const bool keep = keeps(j, key, there);
+        const unsigned f = __ballot_sync(FULL, there && j < m && !keep), l = __ballot_sync(FULL, j >= m && keep);
+        if (there && j < m) {
+            if (keep) {
+                nw[j] = w[j];
+                np[j] = pos[j];
+            } else {
+                to[free + __popc(f & lanemask_lt())] = j;
+            }
         }
-        if (j < m && !keep) to[free + __popc(f & lanemask_lt())] = j;
         if (j >= m && keep) from[late + __popc(l & lanemask_lt())] = j;
         free += __popc(f);
         late += __popc(l);
     });
-    __syncthreads();
-    for (int i = threadIdx.x; i < moved; i += SELECT_THREADS) {
-        nw[to[i]] = w[from[i]];
-        np[to[i]] = pos[from[i]];
-    }
     if (threadIdx.x == 0) P.counts[head] = moved;
 }
 
 constexpr int MOVE_THREADS = 256;
-constexpr int MOVE_ROWS = 32;      // rows of a block
+constexpr int MOVE_ROWS = 32;      // rows of a CTA
+constexpr int MOVE_SLOTS = 4096;   // slots beyond the budget of a CTA
 
+// the rows that move, with their weights and positions, and the slots that now hold nothing
 __global__ void __launch_bounds__(MOVE_THREADS) move_kernel(const __grid_constant__ Evict P) {
-    dependency_wait();
     const int64_t head = blockIdx.x;
     const int b = (int)(head / P.c.kv_heads), g = (int)(head % P.c.kv_heads);
+    const float* w = P.weights + head * P.width;
+    const int32_t* pos = P.positions + head * P.width;
+    float* nw = P.new_weights + head * P.width;
+    int32_t* np = P.new_positions + head * P.width;
+    {
+        const int64_t held = max(0, min(P.c.lengths[b], P.budget));
+        const int64_t j0 = held + (int64_t)blockIdx.y * MOVE_SLOTS, j1 = min(P.width, j0 + MOVE_SLOTS);
+        for (int64_t j = j0 + threadIdx.x; j < j1; j += MOVE_THREADS) {
+            nw[j] = 0.f;
+            np[j] = -1;
+        }
+    }
+    dependency_wait();
     const int n = P.counts[head];
     const int32_t* from = P.moves + head * 2 * P.budget;
     const int32_t* to = from + P.budget;
     const int i0 = blockIdx.y * MOVE_ROWS, i1 = min(n, i0 + MOVE_ROWS);
+    if (i0 + (int)threadIdx.x < i1) {
+        const int a = from[i0 + threadIdx.x], z = to[i0 + threadIdx.x];
+        nw[z] = w[a];
+        np[z] = pos[a];
+    }
     for (int x = threadIdx.x; x < (i1 - i0) * P.row_chunks; x += MOVE_THREADS) {
         const int i = i0 + x / P.row_chunks, c = x % P.row_chunks;
         const int64_t a = P.c.row(b, from[i]), z = P.c.row(b, to[i]);
@@ -373,10 +435,8 @@ using namespace swb::attn;
 
 template <typename T, int D>
 static int launch_append(const Append& a, cudaStream_t st) {
-    constexpr int per = APPEND_THREADS / (D / 8) * APPEND_HEADS;
-    const int64_t by = ((int64_t)a.q_heads + 2 * a.c.kv_heads + per - 1) / per;
-    if (a.tokens >= ((int64_t)1 << 31) || by > 65535) return abi::fail(SWB_ERR_ARG, "too many tokens or heads in one call");
-    append_kernel<T, D><<<dim3((unsigned)a.tokens, (unsigned)by), APPEND_THREADS, 0, st>>>(a);
+    if (a.tokens >= ((int64_t)1 << 31)) return abi::fail(SWB_ERR_ARG, "too many tokens in one call");
+    append_kernel<T, D><<<(unsigned)a.tokens, APPEND_THREADS, 0, st>>>(a);
     return abi::cuda_check("append launch");
 }
 
@@ -472,17 +532,25 @@ extern "C" int swb_kv_evict(const swb_kv_cache* cache, const int32_t* seen, cons
     e.counts = e.moves + heads * 2 * budget;
     e.row_chunks = cache->head_dim / 8;
     cudaStream_t st = (cudaStream_t)stream;
-    if (e.c.capacity() <= 4 * SELECT_THREADS) select_kernel<4><<<(unsigned)heads, SELECT_THREADS, 0, st>>>(e);
-    else select_kernel<16><<<(unsigned)heads, SELECT_THREADS, 0, st>>>(e);
+    constexpr int smem = BINS * COPIES * 4;
+    static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+    const bool few = e.c.capacity() <= 8 * SELECT_THREADS;
+    const void* kernel = few ? (const void*)select_kernel<8> : (const void*)select_kernel<16>;
+    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (err != cudaSuccess) return abi::cuda_fail(err, "cudaFuncSetAttribute(evict)");
+    if (few) select_kernel<8><<<(unsigned)heads, SELECT_THREADS, smem, st>>>(e);
+    else select_kernel<16><<<(unsigned)heads, SELECT_THREADS, smem, st>>>(e);
     const int rc2 = abi::cuda_check("evict launch");
     if (rc2) return rc2;
-    // at most min(budget, slots beyond it) rows of a head move
+    // at most min(budget, slots beyond it) rows of a head move, and slots beyond the
+    // budget or the shortest length hold nothing
     const int64_t beyond = e.c.capacity() - budget;
-    const int64_t most = beyond < budget ? beyond : budget;
-    if (most <= 0) return SWB_OK;
-    const int64_t by = (most + MOVE_ROWS - 1) / MOVE_ROWS;
+    const int64_t most = beyond < budget ? (beyond > 0 ? beyond : 0) : budget;
+    const int64_t rows = (most + MOVE_ROWS - 1) / MOVE_ROWS, slots = (width + MOVE_SLOTS - 1) / MOVE_SLOTS;
+    const int64_t by = rows > slots ? rows : slots;
+    if (by == 0) return SWB_OK;
     if (by > 65535) return abi::fail(SWB_ERR_ARG, "budget too large");
-    const cudaError_t err = launch_after(move_kernel, dim3((unsigned)heads, (unsigned)by), dim3(MOVE_THREADS), 0, st, e);
+    err = launch_after(move_kernel, dim3((unsigned)heads, (unsigned)by), dim3(MOVE_THREADS), 0, st, e);
     if (err != cudaSuccess) return abi::cuda_fail(err, "evict move launch");
     return abi::cuda_check("evict move launch");
 }
