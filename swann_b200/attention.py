@@ -91,14 +91,13 @@ def _cache_arg(what, k, v, table, lengths):
                         pages, most, page, seqs, heads, d, kind), dev
 
 
-def _heads(what, name, t, k, dev, heads=None):
+def _heads(what, name, t, d, dtype, dev, heads=None):
     """[tokens, heads, head_dim] of the cache's type, any strides with contiguous rows; its shape and strides."""
-    shape = t.shape
-    if len(shape) != 3 or shape[2] != k.shape[3] or t.dtype is not k.dtype or t.get_device() != dev:
-        _fail(what, f"{name} must be [tokens, heads, {k.shape[3]}] {k.dtype} on cuda:{dev}")
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 3 or shape[2] != d or t.dtype is not dtype or t.get_device() != dev:
+        _fail(what, f"{name} must be [tokens, heads, {d}] {dtype} on cuda:{dev}")
     if heads is not None and shape[1] != heads:
         _fail(what, f"{name} must have {heads} heads")
-    strides = t.stride()
     if strides[2] != 1:
         _fail(what, f"the rows of {name} must be contiguous")
     return shape, strides
@@ -131,9 +130,10 @@ def rope_append(q, k, v, cos, sin, k_cache, v_cache, table, starts, lengths, *, 
     what = "rope_append"
     arg, dev = _cache_arg(what, k_cache, v_cache, table, lengths)
     hkv, seqs = arg.kv_heads, arg.seqs
-    (T, hq, d), qs = _heads(what, "q", q, k_cache, dev)
-    ksh, ks = _heads(what, "k", k, k_cache, dev, hkv)
-    vsh, vs = _heads(what, "v", v, k_cache, dev, hkv)
+    d, dtype = arg.head_dim, k_cache.dtype
+    (T, hq, _), qs = _heads(what, "q", q, d, dtype, dev)
+    ksh, ks = _heads(what, "k", k, d, dtype, dev, hkv)
+    vsh, vs = _heads(what, "v", v, d, dtype, dev, hkv)
     if ksh[0] != T or vsh[0] != T:
         _fail(what, "q, k and v must have the same tokens")
     _group(what, hq, hkv)
@@ -154,7 +154,7 @@ def rope_append(q, k, v, cos, sin, k_cache, v_cache, table, starts, lengths, *, 
     if slot_positions is not None:
         width = slot_positions.shape[-1]
         _ints(what, "slot_positions", slot_positions, (seqs, hkv, width), dev)
-    out = q.new_empty((T, hq, d)) if out is None else _given(what, "out", out, (T, hq, d), q.dtype, dev)
+    out = (torch.empty_like(q) if q.is_contiguous() else q.new_empty((T, hq, d))) if out is None else _given(what, "out", out, (T, hq, d), q.dtype, dev)
     if T:
         _call(what, N.lib().swb_rope_append, q, q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0],
               vs[1], hq, starts.data_ptr(), T, N.ptr(q_norm), N.ptr(k_norm), eps, cos.data_ptr(), sin.data_ptr(), rows[0],
@@ -175,7 +175,8 @@ def decode(q, k_cache, v_cache, table, lengths, *, scale=None, window=0, sinks=0
     d] and lse float32 [seqs, q_heads], 0 and -inf where nothing is seen."""
     what = "decode"
     arg, dev = _cache_arg(what, k_cache, v_cache, table, lengths)
-    (B, hq, d), qs = _heads(what, "q", q, k_cache, dev)
+    d, dtype = arg.head_dim, k_cache.dtype
+    (B, hq, _), qs = _heads(what, "q", q, d, dtype, dev)
     if B != arg.seqs:
         _fail(what, f"q must have one token for each of the {arg.seqs} sequences")
     _group(what, hq, arg.kv_heads)
@@ -189,14 +190,14 @@ def decode(q, k_cache, v_cache, table, lengths, *, scale=None, window=0, sinks=0
         wp = _given(what, "weights", weights, (B, arg.kv_heads, width), torch.float32, dev).data_ptr()
         if width < arg.max_pages * arg.page_size:
             _fail(what, "weights are narrower than the page table's slots")
-    out = q.new_empty((B, hq, d)) if out is None else _given(what, "out", out, (B, hq, d), q.dtype, dev)
-    lse = torch.empty((B, hq), dtype=torch.float32, device=q.device)
+    out = (torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, hq, d))) if out is None else _given(what, "out", out, (B, hq, d), q.dtype, dev)
+    lse = q.new_empty((B, hq), dtype=torch.float32)
     if B == 0:
         return out, lse
     L = N.lib()
     need = L.swb_attn_decode_workspace(arg, hq, wp is not None)
     # a size that says the call will be refused is left to the call
-    ws = torch.empty(need if need < 1 << 62 else 0, dtype=torch.uint8, device=q.device)
+    ws = q.new_empty(need if need < 1 << 62 else 0, dtype=torch.uint8)
     _call(what, L.swb_attn_decode, q, q.data_ptr(), qs[0], qs[1], hq, arg, d ** -0.5 if scale is None else scale, window,
           sinks, po, pl, out.data_ptr(), lse.data_ptr(), wp, width, bool(accumulate), ws.data_ptr(), need)
     return out, lse
@@ -211,11 +212,12 @@ def prefill(q, k_cache, v_cache, table, starts, lengths, *, scale=None, window=0
     [tokens, q_heads, d] and lse float32 [tokens, q_heads]."""
     what = "prefill"
     arg, dev = _cache_arg(what, k_cache, v_cache, table, lengths)
-    (T, hq, d), qs = _heads(what, "q", q, k_cache, dev)
+    d = arg.head_dim
+    (T, hq, _), qs = _heads(what, "q", q, d, k_cache.dtype, dev)
     _group(what, hq, arg.kv_heads)
     _ints(what, "starts", starts, (arg.seqs + 1,), dev)
-    out = q.new_empty((T, hq, d)) if out is None else _given(what, "out", out, (T, hq, d), q.dtype, dev)
-    lse = torch.empty((T, hq), dtype=torch.float32, device=q.device)
+    out = (torch.empty_like(q) if q.is_contiguous() else q.new_empty((T, hq, d))) if out is None else _given(what, "out", out, (T, hq, d), q.dtype, dev)
+    lse = q.new_empty((T, hq), dtype=torch.float32)
     if T:
         _call(what, N.lib().swb_attn_prefill, q, q.data_ptr(), qs[0], qs[1], hq, starts.data_ptr(), T, arg,
               d ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(), lse.data_ptr(), None)
@@ -249,7 +251,7 @@ def evict(k_cache, v_cache, table, lengths, weights, positions, budget, *, seen,
         return nl, nw, np_
     L = N.lib()
     need = L.swb_kv_evict_workspace(B, hkv, budget)
-    ws = torch.empty(need, dtype=torch.uint8, device=weights.device)
+    ws = weights.new_empty(need, dtype=torch.uint8)
     _call(what, L.swb_kv_evict, weights, arg, seen.data_ptr(), weights.data_ptr(), positions.data_ptr(), width, budget, sinks,
           recent, nl.data_ptr(), nw.data_ptr(), np_.data_ptr(), ws.data_ptr(), need)
     return nl, nw, np_

@@ -590,7 +590,8 @@ template <typename T, int D, int W, int NT>
 int launch_walk(const Walk& w, int64_t ctas, cudaStream_t st) {
     constexpr int ring = W * stages_of(W) * 2 * KEYS * D * 2, joined = W * 8 * NT * (D + 4) * 4;
     constexpr int smem = ring > joined ? ring : joined;
-    cudaError_t e = cudaFuncSetAttribute(walk_kernel<T, D, W, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem((const void*)walk_kernel<T, D, W, NT>, smem, done);
     if (e != cudaSuccess) return abi::cuda_fail(e, "cudaFuncSetAttribute(attention)");
     walk_kernel<T, D, W, NT><<<(unsigned)ctas, W * 32, smem, st>>>(w);
     return abi::cuda_check("attention launch");

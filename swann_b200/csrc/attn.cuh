@@ -5,6 +5,8 @@
 
 #include <cuda_bf16.h>
 
+#include <atomic>
+
 #include "../../include/swann_b200.h"
 #include "abi_util.h"
 #include "common.cuh"
@@ -162,6 +164,17 @@ inline int check_query(const void* q, int64_t ts, int64_t hs, int q_heads, const
     if (reinterpret_cast<uintptr_t>(q) % 16 || ts % 8 || hs % 8)
         return abi::fail(SWB_ERR_ARG, "query rows must start on 16-byte boundaries");
     return SWB_OK;
+}
+
+// Lets `kernel` have `bytes` of dynamic shared memory; asked of the driver once a
+// device (`done`: one bit each, a static of the caller's).
+inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+    const int dev = abi::current_device();
+    const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+    if (bit && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 // Launches a kernel that may begin while the one before it in the stream ends:

@@ -536,7 +536,8 @@ extern "C" int swb_kv_evict(const swb_kv_cache* cache, const int32_t* seen, cons
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
     const bool few = e.c.capacity() <= 8 * SELECT_THREADS;
     const void* kernel = few ? (const void*)select_kernel<8> : (const void*)select_kernel<16>;
-    cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint64_t> done[2];
+    cudaError_t err = allow_smem(kernel, smem, done[few]);
     if (err != cudaSuccess) return abi::cuda_fail(err, "cudaFuncSetAttribute(evict)");
     if (few) select_kernel<8><<<(unsigned)heads, SELECT_THREADS, smem, st>>>(e);
     else select_kernel<16><<<(unsigned)heads, SELECT_THREADS, smem, st>>>(e);

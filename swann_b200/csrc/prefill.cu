@@ -774,8 +774,8 @@ inline bool pool_map(CUtensorMap* m, const void* pool, const Cache& c, int d, bo
 
 template <typename T, int D>
 int launch(Prefill p, int64_t items, cudaStream_t st) {
-    const cudaError_t e = cudaFuncSetAttribute(prefill_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               Layout<D>::TOTAL);
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_smem((const void*)prefill_kernel<T, D>, Layout<D>::TOTAL, done);
     if (e != cudaSuccess) return abi::cuda_fail(e, "cudaFuncSetAttribute(prefill)");
     // 8 rows are a swizzle period, 32 a piece
     CUtensorMap mk = {}, mv = {};
