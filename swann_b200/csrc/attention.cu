@@ -25,7 +25,7 @@
 // and every CTA of a grid that the SMs hold at once takes an equal run of them,
 // whatever the sequences' lengths are; a pair cut by the end of a run leaves
 // parts (m, l, unnormalised rows), at most two a CTA, which a second kernel
-// joins.  Very many pairs: a one-warp CTA each.
+// joins.  Very many pairs: a warp a pair.
 
 #include "attn.cuh"
 
@@ -157,19 +157,174 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     return y;
 }
 
-// stages of a warp's ring, and CTAs that an SM holds by shared memory and registers
-constexpr int stages_of(int warps) { return warps > 1 ? 3 : 2; }
-constexpr int cta_per_sm(int d, int warps) { return warps > 1 ? (d == 128 ? 2 : 4) : (d == 128 ? 12 : 16); }
+constexpr int STAGES = 3;                              // of a warp's ring
+// CTAs of a run that an SM holds, by shared memory and registers
+constexpr int cta_per_sm(int d) { return d == 128 ? 2 : 4; }
 
-// W warps; up to 8 * NT query rows
-template <typename T, int D, int W, int NT>
-__global__ void __launch_bounds__(W * 32, cta_per_sm(D, W)) walk_kernel(const __grid_constant__ Walk P) {
-    constexpr int THREADS = W * 32;
-    constexpr bool RUNS = W > 1;                       // an equal run of units a CTA, or a pair a warp
-    constexpr int STAGES = stages_of(W);
-    constexpr int CH = D / 8;                          // 16-byte chunks of a row
+// What a warp keeps of the rows of a pair: this thread's columns of the products
+// are the heads n * 8 + (lane & 3) * 2 + e, its keys lane / 4 and lane / 4 + 8, its
+// dimensions j * 16 + lane / 4 and + 8.
+template <typename T, int D, int NT>
+struct Rows {
+    static constexpr int MT = D / 16;
+    float o[MT][NT][4], m[NT][2], l[NT][2];
+    uint32_t q[D / 16][NT][2];                         // the query rows as fragments of the second operand
+
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int j = 0; j < MT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[j][n][e] = 0.f;
+            m[n][0] = m[n][1] = NEG_INF;
+            l[n][0] = l[n][1] = 0.f;
+        }
+    }
+    // q: the first row; rows from `heads` on are zeros
+    __device__ __forceinline__ void load_q(const T* q0, int64_t stride, int heads, int lane) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int r = n * 8 + (lane >> 2);
+            const T* qr = q0 + r * stride + (lane & 3) * 2;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+                q[kk][n][0] = r < heads ? *reinterpret_cast<const uint32_t*>(qr + kk * 16) : 0u;
+                q[kk][n][1] = r < heads ? *reinterpret_cast<const uint32_t*>(qr + kk * 16 + 8) : 0u;
+            }
+        }
+    }
+    // one block of 16 keys: K at `st`, V behind it; bit k of `seen`: key k counts.
+    // logit(n, e, value) is told every logit.
+    template <typename F>
+    __device__ __forceinline__ void block(uint32_t st, unsigned seen, float scale2, int lane, F logit) {
+        float y[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[n][e] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+            uint32_t f[4];
+            ldmatrix4(f, st + swz<D>(((lane >> 3) & 1) * 8 + (lane & 7), 2 * kk + (lane >> 4)));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) Elem<T>::mma(y[n], f, q[kk][n][0], q[kk][n][1]);
+        }
+        const bool see0 = (seen >> (lane >> 2)) & 1u, see1 = (seen >> ((lane >> 2) + 8)) & 1u;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                y[n][e] = (e < 2 ? see0 : see1) ? y[n][e] * scale2 : NEG_INF;
+                logit(n, e, y[n][e]);
+            }
+        bool grows = false;
+        float a[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                a[n][e] = fmaxf(y[n][e], y[n][e + 2]);
+#pragma unroll
+                for (int s = 4; s <= 16; s <<= 1) a[n][e] = fmaxf(a[n][e], __shfl_xor_sync(FULL, a[n][e], s));
+                grows = grows || a[n][e] > m[n][e];
+            }
+        if (__any_sync(FULL, grows)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                float f[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float t = fmaxf(m[n][e], a[n][e]);
+                    f[e] = t == NEG_INF ? 1.f : exp2_fast(m[n][e] - t);
+                    m[n][e] = t;
+                    l[n][e] *= f[e];
+                }
+#pragma unroll
+                for (int j = 0; j < MT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[j][n][e] *= f[e & 1];
+            }
+        }
+        uint32_t pf[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float s0 = m[n][0] == NEG_INF ? 0.f : m[n][0], s1 = m[n][1] == NEG_INF ? 0.f : m[n][1];
+            const float w0 = exp2_fast(y[n][0] - s0), w1 = exp2_fast(y[n][1] - s1);
+            const float w2 = exp2_fast(y[n][2] - s0), w3 = exp2_fast(y[n][3] - s1);
+            l[n][0] += w0 + w2;
+            l[n][1] += w1 + w3;
+            pf[n][0] = transposed(Elem<T>::pack(w0, w1));
+            pf[n][1] = transposed(Elem<T>::pack(w2, w3));
+        }
+        const uint32_t sv = st + KEYS * D * 2;
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            uint32_t f[4];
+            ldmatrix4_t(f, sv + swz<D>((lane >> 4) * 8 + (lane & 7), 2 * j + ((lane >> 3) & 1)));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) Elem<T>::mma(o[j][n], f, pf[n][0], pf[n][1]);
+        }
+    }
+    // the sums over all keys: l of a column in every lane that has it
+    __device__ __forceinline__ void sum() {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int s = 4; s <= 16; s <<= 1) l[n][e] += __shfl_xor_sync(FULL, l[n][e], s);
+    }
+};
+
+// 16 rows of K and of V into a stage; lane < 16 has the element offset of row
+// `lane`, -1 for zeros.  Which rows are there.
+template <typename T, int D>
+__device__ __forceinline__ unsigned copy_block(uint32_t st, const T* kp, const T* vp, int64_t off, int lane) {
+    constexpr int CH = D / 8;
+#pragma unroll
+    for (int it = 0; it < KEYS * CH / 32; ++it) {
+        const int r = (it * 32 + lane) / CH, c = (it * 32 + lane) % CH;
+        const int64_t o = __shfl_sync(FULL, (long long)off, r);
+        const bool real = o >= 0;
+        const int64_t e = real ? o + c * 8 : 0;
+        cp_async16_or_zero(st + swz<D>(r, c), kp + e, real);
+        cp_async16_or_zero(st + KEYS * D * 2 + swz<D>(r, c), vp + e, real);
+    }
+    return __ballot_sync(FULL, off >= 0);
+}
+
+// four dimensions of a row that is whole but for the prior part: joined and written
+template <typename T, int D>
+__device__ __forceinline__ void write_row(const Walk& P, int64_t row, int d, float4 acc, float top, float sum) {
+    const float pm = P.prior_lse ? P.prior_lse[row] * LOG2E : NEG_INF;
+    const float most = fmaxf(top, pm);
+    const float fa = sum == 0.f ? 0.f : exp2_fast(top - most), fb = pm == NEG_INF ? 0.f : exp2_fast(pm - most);
+    const float whole = sum * fa + fb;
+    const float inv = whole == 0.f ? 0.f : 1.f / whole;
+    acc = make_float4(acc.x * fa, acc.y * fa, acc.z * fa, acc.w * fa);
+    if (pm != NEG_INF) {
+        const uint2 z = *reinterpret_cast<const uint2*>(static_cast<const T*>(P.prior_out) + row * D + d);
+        const float2 z0 = Elem<T>::wide(z.x), z1 = Elem<T>::wide(z.y);
+        acc.x += fb * z0.x;
+        acc.y += fb * z0.y;
+        acc.z += fb * z1.x;
+        acc.w += fb * z1.y;
+    }
+    *reinterpret_cast<uint2*>(static_cast<T*>(P.out) + row * D + d) =
+        make_uint2(Elem<T>::pack(acc.x * inv, acc.y * inv), Elem<T>::pack(acc.z * inv, acc.w * inv));
+    if (d == 0) {
+        const float z = whole == 0.f ? NEG_INF : most + log2f(whole);
+        P.lse[row] = z * LN2;
+        if (P.lse2) P.lse2[row] = z;
+    }
+}
+
+// An equal run of units a CTA; up to 8 * NT query rows
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(WARPS * 32, cta_per_sm(D)) walk_kernel(const __grid_constant__ Walk P) {
+    constexpr int W = WARPS, THREADS = W * 32;
     constexpr int STAGE = 2 * KEYS * D * 2;            // K and V of a block of keys
-    constexpr int MT = D / 16;                         // 16-high tiles of the dimensions
     constexpr int R = 8 * NT;
     constexpr int LD = D + 4;                          // of the joined rows: no two of a warp's stores meet in a bank
     extern __shared__ __align__(128) char smem[];
@@ -180,26 +335,13 @@ __global__ void __launch_bounds__(W * 32, cta_per_sm(D, W)) walk_kernel(const __
     const int tiles = P.c.kv_heads * P.head_tiles;
 
     // -- which pairs, and which of their keys
-    Spot at;
-    int left = 1, x = 0;                               // units still to walk; the next one
-    int all = 1;
-    if constexpr (RUNS) {
-        Units U;
-        U.count(P);
-        const Runs runs(U.total * tiles, P.runs);
-        const int i = blockIdx.x;
-        if (threadIdx.x == 0) P.cuts[i] = make_int4(0, 0, 0, 0);
-        if (i >= runs.used) return;
-        x = runs.begin(i);
-        left = runs.begin(i + 1) - x;
-        at = spot_of(P, U, x);
-        all = U.total * tiles;
-    } else {
-        at.b = (int)(blockIdx.x / tiles);
-        at.h = (int)(blockIdx.x % tiles);
-        at.unit = 0;
-        at.units = 1;
-    }
+    Units U;
+    U.count(P);
+    const Runs runs(U.total * tiles, P.runs);
+    if (threadIdx.x == 0) P.cuts[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if ((int)blockIdx.x >= runs.used) return;
+    int x = runs.begin(blockIdx.x), left = runs.begin(blockIdx.x + 1) - x;    // the next unit; units still to walk
+    Spot at = spot_of(P, U, x);
 
     for (bool first = true; left > 0; first = false) {
         const int b = at.b, g = at.h / P.head_tiles, ht = at.h % P.head_tiles;
@@ -207,7 +349,7 @@ __global__ void __launch_bounds__(W * 32, cta_per_sm(D, W)) walk_kernel(const __
         const int64_t row0 = (int64_t)b * P.q_heads + g * P.group + ht * P.tile_heads;   // first output row
         const Range rg = visible(P.c.lengths[b] - 1, P.window, P.sinks, P.c.capacity());
         const int take = min(left, at.units - at.unit);
-        const int u0 = RUNS ? min(rg.n, at.unit * UNIT) : 0, u1 = RUNS ? min(rg.n, u0 + take * UNIT) : rg.n;
+        const int u0 = min(rg.n, at.unit * UNIT), u1 = min(rg.n, u0 + take * UNIT);
         const bool entire = take == at.units;          // nothing of the pair is left to others
         const int nblk = (u1 - u0 + KEYS - 1) / KEYS;  // blocks of the stretch; warp w has w, w + W, ..
         const int mine = nblk > warp ? (nblk - warp - 1) / W + 1 : 0;
@@ -220,19 +362,9 @@ __global__ void __launch_bounds__(W * 32, cta_per_sm(D, W)) walk_kernel(const __
             return (lane < KEYS && i < mine && u < u1) ? P.c.row(b, rg.slot(u)) : -1;
         };
         auto issue = [&](int i, int64_t off) {
-            const uint32_t st = ring + (i % STAGES) * STAGE;
             if (i < mine) {
-                const unsigned seen = __ballot_sync(FULL, off >= 0);
+                const unsigned seen = copy_block<T, D>(ring + (i % STAGES) * STAGE, kp, vp, off, lane);
                 if (lane == 0) s_seen[warp][i % STAGES] = seen;
-#pragma unroll
-                for (int it = 0; it < KEYS * CH / 32; ++it) {
-                    const int r = (it * 32 + lane) / CH, c = (it * 32 + lane) % CH;
-                    const int64_t o = __shfl_sync(FULL, (long long)off, r);
-                    const bool real = o >= 0;
-                    const int64_t e = real ? o + c * 8 : 0;
-                    cp_async16_or_zero(st + swz<D>(r, c), kp + e, real);
-                    cp_async16_or_zero(st + KEYS * D * 2 + swz<D>(r, c), vp + e, real);
-                }
             }
             cp_async_commit();
         };
@@ -240,131 +372,36 @@ __global__ void __launch_bounds__(W * 32, cta_per_sm(D, W)) walk_kernel(const __
         for (int i = 0; i < STAGES - 1; ++i) issue(i, find(i));
         int64_t next = find(STAGES - 1);
 
-        // -- the query rows as fragments of the second operand: column r is head r of the tile
-        const T* q = static_cast<const T*>(P.q) + b * P.q_seq_stride +
-                     (int64_t)(g * P.group + ht * P.tile_heads) * P.q_head_stride;
-        uint32_t qf[D / 16][NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int r = n * 8 + (lane >> 2);
-            const T* qr = q + r * P.q_head_stride + (lane & 3) * 2;
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-                qf[kk][n][0] = r < heads ? *reinterpret_cast<const uint32_t*>(qr + kk * 16) : 0u;
-                qf[kk][n][1] = r < heads ? *reinterpret_cast<const uint32_t*>(qr + kk * 16 + 8) : 0u;
-            }
-        }
-
-        // this thread's columns: heads n * 8 + (lane & 3) * 2 + e
-        float o[MT][NT][4], m[NT][2], l[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int j = 0; j < MT; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[j][n][e] = 0.f;
-            m[n][0] = m[n][1] = NEG_INF;
-            l[n][0] = l[n][1] = 0.f;
-        }
+        Rows<T, D, NT> rows;
+        rows.load_q(static_cast<const T*>(P.q) + b * P.q_seq_stride +
+                        (int64_t)(g * P.group + ht * P.tile_heads) * P.q_head_stride,
+                    P.q_head_stride, heads, lane);
+        rows.clear();
         for (int i = 0; i < mine; ++i) {
             cp_async_wait<STAGES - 2>();
             __syncwarp();
             issue(i + STAGES - 1, next);      // into the stage that block i - 1 has left
             next = find(i + STAGES);
-            const uint32_t st = ring + (i % STAGES) * STAGE;
-            const unsigned seen = s_seen[warp][i % STAGES];
-
-            float y[NT][4];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[n][e] = 0.f;
-#pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-                uint32_t f[4];
-                ldmatrix4(f, st + swz<D>(((lane >> 3) & 1) * 8 + (lane & 7), 2 * kk + (lane >> 4)));
-#pragma unroll
-                for (int n = 0; n < NT; ++n) Elem<T>::mma(y[n], f, qf[kk][n][0], qf[kk][n][1]);
-            }
-            const int k0 = lane >> 2;         // this thread's keys: k0 and k0 + 8
-            const bool see0 = (seen >> k0) & 1u, see1 = (seen >> (k0 + 8)) & 1u;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[n][e] = (e < 2 ? see0 : see1) ? y[n][e] * P.scale2 : NEG_INF;
-            if (P.logits) {
-                const int u = u0 + (i * W + warp) * KEYS + k0;
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = n * 8 + (lane & 3) * 2 + (e & 1), v = u + (e < 2 ? 0 : 8);
-                        if (r < heads && v < u1) P.logits[(row0 + r) * P.c.capacity() + rg.slot(v)] = y[n][e];
-                    }
-            }
-            bool grows = false;
-            float a[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    a[n][e] = fmaxf(y[n][e], y[n][e + 2]);
-#pragma unroll
-                    for (int s = 4; s <= 16; s <<= 1) a[n][e] = fmaxf(a[n][e], __shfl_xor_sync(FULL, a[n][e], s));
-                    grows = grows || a[n][e] > m[n][e];
-                }
-            if (__any_sync(FULL, grows)) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    float f[2];
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float t = fmaxf(m[n][e], a[n][e]);
-                        f[e] = t == NEG_INF ? 1.f : exp2_fast(m[n][e] - t);
-                        m[n][e] = t;
-                        l[n][e] *= f[e];
-                    }
-#pragma unroll
-                    for (int j = 0; j < MT; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[j][n][e] *= f[e & 1];
-                }
-            }
-            uint32_t pf[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const float s0 = m[n][0] == NEG_INF ? 0.f : m[n][0], s1 = m[n][1] == NEG_INF ? 0.f : m[n][1];
-                const float w0 = exp2_fast(y[n][0] - s0), w1 = exp2_fast(y[n][1] - s1);
-                const float w2 = exp2_fast(y[n][2] - s0), w3 = exp2_fast(y[n][3] - s1);
-                l[n][0] += w0 + w2;
-                l[n][1] += w1 + w3;
-                pf[n][0] = transposed(Elem<T>::pack(w0, w1));
-                pf[n][1] = transposed(Elem<T>::pack(w2, w3));
-            }
-            const uint32_t sv = st + KEYS * D * 2;
-#pragma unroll
-            for (int j = 0; j < MT; ++j) {
-                uint32_t f[4];
-                ldmatrix4_t(f, sv + swz<D>((lane >> 4) * 8 + (lane & 7), 2 * j + ((lane >> 3) & 1)));
-#pragma unroll
-                for (int n = 0; n < NT; ++n) Elem<T>::mma(o[j][n], f, pf[n][0], pf[n][1]);
-            }
+            rows.block(ring + (i % STAGES) * STAGE, s_seen[warp][i % STAGES], P.scale2, lane, [&](int n, int e, float y) {
+                if (!P.logits) return;
+                const int r = n * 8 + (lane & 3) * 2 + (e & 1);
+                const int u = u0 + (i * W + warp) * KEYS + (lane >> 2) + (e < 2 ? 0 : 8);
+                if (r < heads && u < u1) P.logits[(row0 + r) * P.c.capacity() + rg.slot(u)] = y;
+            });
             __syncwarp();
         }
         cp_async_wait<0>();
 
         // -- join the warps
+        rows.sum();
+        if (lane < 4)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                for (int s = 4; s <= 16; s <<= 1) l[n][e] += __shfl_xor_sync(FULL, l[n][e], s);
-                if (lane < 4) {
-                    s_m[warp][n * 8 + lane * 2 + e] = m[n][e];
-                    s_l[warp][n * 8 + lane * 2 + e] = l[n][e];
+                for (int e = 0; e < 2; ++e) {
+                    s_m[warp][n * 8 + lane * 2 + e] = rows.m[n][e];
+                    s_l[warp][n * 8 + lane * 2 + e] = rows.l[n][e];
                 }
-            }
         __syncthreads();      // the ring is free too
         float* so = reinterpret_cast<float*>(smem);    // [W][R][LD]
 #pragma unroll
@@ -375,12 +412,12 @@ __global__ void __launch_bounds__(W * 32, cta_per_sm(D, W)) walk_kernel(const __
                 float top = NEG_INF;
 #pragma unroll
                 for (int w = 0; w < W; ++w) top = fmaxf(top, s_m[w][r]);
-                const float f = l[n][e] == 0.f ? 0.f : exp2_fast(m[n][e] - top);
+                const float f = rows.l[n][e] == 0.f ? 0.f : exp2_fast(rows.m[n][e] - top);
                 float* dst = so + (warp * R + r) * LD + (lane >> 2);
 #pragma unroll
-                for (int j = 0; j < MT; ++j) {
-                    dst[j * 16] = o[j][n][e] * f;
-                    dst[j * 16 + 8] = o[j][n][e + 2] * f;
+                for (int j = 0; j < D / 16; ++j) {
+                    dst[j * 16] = rows.o[j][n][e] * f;
+                    dst[j * 16 + 8] = rows.o[j][n][e + 2] * f;
                 }
             }
         __syncthreads();
@@ -399,42 +436,18 @@ __global__ void __launch_bounds__(W * 32, cta_per_sm(D, W)) walk_kernel(const __
                 acc.z += z.z;
                 acc.w += z.w;
             }
-            if (!entire) {
+            if (entire) {
+                write_row<T, D>(P, row0 + r, d, acc, top, sum);
+            } else {
                 const int64_t part = (2 * (int64_t)blockIdx.x + (first ? 0 : 1)) * ROWS + r;
                 *reinterpret_cast<float4*>(P.part_out + part * D + d) = acc;
                 if (d == 0) P.part_ml[part] = make_float2(top, sum);
-                continue;
-            }
-            // the whole pair: this is the answer, up to the prior part
-            const int64_t row = row0 + r;
-            const float pm = P.prior_lse ? P.prior_lse[row] * LOG2E : NEG_INF;
-            const float most = fmaxf(top, pm);
-            const float fa = sum == 0.f ? 0.f : exp2_fast(top - most), fb = pm == NEG_INF ? 0.f : exp2_fast(pm - most);
-            const float whole = sum * fa + fb;
-            const float inv = whole == 0.f ? 0.f : 1.f / whole;
-            acc = make_float4(acc.x * fa, acc.y * fa, acc.z * fa, acc.w * fa);
-            if (pm != NEG_INF) {
-                const uint2 z = *reinterpret_cast<const uint2*>(static_cast<const T*>(P.prior_out) + row * D + d);
-                const float2 z0 = Elem<T>::wide(z.x), z1 = Elem<T>::wide(z.y);
-                acc.x += fb * z0.x;
-                acc.y += fb * z0.y;
-                acc.z += fb * z1.x;
-                acc.w += fb * z1.y;
-            }
-            *reinterpret_cast<uint2*>(static_cast<T*>(P.out) + row * D + d) =
-                make_uint2(Elem<T>::pack(acc.x * inv, acc.y * inv), Elem<T>::pack(acc.z * inv, acc.w * inv));
-            if (d == 0) {
-                const float z = whole == 0.f ? NEG_INF : most + log2f(whole);
-                P.lse[row] = z * LN2;
-                if (P.lse2) P.lse2[row] = z;
             }
         }
-        if constexpr (RUNS) {
-            if (!entire && at.unit == 0 && threadIdx.x == 0) {
-                // the pair begins here and goes on in the runs that follow
-                const int last = Runs(all, P.runs).owner(x + at.units - 1);
-                P.cuts[blockIdx.x] = make_int4((int)row0, heads, last - (int)blockIdx.x + 1, 2 * blockIdx.x + (first ? 0 : 1));
-            }
+        if (!entire && at.unit == 0 && threadIdx.x == 0) {
+            // the pair begins here and goes on in the runs that follow
+            const int last = runs.owner(x + at.units - 1);
+            P.cuts[blockIdx.x] = make_int4((int)row0, heads, last - (int)blockIdx.x + 1, 2 * blockIdx.x + (first ? 0 : 1));
         }
         left -= take;
         x += take;
@@ -448,6 +461,197 @@ __global__ void __launch_bounds__(W * 32, cta_per_sm(D, W)) walk_kernel(const __
             __syncthreads();      // the joined rows have been read: the ring is free
         }
     }
+}
+
+// -- very many pairs ------------------------------------------------------------
+
+constexpr int PAIR_STAGES = 2;
+// one-warp CTAs that an SM holds: with short pairs what counts is how many chains of
+// dependent reads (length, table, rows) are under way, so few stages and many warps
+constexpr int pair_ctas(int d) { return d == 128 ? 12 : 16; }
+
+// A warp a pair.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(32, pair_ctas(D)) pair_kernel(const __grid_constant__ Walk P) {
+    constexpr int STAGE = 2 * KEYS * D * 2, LD = D + 4;
+    extern __shared__ __align__(128) char smem[];      // the stages; then the rows on their way out
+    const int lane = threadIdx.x;
+    const uint32_t ring = smem_u32(smem);
+    const int tiles = P.c.kv_heads * P.head_tiles;
+    const int b = (int)(blockIdx.x / tiles), h = (int)(blockIdx.x % tiles), g = h / P.head_tiles, ht = h % P.head_tiles;
+    const int heads = min(P.tile_heads, P.group - ht * P.tile_heads), head0 = g * P.group + ht * P.tile_heads;
+    const int64_t row0 = (int64_t)b * P.q_heads + head0;
+    const Range rg = visible(P.c.lengths[b] - 1, P.window, P.sinks, P.c.capacity());
+    const int blocks = (rg.n + KEYS - 1) / KEYS;
+    const T* kp = static_cast<const T*>(P.c.k) + (int64_t)g * P.c.head_stride;
+    const T* vp = static_cast<const T*>(P.c.v) + (int64_t)g * P.c.head_stride;
+    unsigned seen[PAIR_STAGES];
+    auto find = [&](int i) -> int64_t {
+        const int u = i * KEYS + lane;
+        return lane < KEYS && u < rg.n ? P.c.row(b, rg.slot(u)) : -1;
+    };
+    seen[1] = blocks > 0 ? copy_block<T, D>(ring, kp, vp, find(0), lane) : 0u;
+    cp_async_commit();
+    int64_t next = find(1);
+    Rows<T, D, NT> rows;
+    rows.load_q(static_cast<const T*>(P.q) + b * P.q_seq_stride + (int64_t)head0 * P.q_head_stride, P.q_head_stride, heads, lane);
+    rows.clear();
+    for (int i = 0; i < blocks; ++i) {
+        cp_async_wait<0>();
+        __syncwarp();
+        seen[0] = seen[1];
+        if (i + 1 < blocks) seen[1] = copy_block<T, D>(ring + ((i + 1) & 1) * STAGE, kp, vp, next, lane);
+        cp_async_commit();
+        next = find(i + 2);
+        if (seen[0] || P.logits) rows.block(ring + (i & 1) * STAGE, seen[0], P.scale2, lane, [&](int n, int e, float y) {
+            if (!P.logits) return;
+            const int r = n * 8 + (lane & 3) * 2 + (e & 1), u = i * KEYS + (lane >> 2) + (e < 2 ? 0 : 8);
+            if (r < heads && u < rg.n) P.logits[(row0 + r) * P.c.capacity() + rg.slot(u)] = y;
+        });
+        __syncwarp();
+    }
+    cp_async_wait<0>();
+    rows.sum();
+    float* out = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = n * 8 + (lane & 3) * 2 + e;
+            if (r >= heads) continue;
+            float* dst = out + r * LD + (lane >> 2);
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) {
+                dst[j * 16] = rows.o[j][n][e];
+                dst[j * 16 + 8] = rows.o[j][n][e + 2];
+            }
+            if (lane < 4) {
+                out[r * LD + D] = rows.m[n][e];
+                out[r * LD + D + 1] = rows.l[n][e];
+            }
+        }
+    __syncwarp();
+    for (int c = lane; c < heads * (D / 4); c += 32) {
+        const int r = c / (D / 4), d = c % (D / 4) * 4;
+        const float* src = out + r * LD;
+        write_row<T, D>(P, row0 + r, d, *reinterpret_cast<const float4*>(src + d), src[D], src[D + 1]);
+    }
+}
+
+// A warp a pair of one query row: what a search of each head's keys gives.  There a
+// matrix product would be seven eighths empty and most of its instructions spent on
+// bringing operands into place (35 us against 26 for 4096 queries of up to 100 rows),
+// so rows go straight into registers: D / 8 lanes have a row's 16-byte chunks, 32 / (D
+// / 8) rows at a time, and a row's sum is folded over its lanes.
+// Eight rows at a time keep its registers low (7 CTAs an SM): all warps of 4096 pairs
+// are resident and wait for their rows side by side (26 us; 16 rows and 5 CTAs 30, 4
+// rows and 9 CTAs 32).
+constexpr int ROW_WARPS = 4, ROW_KEYS = 8;
+template <typename T, int D>
+__global__ void __launch_bounds__(ROW_WARPS * 32, 7) row_kernel(const __grid_constant__ Walk P, int64_t pairs) {
+    constexpr int CH = D / 8, AT = 32 / CH, NI = ROW_KEYS / AT;     // lanes of a row; rows at a time; times
+    const int lane = threadIdx.x & 31, c = lane % CH, sub = lane / CH;
+    const int64_t pair = (int64_t)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+    if (pair >= pairs) return;                                   // whole warps; nothing below is the CTA's
+    const int b = (int)(pair / P.c.kv_heads), g = (int)(pair % P.c.kv_heads);
+    const Range rg = visible(P.c.lengths[b] - 1, P.window, P.sinks, P.c.capacity());
+    const int64_t head = (int64_t)g * P.c.head_stride + c * 8;
+    const T* kp = static_cast<const T*>(P.c.k) + head;
+    const T* vp = static_cast<const T*>(P.c.v) + head;
+    auto find = [&](int u) -> int64_t { return u < rg.n ? P.c.row(b, rg.slot(u)) : -1; };
+    int64_t next = find(lane);                                   // rows are looked up 32 at a time, one time ahead
+    float q[8];
+    {
+        const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const T*>(P.q) + b * P.q_seq_stride + g * P.q_head_stride + c * 8);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float2 f = Elem<T>::wide(w[e]);
+            q[2 * e] = f.x;
+            q[2 * e + 1] = f.y;
+        }
+    }
+    float m = NEG_INF, l = 0.f, acc[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+    for (int u1 = 0; u1 < rg.n; u1 += 32) {
+        const int64_t off = next;
+        next = find(u1 + 32 + lane);
+        const unsigned there = __ballot_sync(FULL, off >= 0);
+        for (int k0 = 0; k0 < 32 && u1 + k0 < rg.n; k0 += ROW_KEYS) {
+            // a search pads with -1 what it did not find
+            if (!P.logits && !((there >> k0) & ((1u << ROW_KEYS) - 1u))) continue;
+            const int u0 = u1 + k0;
+            uint4 k[NI], v[NI];
+            bool real[NI];
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int64_t o = __shfl_sync(FULL, (long long)off, k0 + i * AT + sub);
+                real[i] = o >= 0;
+                k[i] = v[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (real[i]) {
+                    k[i] = ld_row16(reinterpret_cast<const uint4*>(kp + o));
+                    v[i] = ld_row16(reinterpret_cast<const uint4*>(vp + o));
+                }
+            }
+            float x[NI], top = NEG_INF;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const uint32_t w[4] = {k[i].x, k[i].y, k[i].z, k[i].w};
+                float s = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 f = Elem<T>::wide(w[e]);
+                    s = fmaf(q[2 * e], f.x, s);
+                    s = fmaf(q[2 * e + 1], f.y, s);
+                }
+                x[i] = s;
+            }
+#pragma unroll
+            for (int s = CH / 2; s > 0; s >>= 1)
+#pragma unroll
+                for (int i = 0; i < NI; ++i) x[i] += __shfl_xor_sync(FULL, x[i], s);
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                x[i] = real[i] ? x[i] * P.scale2 : NEG_INF;
+                top = fmaxf(top, x[i]);
+                const int u = u0 + i * AT + sub;
+                if (P.logits && c == 0 && u < rg.n) P.logits[((int64_t)b * P.q_heads + g) * P.c.capacity() + rg.slot(u)] = x[i];
+            }
+#pragma unroll
+            for (int s = CH; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, s));
+            if (top > m) {                                           // the same in all lanes
+                const float f = exp2_fast(m - top);
+                m = top;
+                l *= f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[e] *= f;
+            }
+            const float base = m == NEG_INF ? 0.f : m;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const float p = exp2_fast(x[i] - base);
+                l += p;
+                const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 f = Elem<T>::wide(w[e]);
+                    acc[2 * e] = fmaf(p, f.x, acc[2 * e]);
+                    acc[2 * e + 1] = fmaf(p, f.y, acc[2 * e + 1]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int s = CH; s < 32; s <<= 1) {
+        l += __shfl_xor_sync(FULL, l, s);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] += __shfl_xor_sync(FULL, acc[e], s);
+    }
+    // the lanes of the first two row places write four dimensions each
+    if (sub < 2)
+        write_row<T, D>(P, (int64_t)b * P.q_heads + g, c * 8 + sub * 4,
+                        sub ? make_float4(acc[4], acc[5], acc[6], acc[7]) : make_float4(acc[0], acc[1], acc[2], acc[3]), m, l);
 }
 
 // -- the join of a pair's parts ------------------------------------------------
@@ -577,32 +781,40 @@ __global__ void __launch_bounds__(SHARE_THREADS) share_kernel(const __grid_const
 
 // -- host side --------------------------------------------------------------
 
-// Whether every pair gets a warp of its own.  With short tables (search results)
-// a run would be many short pairs one after the other, each a chain of dependent
-// reads; a warp a pair has as many chains in flight as the SMs hold warps.  With
-// long ones it needs enough pairs that the last round of unequal lengths is short.
-inline bool warp_a_pair(const Cache& c, int64_t pairs) {
+// Whether a warp takes a whole pair.  With short tables (search results) a run of a
+// CTA would be many short pairs, each joined by its warps.  With long ones it needs
+// enough pairs that the last round of unequal lengths is short.
+inline bool whole_pairs(const Cache& c, int64_t pairs) {
     const int64_t warps = 8ll * abi::num_sms();
     return c.capacity() <= 512 ? pairs >= warps / 2 : pairs >= 16 * warps;
 }
 
-template <typename T, int D, int W, int NT>
-int launch_walk(const Walk& w, int64_t ctas, cudaStream_t st) {
-    constexpr int ring = W * stages_of(W) * 2 * KEYS * D * 2, joined = W * 8 * NT * (D + 4) * 4;
+template <typename T, int D, int NT>
+int launch_walk(const Walk& w, int64_t pairs, cudaStream_t st) {
+    static std::atomic<uint64_t> done[2];
+    if (!w.runs && w.group == 1) {
+        row_kernel<T, D><<<(unsigned)((pairs + ROW_WARPS - 1) / ROW_WARPS), ROW_WARPS * 32, 0, st>>>(w, pairs);
+        return abi::cuda_check("attention launch");
+    }
+    if (!w.runs) {
+        constexpr int ring = PAIR_STAGES * 2 * KEYS * D * 2, rows = 8 * NT * (D + 4) * 4, smem = ring > rows ? ring : rows;
+        const cudaError_t e = allow_smem((const void*)pair_kernel<T, D, NT>, smem, done[0]);
+        if (e != cudaSuccess) return abi::cuda_fail(e, "cudaFuncSetAttribute(attention)");
+        pair_kernel<T, D, NT><<<(unsigned)pairs, 32, smem, st>>>(w);
+        return abi::cuda_check("attention launch");
+    }
+    constexpr int ring = WARPS * STAGES * 2 * KEYS * D * 2, joined = WARPS * 8 * NT * (D + 4) * 4;
     constexpr int smem = ring > joined ? ring : joined;
-    static std::atomic<uint64_t> done{0};
-    const cudaError_t e = allow_smem((const void*)walk_kernel<T, D, W, NT>, smem, done);
+    const cudaError_t e = allow_smem((const void*)walk_kernel<T, D, NT>, smem, done[1]);
     if (e != cudaSuccess) return abi::cuda_fail(e, "cudaFuncSetAttribute(attention)");
-    walk_kernel<T, D, W, NT><<<(unsigned)ctas, W * 32, smem, st>>>(w);
+    walk_kernel<T, D, NT><<<(unsigned)w.runs, WARPS * 32, smem, st>>>(w);
     return abi::cuda_check("attention launch");
 }
 
 template <typename T, int D>
 int launch_decode(const Walk& w, int64_t pairs, cudaStream_t st) {
-    const bool wide = w.tile_heads > 8;
-    if (!w.runs) return wide ? launch_walk<T, D, 1, 2>(w, pairs, st) : launch_walk<T, D, 1, 1>(w, pairs, st);
-    const int rc = wide ? launch_walk<T, D, WARPS, 2>(w, w.runs, st) : launch_walk<T, D, WARPS, 1>(w, w.runs, st);
-    if (rc || w.runs == 1) return rc;
+    const int rc = w.tile_heads > 8 ? launch_walk<T, D, 2>(w, pairs, st) : launch_walk<T, D, 1>(w, pairs, st);
+    if (rc || w.runs <= 1) return rc;
     const cudaError_t e = launch_after(join_kernel<T, D>, dim3((unsigned)(w.runs - 1), (unsigned)w.tile_heads),
                                        dim3(JOIN_THREADS), 0, st, w);
     if (e != cudaSuccess) return abi::cuda_fail(e, "attention join launch");
@@ -617,7 +829,7 @@ inline int tiles_of(int group) { return (group + ROWS - 1) / ROWS; }
 inline Space decode_space(const Cache& c, int d, int q_heads, bool weights) {
     Space s;
     const int64_t pairs = (int64_t)c.seqs * c.kv_heads * tiles_of(q_heads / c.kv_heads);
-    s.runs = warp_a_pair(c, pairs) ? 0 : cta_per_sm(d, WARPS) * abi::num_sms();
+    s.runs = whole_pairs(c, pairs) ? 0 : cta_per_sm(d) * abi::num_sms();
     // no more runs than there can be units
     const int64_t most = pairs * ((c.capacity() + UNIT - 1) / UNIT + 1);
     if (s.runs > most) s.runs = (int)most;

@@ -182,6 +182,39 @@ def test_decode_over_search_results():
     assert (out[0] == 0).all() and lse[0, 0] == -math.inf
 
 
+@pytest.mark.parametrize("B,hq,hkv,d,page,dtype", [
+    (700, 1, 1, 128, 1, torch.float16), (650, 1, 1, 64, 1, torch.bfloat16), (300, 3, 3, 128, 16, torch.bfloat16),
+    (700, 4, 1, 128, 1, torch.float16), (620, 7, 1, 64, 8, torch.bfloat16), (600, 12, 1, 128, 1, torch.bfloat16),
+    (600, 20, 1, 64, 1, torch.float16)])
+@pytest.mark.parametrize("window,sinks,extra", [(0, 0, "prior"), (0, 0, "weights"), (21, 3, "plain")])
+def test_decode_of_very_many_short_sequences(B, hq, hkv, d, page, dtype, window, sinks, extra):
+    """Short tables and hundreds of sequences: lengths of 0 to 90, -1 at the end of the table and inside it."""
+    lengths = [(37 * b) % 91 for b in range(B)]
+    k, v, table, L = make_cache(lengths, hkv, d, page, dtype, 51, max_pages=96 // page)
+    table[::5, 1::3] = -1
+    table[7, :] = -1
+    q = (torch.randn((B, hq, d), device=DEV) * 1.5).to(dtype)
+    prior = weights = None
+    if extra == "prior":
+        po, pl = torch.randn((B, hq, d), device=DEV).to(dtype), torch.randn((B, hq), device=DEV) * 3 + 3
+        pl[::3], po[::3] = -math.inf, math.nan
+        prior = (po, pl)
+    if extra == "weights":
+        weights = torch.full((B, hkv, 96), math.nan, device=DEV)
+    out, lse = A.decode(q, k, v, table, L, window=window, sinks=sinks, prior=prior, weights=weights)
+    G = hq // hkv
+    for b in [*range(12), 35, B // 2, B - 2, B - 1]:
+        for g in range(hkv):
+            share, e = torch.zeros(96, dtype=torch.float64, device=DEV), 0.0
+            for h in range(g * G, (g + 1) * G):
+                want = attend(q[b, h], k, v, table, b, g, lengths[b] - 1, d ** -0.5, window, sinks, lengths[b])
+                check_row(out[b, h], lse[b, h], want, U[dtype], (po[b, h], pl[b, h]) if prior else None)
+                share[torch.from_numpy(want[0]).to(DEV)] += want[4]
+                e = max(e, want[5])
+            if weights is not None:
+                assert ((weights[b, g].double() - share).abs() <= (2 * e + 2.0 ** -18) * share + 1e-30).all()
+
+
 def test_decode_lengths_beyond_the_table_are_cut():
     k, v, table, L = make_cache([64], 1, 64, 16, torch.float16, 6)
     q = torch.randn((1, 2, 64), device=DEV).half()
