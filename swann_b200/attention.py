@@ -255,3 +255,82 @@ def evict(k_cache, v_cache, table, lengths, weights, positions, budget, *, seen,
     _call(what, L.swb_kv_evict, weights, arg, seen.data_ptr(), weights.data_ptr(), positions.data_ptr(), width, budget, sinks,
           recent, nl.data_ptr(), nw.data_ptr(), np_.data_ptr(), ws.data_ptr(), need)
     return nl, nw, np_
+
+
+class KVCache:
+    """One layer's paged cache of `seqs` sequences of up to `slots` slots.
+
+        cache = KVCache(seqs, slots, kv_heads, head_dim)
+        q = cache.append(q, k, v, cos, sin, starts)      # a prompt, or starts=None: a token a sequence
+        out, lse = cache.prefill(q, starts, window=4096, sinks=4)
+        out, lse = cache.attend(q, window=4096, sinks=4)
+
+    `track` keeps what eviction goes by: every slot's position and the weight it
+    has had in `attend` so far (float32 and int32 [seqs, kv_heads, slots]).
+    The pools and the table are plain tensors (k, v, table, lengths, seen) and may be
+    handed to this module's functions; `lengths` and `seen` are on the device,
+    and nothing here waits for them: tokens past the last slot are not stored."""
+
+    def __init__(self, seqs, slots, kv_heads, head_dim, *, page_size=64, dtype=torch.float16, device="cuda",
+                 track=False):
+        if page_size < 1 or page_size & (page_size - 1):
+            _fail("KVCache", "page_size must be a power of two")
+        if head_dim not in HEAD_DIMS:
+            _fail("KVCache", f"head_dim must be one of {HEAD_DIMS}")
+        if dtype not in _DTYPES:
+            _fail("KVCache", "the cache must be float16 or bfloat16")
+        per = -(-slots // page_size)
+        self.k = torch.zeros((seqs * per, kv_heads, page_size, head_dim), dtype=dtype, device=device)
+        self.v = torch.zeros_like(self.k)
+        dev = self.k.device
+        self.table = torch.arange(seqs * per, dtype=torch.int32, device=dev).view(seqs, per)
+        self.lengths = torch.zeros(seqs, dtype=torch.int32, device=dev)
+        self.seen = torch.zeros(seqs, dtype=torch.int32, device=dev)
+        self.weights = self.positions = None
+        if track:
+            self.weights = torch.zeros((seqs, kv_heads, per * page_size), dtype=torch.float32, device=dev)
+            self.positions = torch.full(self.weights.shape, -1, dtype=torch.int32, device=dev)
+        # a token a sequence
+        self._each = torch.arange(seqs + 1, dtype=torch.int32, device=dev)
+        self._evicted = False
+
+    def append(self, q, k, v, cos, sin, starts=None, *, q_norm=None, k_norm=None, eps=1e-6, interleaved=False):
+        """New tokens' keys and values into their slots; returns their queries, normed and rotated.
+
+        starts int32 [seqs + 1]: tokens starts[b] .. starts[b + 1] - 1 are sequence b's; None: one token for each."""
+        starts = self._each if starts is None else starts
+        _ints("append", "starts", starts, (self.table.shape[0] + 1,), self.k.get_device())
+        counts = starts.diff()
+        lengths, seen = self.lengths + counts, self.seen + counts
+        positions = None
+        if self._evicted:            # slots are no longer positions
+            n = q.shape[0]
+            at = torch.arange(n, dtype=torch.int32, device=q.device)
+            of = torch.repeat_interleave(seen - starts[1:], counts, output_size=n)
+            positions = (at + of).to(torch.int32)
+        out = rope_append(q, k, v, cos, sin, self.k, self.v, self.table, starts, lengths, q_norm=q_norm, k_norm=k_norm,
+                          eps=eps, positions=positions, interleaved=interleaved, slot_positions=self.positions)
+        self.lengths, self.seen = lengths, seen
+        return out
+
+    def prefill(self, q, starts, *, scale=None, window=0, sinks=0):
+        """Attention of the tokens just appended, causal."""
+        if self._evicted:
+            _fail("prefill", "after an eviction the slots' order is not the positions': append and attend token by token")
+        return prefill(q, self.k, self.v, self.table, starts, self.lengths, scale=scale, window=window, sinks=sinks)
+
+    def attend(self, q, *, scale=None, window=0, sinks=0, prior=None):
+        """Attention of the token just appended to each sequence; with `track` its weights are added to the slots'."""
+        if self._evicted and window:
+            _fail("attend", "after an eviction the slots' order is not the positions': no window")
+        return decode(q, self.k, self.v, self.table, self.lengths, scale=scale, window=window, sinks=sinks, prior=prior,
+                      weights=self.weights, accumulate=True)
+
+    def evict(self, budget, *, sinks=0, recent=0):
+        """Every sequence cut to `budget` slots: its first `sinks` and newest `recent` positions, then by weight."""
+        if self.weights is None:
+            _fail("evict", "the cache was made without track=True")
+        self.lengths, self.weights, self.positions = evict(
+            self.k, self.v, self.table, self.lengths, self.weights, self.positions, budget, seen=self.seen, sinks=sinks,
+            recent=recent)
+        self._evicted = True
