@@ -307,6 +307,24 @@ def test_prefill(new, held, hq, hkv, d, page, dtype, window, sinks, layout):
     assert torch.isfinite(out).all()
 
 
+def test_prefill_of_many_sequences():
+    """More sequences than a warp's lanes, more tiles than the GPU has SMs, some sequences without a new token."""
+    new = [(37 * b) % 90 for b in range(70)]
+    held = [(53 * b) % 200 for b in range(70)]
+    lengths = [a + c for a, c in zip(new, held)]
+    k, v, table, L = make_cache(lengths, 4, 64, 16, torch.float16, 61)
+    starts = np.concatenate([[0], np.cumsum(new)])
+    q = torch.randn((sum(new), 4, 64), device=DEV).half()
+    for window, sinks in ((0, 0), (64, 2)):
+        out, lse = A.prefill(q, k, v, table, torch.tensor(starts, dtype=torch.int32, device=DEV), L, window=window, sinks=sinks)
+        for b in (0, 1, 2, 31, 32, 33, 63, 64, 69):
+            for t in sorted({0, new[b] // 2, new[b] - 1} & set(range(new[b]))):
+                for h in range(4):
+                    want = attend(q[starts[b] + t, h], k, v, table, b, h, held[b] + t, 0.125, window, sinks, lengths[b])
+                    check_row(out[starts[b] + t, h], lse[starts[b] + t, h], want, U[torch.float16])
+        assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+
+
 def test_prefill_pages_that_hold_nothing():
     """Whole pages missing, among them all that the first tokens see."""
     k, v, table, L = make_cache([200], 2, 64, 16, torch.float16, 13)
