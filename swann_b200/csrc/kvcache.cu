@@ -214,7 +214,8 @@ struct Evict {
 constexpr int SELECT_THREADS = 1024;
 constexpr int SELECT_WARPS = SELECT_THREADS / 32;
 constexpr int BINS = 2048;
-constexpr int COPIES = 8;        // of a bin: weights share exponents, so neighbouring lanes would meet in one
+constexpr int COPIES = 8;        // of the bins: weights share exponents, so neighbouring lanes would meet in one
+constexpr int COPY = BINS + 4;   // counts from a copy to the next: the same bin of each lies in banks of its own
 
 // a slot's key: larger stays.  First and newest positions above every weight,
 // then the weights as numbers, NaN below all of them.
@@ -248,7 +249,7 @@ static_assert(SELECT_WARPS == 32, "one lane a warp");
 // read again in each pass
 template <int KEEP>
 __global__ void __launch_bounds__(SELECT_THREADS) select_kernel(const __grid_constant__ Evict P) {
-    extern __shared__ int4 s_bins[];                       // [BINS][COPIES] counts
+    extern __shared__ int4 s_bins[];                       // [COPIES][COPY] counts
     int* s_hist = reinterpret_cast<int*>(s_bins);
     __shared__ int s_warp[SELECT_WARPS], s_pick[2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -306,20 +307,19 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_kernel(const __grid_con
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const uint32_t digit = pass == 2 ? 1023u : 2047u;
-#pragma unroll
-        for (int i = 0; i < BINS * COPIES / 4 / SELECT_THREADS; ++i)
-            s_bins[threadIdx.x + i * SELECT_THREADS] = make_int4(0, 0, 0, 0);
+        for (int i = threadIdx.x; i < COPY * COPIES / 4; i += SELECT_THREADS) s_bins[i] = make_int4(0, 0, 0, 0);
         __syncthreads();
         each([&](int, uint32_t key, bool there) {
-            if (there && (key & mask) == prefix) atomicAdd(&s_hist[((key >> shift) & digit) * COPIES + (lane & (COPIES - 1))], 1);
+            if (there && (key & mask) == prefix) atomicAdd(&s_hist[(lane & (COPIES - 1)) * COPY + ((key >> shift) & digit)], 1);
         });
         __syncthreads();
         // bins from the largest down, two a thread: the one that holds the need-th
-        int count[2];
+        int count[2] = {0, 0};
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const int4 x = s_bins[(BINS - 1 - 2 * threadIdx.x - k) * 2], y = s_bins[(BINS - 1 - 2 * threadIdx.x - k) * 2 + 1];
-            count[k] = (x.x + x.y) + (x.z + x.w) + (y.x + y.y) + (y.z + y.w);
+        for (int k = 0; k < COPIES; ++k) {
+            const int2 x = *reinterpret_cast<const int2*>(s_hist + k * COPY + BINS - 2 - 2 * threadIdx.x);
+            count[0] += x.y;
+            count[1] += x.x;
         }
         int sum = count[0] + count[1];
 #pragma unroll
@@ -371,18 +371,20 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_kernel(const __grid_con
     each([&](int j, uint32_t key, bool there) {
         const bool keep = keeps(j, key, there);
         const unsigned f = __ballot_sync(FULL, there && j < m && !keep), l = __ballot_sync(FULL, j >= m && keep);
-        if (there && j < m) {
-            if (keep) {
-                nw[j] = w[j];
-                np[j] = pos[j];
-            } else {
-                to[free + __popc(f & lanemask_lt())] = j;
-            }
-        }
+        if (there && j < m && !keep) to[free + __popc(f & lanemask_lt())] = j;
         if (j >= m && keep) from[late + __popc(l & lanemask_lt())] = j;
         free += __popc(f);
         late += __popc(l);
     });
+    // what stays in place, by all threads side by side
+    for (int j = threadIdx.x; j < m; j += SELECT_THREADS) {
+        const float wj = w[j];
+        const int pj = pos[j];
+        if (keeps(j, keep_key(wj, pj, P.sinks, fresh), true)) {
+            nw[j] = wj;
+            np[j] = pj;
+        }
+    }
     if (threadIdx.x == 0) P.counts[head] = moved;
 }
 
@@ -534,7 +536,7 @@ extern "C" int swb_kv_evict(const swb_kv_cache* cache, const int32_t* seen, cons
     e.counts = e.moves + heads * 2 * budget;
     e.row_chunks = cache->head_dim / 8;
     cudaStream_t st = (cudaStream_t)stream;
-    constexpr int smem = BINS * COPIES * 4;
+    constexpr int smem = COPY * COPIES * 4;
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
     const bool few = e.c.capacity() <= 8 * SELECT_THREADS;
     const void* kernel = few ? (const void*)select_kernel<8> : (const void*)select_kernel<16>;
