@@ -613,11 +613,11 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         const int ua = P.window > 0 ? pos - P.window + 1 - J.base : 0;
         float m = NEG_INF;
         float2 l[2] = {{0.f, 0.f}, {0.f, 0.f}};
-        bool ok = true;
+        bool ok = !*s_abort;
         for (int j = S.a; j < S.z; ++j) {
             const int i = j - S.a, all = done + i, u0 = j * STEP, buf = all & 1;
             const uint32_t st = tmem + quarter + t * TILE + buf * STEP;
-            ok = ok && !*s_abort && await(&sbar[2 * t + buf], (all >> 1) & 1);
+            ok = ok && await(&sbar[2 * t + buf], (all >> 1) & 1);
             if (!__all_sync(FULL, ok)) {
                 ok = false;
                 break;
@@ -711,7 +711,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         // through shared memory, so that a store writes whole 128-byte lines: 64 dimensions of
         // 32 rows at a time, chunks placed so that neither side meets in a bank
         char* box = sm + Ly::OUT + warp * (32 * 128);
-#pragma unroll
+#pragma unroll 1
         for (int h = 0; h < D / 64; ++h) {
             uint32_t z[2][32];
             if (steps > 0) {
