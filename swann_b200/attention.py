@@ -100,6 +100,8 @@ def _heads(what, name, t, d, dtype, dev, heads=None):
         _fail(what, f"{name} must have {heads} heads")
     if strides[2] != 1:
         _fail(what, f"the rows of {name} must be contiguous")
+    if t.requires_grad and torch.is_grad_enabled():
+        _fail(what, f"{name} requires a gradient, and there is no backward pass: call under torch.no_grad()")
     return shape, strides
 
 
@@ -107,6 +109,13 @@ def _given(what, name, t, shape, dtype, dev):
     if t.shape != shape or t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
         _fail(what, f"{name} must be contiguous {dtype} {list(shape)} on cuda:{dev}")
     return t
+
+
+def _count(what, name, n):
+    """A count as the native calls take it."""
+    if not 0 <= n < 1 << 31:
+        _fail(what, f"{name} must not be negative or beyond 2^31")
+    return n
 
 
 def _group(what, q_heads, kv_heads):
@@ -120,8 +129,9 @@ def rope_append(q, k, v, cos, sin, k_cache, v_cache, table, starts, lengths, *, 
 
     q [tokens, q_heads, d], k and v [tokens, kv_heads, d]: views into one
     projection are fine.  Tokens starts[b] .. starts[b + 1] - 1 (starts int32
-    [seqs + 1]) are sequence b's, and take the last of its lengths[b] slots:
-    lengths count them already.  cos, sin float32 [positions, r / 2] rotate the
+    [seqs + 1], from 0 to the number of tokens) are sequence b's, and take the last
+    of its lengths[b] slots: lengths count them already; a token whose slot the
+    table has no page for is not stored.  cos, sin float32 [positions, r / 2] rotate the
     first r dimensions, pairs (i, i + r / 2) or, interleaved, (2i, 2i + 1), by
     the token's position: `positions` int32 [tokens], or its slot.  A position
     outside the tables gives NaN.  q_norm, k_norm [d]: weights of the norms,
@@ -198,8 +208,8 @@ def decode(q, k_cache, v_cache, table, lengths, *, scale=None, window=0, sinks=0
     need = L.swb_attn_decode_workspace(arg, hq, wp is not None)
     # a size that says the call will be refused is left to the call
     ws = q.new_empty(need if need < 1 << 62 else 0, dtype=torch.uint8)
-    _call(what, L.swb_attn_decode, q, q.data_ptr(), qs[0], qs[1], hq, arg, d ** -0.5 if scale is None else scale, window,
-          sinks, po, pl, out.data_ptr(), lse.data_ptr(), wp, width, bool(accumulate), ws.data_ptr(), need)
+    _call(what, L.swb_attn_decode, q, q.data_ptr(), qs[0], qs[1], hq, arg, d ** -0.5 if scale is None else scale,
+          _count(what, "window", window), _count(what, "sinks", sinks), po, pl, out.data_ptr(), lse.data_ptr(), wp, width, bool(accumulate), ws.data_ptr(), need)
     return out, lse
 
 
@@ -220,7 +230,8 @@ def prefill(q, k_cache, v_cache, table, starts, lengths, *, scale=None, window=0
     lse = q.new_empty((T, hq), dtype=torch.float32)
     if T:
         _call(what, N.lib().swb_attn_prefill, q, q.data_ptr(), qs[0], qs[1], hq, starts.data_ptr(), T, arg,
-              d ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(), lse.data_ptr(), None)
+              d ** -0.5 if scale is None else scale, _count(what, "window", window), _count(what, "sinks", sinks),
+              out.data_ptr(), lse.data_ptr(), None)
     return out, lse
 
 
@@ -244,7 +255,7 @@ def evict(k_cache, v_cache, table, lengths, weights, positions, budget, *, seen,
     _ints(what, "seen", seen, (B,), dev)
     if width < arg.max_pages * arg.page_size:
         _fail(what, "weights are narrower than the page table's slots")
-    if budget < 1 or sinks < 0 or recent < 0 or sinks + recent > budget:
+    if not 1 <= budget < 1 << 31 or sinks < 0 or recent < 0 or sinks + recent > budget:
         _fail(what, "the budget must be at least 1, and hold sinks and recent")
     nl, nw, np_ = torch.empty_like(lengths), torch.empty_like(weights), torch.empty_like(positions)
     if B == 0:

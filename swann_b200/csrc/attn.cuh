@@ -141,8 +141,9 @@ inline int check_cache(const swb_kv_cache* c, Cache* out) {
     if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16 || c->page_stride % 8 ||
         c->head_stride % 8 || c->row_stride % 8)
         return abi::fail(SWB_ERR_ARG, "cache: rows must start on 16-byte boundaries");
-    out->k = c->k;
-    out->v = c->v;
+    // without pages nothing is read, but copies of nothing want an address all the same
+    out->k = c->pages ? c->k : c->lengths;
+    out->v = c->pages ? c->v : c->lengths;
     out->page_stride = c->page_stride;
     out->head_stride = c->head_stride;
     out->row_stride = c->row_stride;

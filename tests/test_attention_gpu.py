@@ -546,6 +546,12 @@ def test_refusals():
         A.decode(torch.randn((2, 64, 4), device=DEV).half().transpose(1, 2), k, v, table, L)
     with no(ValueError, match="negative"):
         A.decode(q, k, v, table, L, window=-1)
+    with no(ValueError, match="negative"):
+        A.prefill(q, k, v, table, starts, L, window=1 << 31)
+    with no(ValueError, match="no backward pass"):
+        A.decode(q.clone().requires_grad_(), k, v, table, L)
+    with torch.no_grad():
+        A.decode(q.clone().requires_grad_(), k, v, table, L)
     with no(ValueError, match="narrower"):
         A.decode(q, k, v, table, L, weights=w[..., :40].contiguous())
     with no(ValueError, match="prior"):
@@ -566,6 +572,15 @@ def test_refusals():
         A.evict(k, v, table, L, w, pos[..., :40], 8, seen=L)
     with no(ValueError, match="on the GPU"):
         A.decode(q.cpu(), k.cpu(), v.cpu(), table.cpu(), L.cpu())
+
+
+def test_a_pool_without_pages_holds_nothing():
+    k = torch.empty((0, 2, 16, 64), dtype=torch.float16, device=DEV)
+    table, L = torch.zeros((1, 3), dtype=torch.int32, device=DEV), torch.full((1,), 40, dtype=torch.int32, device=DEV)
+    q = torch.randn((40, 4, 64), device=DEV).half()
+    for out, lse in (A.decode(q[:1], k, k, table, L),
+                     A.prefill(q, k, k, table, torch.tensor([0, 40], dtype=torch.int32, device=DEV), L)):
+        assert (out == 0).all() and (lse == -math.inf).all()
 
 
 def test_empty_batches():
