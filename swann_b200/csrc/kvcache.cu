@@ -17,8 +17,8 @@
 // head; each of its warps has a contiguous piece of the slots, so ranks need
 // ballots and one sum over warps.  The moved rows' bytes bound it when many move;
 // one row moves in a step of one token, and then it is the chain of passes.  8
-// sequences of up to 16384 slots cut to 2048, 8 heads: 40 us (24 to select, the rows
-// 13); 8 heads of 4097 slots cut to 4096: 16 us.
+// sequences of up to 16384 slots cut to 2048, 8 heads: 37 us (23 to select, the rows
+// 13); 8 heads of 4097 slots cut to 4096: 14 us.
 
 #include "attn.cuh"
 
