@@ -662,15 +662,12 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, 7) row_kernel(const __grid_con
 
 constexpr int JOIN_THREADS = 256;
 
-// CTA (i, r): row r of the pair that run i begins and others go on with, if any
+// by a CTA: row r of the pair that run i begins and others go on with, if any
 template <typename T, int D>
-__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ Walk P) {
+__device__ __forceinline__ void join_row(const Walk& P, int i, int r) {
     constexpr int W = JOIN_THREADS / 32, E = D / 32;
     __shared__ float s_o[W][D], s_l[W];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = blockIdx.x, r = blockIdx.y;
-    // every CTA waits, also those without work: a kernel after this one may then
-    // rely on the one before it
-    dependency_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int4 cut = P.cuts[i];
     if (r >= cut.y) return;
     const int64_t row = (int64_t)cut.x + r;
@@ -733,53 +730,123 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constan
     }
 }
 
+template <typename T, int D>
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const __grid_constant__ Walk P) {
+    // every CTA waits, also those without work: what comes after this kernel may then
+    // rely on the one before it
+    dependency_wait();
+    join_row<T, D>(P, blockIdx.x, blockIdx.y);
+}
+
 // -- the slots' weights ----------------------------------------------------------
 
 struct Shares {
-    Cache c;
-    int q_heads, group, window, sinks;
-    const float* logits;
-    const float* lse2;
     float* weights;           // [seqs][kv_heads][width]
     int64_t width;
     int accumulate;
-    int chunks;               // blocks of SHARE_SLOTS slots of a row of weights
+    int chunks;               // CTAs of a row of weights
+    int64_t ctas;             // of all rows
 };
 
-constexpr int SHARE_THREADS = 256;
-constexpr int SHARE_SLOTS = 1024;
+// Slots of a CTA.  Its heads' sums cost it as much as some thousand slots do, and long
+// stretches leave SMs idle; by thread, at 131071 slots of 4 key heads, the whole call
+// takes 77.0 us with one, 66.4 with 2, 62.1 with 4, 61.6 with 8 and 64.0 with 16.
+constexpr int SHARE_SLOTS = 8 * JOIN_THREADS;
+constexpr int SHARE_HEADS = 64;                 // whose sums a CTA finds at a time
 
-// a slot's share of the softmax, summed over the query heads of its key head
-__global__ void __launch_bounds__(SHARE_THREADS) share_kernel(const __grid_constant__ Shares P) {
-    constexpr int PER = SHARE_SLOTS / SHARE_THREADS;
-    int64_t item = blockIdx.x;
-    const int chunk = (int)(item % P.chunks);
-    item /= P.chunks;
-    const int g = (int)(item % P.c.kv_heads), b = (int)(item / P.c.kv_heads);
+// The first CTAs write the slots' weights, the rest join the cut pairs' rows, side by
+// side: a slot's share needs its heads' sums, which a cut pair's parts give as well
+// as the joined row does.  One kernel after the other took 63.9 us where this takes
+// 61.6 (fp16, 32 heads on 4, 131071 slots); both wait for memory rather than fill it.
+template <typename T, int D>
+__global__ void __launch_bounds__(JOIN_THREADS) finish_kernel(const __grid_constant__ Walk P,
+                                                              const __grid_constant__ Shares S) {
+    if ((int64_t)blockIdx.x >= S.ctas) {
+        const int x = (int)(blockIdx.x - S.ctas);
+        dependency_wait();
+        join_row<T, D>(P, x / P.tile_heads, x % P.tile_heads);
+        return;
+    }
+    __shared__ float s_off[SHARE_HEADS];
+    constexpr int PER = SHARE_SLOTS / JOIN_THREADS, W = JOIN_THREADS / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int chunk = (int)(blockIdx.x % S.chunks), bg = (int)(blockIdx.x / S.chunks);
+    const int b = bg / P.c.kv_heads, g = bg - b * P.c.kv_heads;
     const int far = P.window > 0 ? max(0, P.c.lengths[b] - P.window) : 0;
     const int L = P.c.length(b);
-    const int64_t s0 = (int64_t)chunk * SHARE_SLOTS + threadIdx.x;
-    float acc[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+    // where the pairs of this key head lie among the runs: lengths are not what the
+    // kernel before this one writes, so all this is found beside it
+    const int tiles = P.c.kv_heads * P.head_tiles, units = units_of(P, b);
+    int base = 0, all = 1;
+    if (P.runs > 1) {
+        Units U;
+        U.count(P);
+        all = U.total * tiles;
+        const int src = b / U.per;
+        int before = U.before;
+        if (lane == src)
+            for (int k = src * U.per; k < b; ++k) before += units_of(P, k);
+        base = __shfl_sync(FULL, before, src) * tiles;
+    }
+    const Runs runs(all, max(1, P.runs));
     dependency_wait();
-    const int64_t row0 = (int64_t)b * P.q_heads + (int64_t)g * P.group;
-#pragma unroll 4
-    for (int h = 0; h < P.group; ++h) {
-        const float lse2 = P.lse2[row0 + h];
-        const float off = lse2 == NEG_INF ? 0.f : lse2;             // nothing seen: every logit is -inf
-        const float* x = P.logits + (row0 + h) * P.c.capacity();
+
+    const int64_t s0 = (int64_t)chunk * SHARE_SLOTS + threadIdx.x, row0 = (int64_t)b * P.q_heads + (int64_t)g * P.group;
+    float acc[PER];
+    bool seen[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int64_t j = s0 + i * SHARE_THREADS;
-            if (j < L && (j >= far || j < P.sinks)) acc[i] += exp2_fast(x[j] - off);
+    for (int k = 0; k < PER; ++k) {
+        const int64_t j = s0 + k * JOIN_THREADS;
+        acc[k] = 0.f;
+        seen[k] = j < L && (j >= far || j < P.sinks);
+    }
+    for (int h0 = 0; h0 < P.group; h0 += SHARE_HEADS) {
+        const int h1 = min(P.group, h0 + SHARE_HEADS);
+        __syncthreads();
+        for (int h = h0 + warp; h < h1; h += W) {
+            const int ht = h / P.tile_heads, r = h - ht * P.tile_heads;
+            const int first = base + (g * P.head_tiles + ht) * units;
+            const int i = P.runs > 1 ? runs.owner(first) : 0;
+            const int n = P.runs > 1 ? runs.owner(first + units - 1) - i + 1 : 1;
+            float lse2;
+            if (n == 1) {
+                lse2 = P.lse2[row0 + h];          // the walk had the whole pair
+            } else {
+                const int part0 = 2 * i + (runs.begin(i) == first ? 0 : 1);
+                const float prior = P.prior_lse ? P.prior_lse[row0 + h] * LOG2E : NEG_INF;
+                auto part = [&](int s) { return P.part_ml[(int64_t)(s ? 2 * (i + s) : part0) * ROWS + r]; };
+                float top = prior, l = 0.f;
+                for (int s = lane; s < n; s += 32) top = fmaxf(top, part(s).x);
+#pragma unroll
+                for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, s));
+                for (int s = lane; s < n; s += 32) {
+                    const float2 y = part(s);
+                    if (y.y != 0.f) l += y.y * exp2_fast(y.x - top);
+                }
+                if (lane == 0 && prior != NEG_INF) l += exp2_fast(prior - top);
+#pragma unroll
+                for (int s = 16; s > 0; s >>= 1) l += __shfl_xor_sync(FULL, l, s);
+                lse2 = l == 0.f ? NEG_INF : top + log2f(l);
+            }
+            if (lane == 0) s_off[h - h0] = lse2 == NEG_INF ? 0.f : lse2;   // nothing seen: every logit is -inf
+        }
+        __syncthreads();
+#pragma unroll 2
+        for (int h = h0; h < h1; ++h) {
+            const float off = s_off[h - h0];
+            const float* x = P.logits + (row0 + h) * P.c.capacity();
+            float y[PER];
+#pragma unroll
+            for (int k = 0; k < PER; ++k) y[k] = seen[k] ? x[s0 + k * JOIN_THREADS] : NEG_INF;
+#pragma unroll
+            for (int k = 0; k < PER; ++k) acc[k] += exp2_fast(y[k] - off);
         }
     }
-    float* w = P.weights + ((int64_t)b * P.c.kv_heads + g) * P.width;
+    float* w = S.weights + (int64_t)bg * S.width;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int64_t j = s0 + i * SHARE_THREADS;
-        if (j < P.width) w[j] = P.accumulate ? w[j] + acc[i] : acc[i];
+    for (int k = 0; k < PER; ++k) {
+        const int64_t j = s0 + k * JOIN_THREADS;
+        if (j < S.width) w[j] = S.accumulate ? w[j] + acc[k] : acc[k];
     }
 }
 
@@ -816,11 +883,16 @@ int launch_walk(const Walk& w, int64_t pairs, cudaStream_t st) {
 }
 
 template <typename T, int D>
-int launch_decode(const Walk& w, int64_t pairs, cudaStream_t st) {
+int launch_decode(const Walk& w, int64_t pairs, const Shares& shares, cudaStream_t st) {
     const int rc = w.tile_heads > 8 ? launch_walk<T, D, 2>(w, pairs, st) : launch_walk<T, D, 1>(w, pairs, st);
-    if (rc || w.runs <= 1) return rc;
-    const cudaError_t e = launch_after(join_kernel<T, D>, dim3((unsigned)(w.runs - 1), (unsigned)w.tile_heads),
-                                       dim3(JOIN_THREADS), 0, st, w);
+    if (rc) return rc;
+    const int cuts = w.runs > 1 ? w.runs - 1 : 0;
+    cudaError_t e = cudaSuccess;
+    if (shares.weights)
+        e = launch_after(finish_kernel<T, D>, dim3((unsigned)(shares.ctas + (int64_t)cuts * w.tile_heads)), dim3(JOIN_THREADS), 0,
+                         st, w, shares);
+    else if (cuts)
+        e = launch_after(join_kernel<T, D>, dim3((unsigned)cuts, (unsigned)w.tile_heads), dim3(JOIN_THREADS), 0, st, w);
     if (e != cudaSuccess) return abi::cuda_fail(e, "attention join launch");
     return abi::cuda_check("attention join launch");
 }
@@ -905,26 +977,16 @@ extern "C" int swb_attn_decode(const void* q, int64_t q_seq_stride, int64_t q_he
     const int64_t chunks = (weights_width + SHARE_SLOTS - 1) / SHARE_SLOTS;
     const int64_t shares = weights ? chunks * c.seqs * c.kv_heads : 0;
     // units, output rows and cuts are counted in 32 bits
-    if (pairs * ((c.capacity() + UNIT - 1) / UNIT + 1) >= ((int64_t)1 << 31) || rows >= ((int64_t)1 << 31) || shares >= ((int64_t)1 << 31))
+    if (pairs * ((c.capacity() + UNIT - 1) / UNIT + 1) >= ((int64_t)1 << 31) || rows >= ((int64_t)1 << 31) || shares >= ((int64_t)1 << 30))
         return abi::fail(SWB_ERR_ARG, "too many sequences in one call");
+    Shares sh = {};
+    sh.weights = weights;
+    sh.width = weights_width;
+    sh.accumulate = accumulate;
+    sh.chunks = (int)chunks;
+    sh.ctas = shares;
     if (cache->dtype == SWB_F16)
-        rc = d == 64 ? launch_decode<__half, 64>(w, pairs, st) : launch_decode<__half, 128>(w, pairs, st);
-    else
-        rc = d == 64 ? launch_decode<__nv_bfloat16, 64>(w, pairs, st) : launch_decode<__nv_bfloat16, 128>(w, pairs, st);
-    if (rc || !weights) return rc;
-    Shares h = {};
-    h.c = c;
-    h.q_heads = q_heads;
-    h.group = w.group;
-    h.window = window;
-    h.sinks = sinks;
-    h.logits = w.logits;
-    h.lse2 = w.lse2;
-    h.weights = weights;
-    h.width = weights_width;
-    h.accumulate = accumulate;
-    h.chunks = (int)chunks;
-    const cudaError_t e = launch_after(share_kernel, dim3((unsigned)shares), dim3(SHARE_THREADS), 0, st, h);
-    if (e != cudaSuccess) return abi::cuda_fail(e, "attention weights launch");
-    return abi::cuda_check("attention weights launch");
+        return d == 64 ? launch_decode<__half, 64>(w, pairs, sh, st) : launch_decode<__half, 128>(w, pairs, sh, st);
+    return d == 64 ? launch_decode<__nv_bfloat16, 64>(w, pairs, sh, st)
+                   : launch_decode<__nv_bfloat16, 128>(w, pairs, sh, st);
 }

@@ -593,3 +593,28 @@ def test_empty_batches():
     assert out.shape == (0, 4, 64)
     cos = torch.ones((4, 32), device=DEV)
     assert A.rope_append(none, none[:, :2], none[:, :2], cos, cos, k, v, table, starts, L).shape == (0, 4, 64)
+
+
+def test_decode_shares_of_many_heads_to_a_key_head():
+    """70 heads share a key head, more than one CTA's table of sums holds, in pairs cut among runs."""
+    test_decode([2000, 0, 65], 140, 2, 64, 16, torch.float16, 0, 0, "head", "weights")
+
+
+@pytest.mark.parametrize("lengths", [[5000], [1, 3000, 64, 0], [40] * 9])
+def test_decode_shares_beside_a_prior_part(lengths):
+    """One head to a key head: a prior part scales its slots' shares by exp(lse alone - lse of both).
+
+    The two lse are fp32 of magnitude below 16 and each within 2^-19 (1 + |lse|), so the
+    factor is within 2 * 17 * 2^-19 < 2^-13."""
+    k, v, table, L = make_cache(lengths, 4, 64, 16, torch.float16, 8)
+    g = torch.Generator(device=DEV).manual_seed(9)
+    B = len(lengths)
+    q = torch.randn((B, 4, 64), generator=g, device=DEV).half()
+    prior = (torch.randn((B, 4, 64), generator=g, device=DEV).half(), torch.randn((B, 4), generator=g, device=DEV) * 3 + 6)
+    prior[1][:, 1] = -math.inf
+    alone, both = (torch.full((B, 4, table.shape[1] * 16), math.nan, device=DEV) for _ in range(2))
+    _, l0 = A.decode(q, k, v, table, L, weights=alone)
+    _, l1 = A.decode(q, k, v, table, L, weights=both, prior=prior)
+    assert float(l1[l1 > -math.inf].abs().max()) < 16
+    f = torch.where(l0 == -math.inf, 0.0, (l0.double() - l1.double()).exp())
+    assert torch.allclose(both.double(), alone.double() * f.unsqueeze(-1), rtol=2.0 ** -13, atol=1e-30)
