@@ -368,7 +368,8 @@ SWB_API int swb_rope_append(const void* q, int64_t q_token_stride, int64_t q_hea
  *            softmax, summed over the query heads of its key head; written (0
  *            where a slot is not seen), or added to when `accumulate`; NULL =
  *            not wanted
- *   workspace: at least swb_attn_decode_workspace(...) bytes */
+ *   workspace: at least swb_attn_decode_workspace(...) bytes
+ * q's rows and workspace on 16-byte boundaries, out and prior_out on 8-byte ones. */
 SWB_API int swb_attn_decode(const void* q, int64_t q_seq_stride, int64_t q_head_stride, int q_heads,
                     const swb_kv_cache* cache, float scale, int window, int sinks, const void* prior_out,
                     const float* prior_lse, void* out, float* lse, float* weights, int64_t weights_width,

@@ -950,6 +950,11 @@ extern "C" int swb_attn_decode(const void* q, int64_t q_seq_stride, int64_t q_he
     const int d = cache->head_dim;
     const Space sp = decode_space(c, d, q_heads, weights != nullptr);
     if (sp.total && (!workspace || ws_bytes < sp.total)) return abi::fail(SWB_ERR_ARG, "workspace too small");
+    // rows go out and prior rows come in four elements at a time; what the workspace holds, 16 bytes
+    if (reinterpret_cast<uintptr_t>(out) % 8 || reinterpret_cast<uintptr_t>(prior_out) % 8)
+        return abi::fail(SWB_ERR_ARG, "out and the prior rows must start on 8-byte boundaries");
+    if (sp.total && reinterpret_cast<uintptr_t>(workspace) % 16)
+        return abi::fail(SWB_ERR_ARG, "the workspace must start on a 16-byte boundary");
     cudaStream_t st = (cudaStream_t)stream;
     char* ws = static_cast<char*>(workspace);
     w.q = q;
