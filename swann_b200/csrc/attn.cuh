@@ -141,11 +141,13 @@ inline int check_cache(const swb_kv_cache* c, Cache* out) {
     if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16 || c->page_stride % 8 ||
         c->head_stride % 8 || c->row_stride % 8)
         return abi::fail(SWB_ERR_ARG, "cache: rows must start on 16-byte boundaries");
-    // without pages nothing is read, but copies of nothing want an address all the same
-    out->k = c->pages ? c->k : c->lengths;
-    out->v = c->pages ? c->v : c->lengths;
+    // without pages nothing is read, but 16-byte copies of nothing want an address all the
+    // same, on their boundary: lengths need not lie on one, the 16 bytes they begin in do
+    const void* none = reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(c->lengths) & ~(uintptr_t)15);
+    out->k = c->pages ? c->k : none;
+    out->v = c->pages ? c->v : none;
     out->page_stride = c->page_stride;
-    out->head_stride = c->head_stride;
+    out->head_stride = c->pages ? c->head_stride : 0;
     out->row_stride = c->row_stride;
     out->table = c->table;
     out->table_stride = c->table_stride;
