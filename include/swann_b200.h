@@ -347,8 +347,10 @@ typedef struct swb_kv_cache {
  * (i, i + rot_dim / 2), or (2i, 2i + 1) when interleaved), in 32 bits with one
  * rounding; queries to out [tokens, q_heads, head_dim], keys and values to
  * their slots.  Tokens of sequence b are starts[b] .. starts[b + 1] - 1 and take
- * the last of the lengths[b] slots, which count them already.  positions
- * [tokens], or NULL: a token's slot; one outside the tables gives NaN.
+ * the last of the lengths[b] slots, which count them already; a token of no
+ * sequence (below starts[0], from starts[seqs] on) is not stored.  positions
+ * [tokens], or NULL: a token's slot; one outside the tables gives NaN (without
+ * positions a token of no sequence is not rotated).
  * slot_positions [seqs, kv_heads, slot_width] records them, or NULL. */
 SWB_API int swb_rope_append(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
                     int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,

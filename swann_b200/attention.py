@@ -129,9 +129,10 @@ def rope_append(q, k, v, cos, sin, k_cache, v_cache, table, starts, lengths, *, 
 
     q [tokens, q_heads, d], k and v [tokens, kv_heads, d]: views into one
     projection are fine.  Tokens starts[b] .. starts[b + 1] - 1 (starts int32
-    [seqs + 1], from 0 to the number of tokens) are sequence b's, and take the last
-    of its lengths[b] slots: lengths count them already; a token whose slot the
-    table has no page for is not stored.  cos, sin float32 [positions, r / 2] rotate the
+    [seqs + 1], ascending) are sequence b's, and take the last of its lengths[b]
+    slots: lengths count them already.  A token whose slot the table has no page
+    for is not stored, nor is one of no sequence (a batch padded beyond
+    starts[seqs]), whose query is rotated only if `positions` has one.  cos, sin float32 [positions, r / 2] rotate the
     first r dimensions, pairs (i, i + r / 2) or, interleaved, (2i, 2i + 1), by
     the token's position: `positions` int32 [tokens], or its slot.  A position
     outside the tables gives NaN.  q_norm, k_norm [d]: weights of the norms,

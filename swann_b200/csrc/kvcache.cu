@@ -87,6 +87,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, APPEND_CTAS) append_kernel(con
     const bool turned = idx < hc;
 
     int b = 0;
+    bool ours = false;
     int64_t slot = 0, pos = 0, row = 0;
     float co[8], si[8];
     for (int hb = threadIdx.x / LPH; hb - (int)threadIdx.x / LPH < heads; hb += HP * U) {
@@ -104,14 +105,20 @@ __global__ void __launch_bounds__(APPEND_THREADS, APPEND_CTAS) append_kernel(con
             }
         }
         if (hb < HP) {
-            // the token's sequence: the last one that starts at or before it
+            // the token's sequence: the last one that starts at or before it, if it has not ended
+            // there; a token of none has no slot
             int hi = P.c.seqs;
             while (hi - b > 1) {
                 const int mid = (b + hi) >> 1;
                 if (P.starts[mid] <= tok) b = mid;
                 else hi = mid;
             }
-            slot = (int64_t)P.c.lengths[b] - (P.starts[b + 1] - tok);
+            slot = -1;
+            if (P.c.seqs > 0) {
+                const int from = P.starts[b], to = P.starts[b + 1];
+                ours = from <= tok && tok < to;
+                if (ours) slot = (int64_t)P.c.lengths[b] - (to - tok);
+            }
             pos = P.positions ? (int64_t)P.positions[tok] : slot;
             row = slot >= 0 && slot < P.c.capacity() ? P.c.row(b, (int)slot) : -1;
             if (turned) {
@@ -123,9 +130,13 @@ __global__ void __launch_bounds__(APPEND_THREADS, APPEND_CTAS) append_kernel(con
                         *reinterpret_cast<float4*>(co + 4 * e) = pc[e];
                         *reinterpret_cast<float4*>(si + 4 * e) = ps[e];
                     }
-                } else {                                    // a position outside the tables gives NaN
+                } else {                                    // a position outside the tables gives NaN, none no turn
+                    const bool none = !ours && !P.positions;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) co[e] = si[e] = __int_as_float(0x7fffffff);
+                    for (int e = 0; e < 8; ++e) {
+                        co[e] = none ? 1.f : __int_as_float(0x7fffffff);
+                        si[e] = none ? 0.f : __int_as_float(0x7fffffff);
+                    }
                 }
             }
         }
@@ -454,7 +465,7 @@ extern "C" int swb_rope_append(const void* q, int64_t q_token_stride, int64_t q_
     Append a = {};
     const int rc = check_cache(cache, &a.c);
     if (rc) return rc;
-    if (tokens <= 0 || a.c.seqs == 0) return SWB_OK;
+    if (tokens <= 0) return SWB_OK;
     if (!q || !k || !v || !starts || !out) return abi::fail(SWB_ERR_ARG, "null buffer");
     if (q_heads < 1 || q_heads % a.c.kv_heads)
         return abi::fail(SWB_ERR_ARG, "query heads must be a multiple of the cache's key heads");

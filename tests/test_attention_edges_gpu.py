@@ -27,3 +27,41 @@ def test_a_pool_without_pages_beside_lengths_on_any_boundary():
                 parts.append(A.prefill(q[:3], k, k, table, ints(0, 3), L))
             for out, lse in parts:
                 assert (out == 0).all() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("starts,own", [((0, 5, 9), (0, 9)), ((2, 2, 9), (2, 9)), ((0, 0, 0), (0, 0)), ((4, 11, 11), (4, 11))])
+@pytest.mark.parametrize("moved", [False, True])
+def test_append_leaves_tokens_of_no_sequence_out(starts, own, moved):
+    """A padded batch: the tables name pages beyond the lengths, and nothing is written there."""
+    k, v, table, L = make_cache([20, 9], 1, 64, 16, torch.float16, 23, max_pages=4, garbage=False)
+    table[:, 2:] = ints(3, 4)[:, None]
+    table[1, 1] = 5
+    k0, v0 = k.clone(), v.clone()
+    sp = torch.full((2, 1, 64), -7, dtype=torch.int32, device=DEV)
+    x = torch.randn((30, 4, 64), device=DEV).half()
+    angle = torch.rand((64, 32), device=DEV) * 6.28
+    cos, sin = angle.cos(), angle.sin()
+    pos = torch.randint(0, 64, (30,), device=DEV, dtype=torch.int32) if moved else None
+
+    def append(x, starts, pos):
+        return A.rope_append(x[:, :2], x[:, 2:3], x[:, 3:], cos, sin, k, v, table, starts, L, positions=pos, slot_positions=sp)
+
+    out = append(x, ints(*starts), pos)
+    k1, v1, sp1 = k.clone(), v.clone(), sp.clone()
+    k.copy_(k0), v.copy_(v0), sp.fill_(-7)
+    a, e = own
+    want = append(x[a:e], ints(*starts) - a, None if pos is None else pos[a:e])
+    assert torch.equal(k1, k) and torch.equal(v1, v) and torch.equal(sp1, sp)
+    assert int((v1 != v0).any(-1).sum()) == e - a
+    assert torch.equal(out[a:e], want)
+    rest = [t for t in range(30) if not a <= t < e]
+    if not moved:
+        assert torch.equal(out[rest], x[rest, :2])
+
+
+def test_append_without_sequences():
+    k, v, table, L = make_cache([8], 1, 64, 16, torch.float16, 24, garbage=False)
+    k0, x = k.clone(), torch.randn((3, 4, 64), device=DEV).half()
+    cos = torch.zeros((4, 32), device=DEV)
+    out = A.rope_append(x[:, :2], x[:, 2:3], x[:, 3:], cos, cos, k, v, table[:0], ints(0), L[:0])
+    assert torch.equal(out, x[:, :2]) and torch.equal(k, k0)
