@@ -309,17 +309,22 @@ class KVCache:
     def append(self, q, k, v, cos, sin, starts=None, *, q_norm=None, k_norm=None, eps=1e-6, interleaved=False):
         """New tokens' keys and values into their slots; returns their queries, normed and rotated.
 
-        starts int32 [seqs + 1]: tokens starts[b] .. starts[b + 1] - 1 are sequence b's; None: one token for each."""
-        starts = self._each if starts is None else starts
-        _ints("append", "starts", starts, (self.table.shape[0] + 1,), self.k.get_device())
+        starts int32 [seqs + 1], ascending from 0: tokens starts[b] .. starts[b + 1] - 1 are sequence b's, those
+        from starts[seqs] on no sequence's (a padded batch) and not stored; None: one token for each."""
+        seqs, n = self.table.shape[0], q.shape[0]
+        if starts is None:
+            if n != seqs:
+                _fail("append", f"without starts there must be one token for each of the {seqs} sequences")
+            starts = self._each
+        _ints("append", "starts", starts, (seqs + 1,), self.k.get_device())
         counts = starts.diff()
         lengths, seen = self.lengths + counts, self.seen + counts
         positions = None
-        if self._evicted:            # slots are no longer positions
-            n = q.shape[0]
-            at = torch.arange(n, dtype=torch.int32, device=q.device)
-            of = torch.repeat_interleave(seen - starts[1:], counts, output_size=n)
-            positions = (at + of).to(torch.int32)
+        if self._evicted and n and seqs:            # slots are no longer positions
+            at = torch.arange(n, dtype=torch.int32, device=starts.device)
+            # a token's sequence: whatever starts holds, one that there is
+            of = torch.searchsorted(starts[1:], at, right=True).clamp_(max=seqs - 1)
+            positions = at + (self.seen - starts[:-1])[of]
         out = rope_append(q, k, v, cos, sin, self.k, self.v, self.table, starts, lengths, q_norm=q_norm, k_norm=k_norm,
                           eps=eps, positions=positions, interleaved=interleaved, slot_positions=self.positions)
         self.lengths, self.seen = lengths, seen
