@@ -220,6 +220,9 @@ struct Evict {
     int32_t* moves;               // [seqs * kv_heads][2][budget]: from, to
     int32_t* counts;              // [seqs * kv_heads]
     int row_chunks;               // 16-byte chunks of a row
+
+    // slots of sequence b that there are: of the table and of a row of weights
+    __device__ __forceinline__ int held(int b) const { return (int)min((int64_t)c.length(b), width); }
 };
 
 constexpr int SELECT_THREADS = 1024;
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_kernel(const __grid_con
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t head = blockIdx.x;                       // sequence * kv_heads + key head
     const int b = (int)(head / P.c.kv_heads);
-    const int n = (int)max((int64_t)0, min((int64_t)P.c.lengths[b], min(P.c.capacity(), P.width)));
+    const int n = P.held(b);
     const int m = P.budget;
     const float* w = P.weights + head * P.width;
     const int32_t* pos = P.positions + head * P.width;
@@ -412,8 +415,7 @@ __global__ void __launch_bounds__(MOVE_THREADS) move_kernel(const __grid_constan
     float* nw = P.new_weights + head * P.width;
     int32_t* np = P.new_positions + head * P.width;
     {
-        const int64_t held = max(0, min(P.c.lengths[b], P.budget));
-        const int64_t j0 = held + (int64_t)blockIdx.y * MOVE_SLOTS, j1 = min(P.width, j0 + MOVE_SLOTS);
+        const int64_t j0 = min(P.held(b), P.budget) + (int64_t)blockIdx.y * MOVE_SLOTS, j1 = min(P.width, j0 + MOVE_SLOTS);
         for (int64_t j = j0 + threadIdx.x; j < j1; j += MOVE_THREADS) {
             nw[j] = 0.f;
             np[j] = -1;

@@ -2,9 +2,11 @@
 import math
 
 import pytest
+import test_attention_gpu as base
 import torch
 from test_attention_gpu import DEV, make_cache
 
+from swann_b200 import _lib as N
 from swann_b200 import attention as A
 
 pytestmark = pytest.mark.gpu
@@ -65,3 +67,30 @@ def test_append_without_sequences():
     cos = torch.zeros((4, 32), device=DEV)
     out = A.rope_append(x[:, :2], x[:, 2:3], x[:, 3:], cos, cos, k, v, table[:0], ints(0), L[:0])
     assert torch.equal(out, x[:, :2]) and torch.equal(k, k0)
+
+
+def evict_into(k, v, table, L, w, pos, budget, seen, sinks=0, recent=0):
+    """The native call with outputs that hold what no eviction gives; (lengths, weights, positions)."""
+    nl, nw, npos = torch.full_like(L, -9), torch.full_like(w, math.nan), torch.full_like(pos, -9)
+    arg, _ = A._cache_arg("evict", k, v, table, L)
+    need = N.lib().swb_kv_evict_workspace(w.shape[0], w.shape[1], budget)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    N.check(N.lib().swb_kv_evict(arg, seen.data_ptr(), w.data_ptr(), pos.data_ptr(), w.shape[2], budget, sinks, recent,
+                                 nl.data_ptr(), nw.data_ptr(), npos.data_ptr(), ws.data_ptr(), need,
+                                 torch.cuda.current_stream().cuda_stream))
+    return nl, nw, npos
+
+
+@pytest.mark.parametrize("lengths", [[1000, 64, 65], [2 ** 31 - 1, -3, 0], [63, 64, 100]])
+@pytest.mark.parametrize("budget", [10, 63, 64, 65, 150, 199, 200, 5000])
+def test_evict_writes_every_slot_whatever_the_lengths(lengths, budget):
+    """Lengths beyond the table and below nothing, and weights that are wider than the table."""
+    k, v, table, _ = make_cache([64] * 3, 2, 64, 16, torch.float16, 25, garbage=False)
+    L, W = ints(*lengths), 200
+    w = torch.rand((3, 2, W), device=DEV)
+    pos = torch.arange(W, device=DEV, dtype=torch.int32).expand(3, 2, W).contiguous()
+    cut = L.clamp(0, 64)
+    want = base.plain_evict(k, v, table, cut, w, pos, budget, cut, 0, 0)
+    got = (*evict_into(k, v, table, L, w, pos, budget, cut), k, v)
+    for a, c in zip(got, want):
+        assert torch.equal(a, c)
