@@ -63,6 +63,7 @@ constexpr int MMA_WARP = 8, PRODUCER0 = 9, PRODUCERS = 3;   // warps
 constexpr int SOFTMAX = 4;                  // warps of a tile
 constexpr int SEEN = 32;                    // steps whose rows are on record
 constexpr int LAG = 2;                      // parts of a warp in flight behind the one being issued
+constexpr int FOLD = 16;                    // steps whose weights are summed by themselves
 constexpr float RAISE = 8.f;                // log2 of how far a maximum may pass the one in use
 
 struct Prefill {
@@ -612,7 +613,11 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         const int ub = pos + 1 - J.base, us = max(J.first, P.sinks - J.base);
         const int ua = P.window > 0 ? pos - P.window + 1 - J.base : 0;
         float m = NEG_INF;
+        // the sum of the weights: of the last few steps, and of those before.  One running sum
+        // would lose, one by one, the thousands of weights below 2^-24 of it that a long flat
+        // tail has; what FOLD steps lose is below 2^-16 of it.
         float2 l[2] = {{0.f, 0.f}, {0.f, 0.f}};
+        float before = 0.f;
         bool ok = !*s_abort;
         for (int j = S.a; j < S.z; ++j) {
             const int i = j - S.a, all = done + i, u0 = j * STEP, buf = all & 1;
@@ -654,6 +659,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
                 if (raise) m = top;
                 l[0] = make_float2(l[0].x * f, l[0].y * f);
                 l[1] = make_float2(l[1].x * f, l[1].y * f);
+                before *= f;
                 if (i > 0) {
                     // the product of step i - 1 is done when the next logits are there, or at the
                     // last step when its own commit says so
@@ -696,6 +702,10 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
             tmem_stored();
             tc_fence_before();
             arrive_warp(&pbar[2 * t + buf]);
+            if ((i & (FOLD - 1)) == FOLD - 1) {
+                before += (l[0].x + l[0].y) + (l[1].x + l[1].y);
+                l[0] = l[1] = make_float2(0.f, 0.f);
+            }
         }
         // ---- the rows
         const int steps = S.z - S.a;
@@ -705,7 +715,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         ok = __all_sync(FULL, ok);
         if (!ok) *s_abort = 1;
         tc_fence_after();
-        const float sum = (l[0].x + l[0].y) + (l[1].x + l[1].y);
+        const float sum = before + ((l[0].x + l[0].y) + (l[1].x + l[1].y));
         const float inv = ok ? (sum == 0.f ? 0.f : 1.f / sum) : __int_as_float(0x7fffffff);
         const int64_t row = (J.token0 + t * P.tile_tokens + tok) * P.q_heads + J.head0 + r % J.heads;
         // through shared memory, so that a store writes whole 128-byte lines: 64 dimensions of

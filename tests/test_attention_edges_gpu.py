@@ -94,3 +94,20 @@ def test_evict_writes_every_slot_whatever_the_lengths(lengths, budget):
     got = (*evict_into(k, v, table, L, w, pos, budget, cut), k, v)
     for a, c in zip(got, want):
         assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prefill_sums_a_long_flat_tail(dtype):
+    """A first logit of 18 and 70000 of about 0: weights of 2^-26 that make up 2^-10 of the sum."""
+    n, new = 70000, 9
+    k, v, table, L = make_cache([n], 1, 64, 64, dtype, 3, garbage=False)
+    k.mul_(0.3)
+    k[..., 0] = 0
+    k[table[0, 0], :, 0, 0] = 2.25
+    q = (torch.randn((new, 4, 64), device=DEV) * 0.05).to(dtype)
+    q[..., 0] = 8
+    _, lse = A.prefill(q, k, v, table, ints(0, new), L, scale=1.0)
+    for t in (0, 4, 8):
+        for h in range(4):
+            _, wl, _, _, _, e = base.attend(q[t, h], k, v, table, 0, 0, n - new + t, 1.0, 0, 0, n)
+            assert abs(float(lse[t, h]) - wl) <= e + 2.0 ** -19 * (1 + abs(wl)), (float(lse[t, h]), wl)
