@@ -24,6 +24,10 @@ template <typename T>
 struct Elem;
 template <>
 struct Elem<__half> {
+    // A softmax weight that is rounded to this type is taken 2^x times larger, x so that the
+    // largest comes to 2^TOP: fp16's steps end at 2^-24, and a weight of 2^-25 of the largest
+    // would be 0 in the product with V but count in the sum.
+    static constexpr float TOP = 15.f;
     static __device__ __forceinline__ float2 wide(uint32_t u) {
         return __half22float2(*reinterpret_cast<const __half2*>(&u));
     }
@@ -40,6 +44,7 @@ struct Elem<__half> {
 };
 template <>
 struct Elem<__nv_bfloat16> {
+    static constexpr float TOP = 0.f;      // has the exponents of fp32
     static __device__ __forceinline__ float2 wide(uint32_t u) {
         return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
     }

@@ -31,7 +31,10 @@
 // The running maximum that the exponentials are taken against is only raised when
 // a row's maximum has passed it by 2^8 (weights stay below 2^8 and sums in range);
 // only then is O rescaled in TMEM, which the first blocks of a row need and later
-// ones hardly ever do.
+// ones hardly ever do.  In fp16 the weights and their sum are 2^7 times that, up to
+// 2^15 (no instruction more: the exponents' offset is another one), so that what a
+// long flat tail has is not lost beside one strong key: a weight that vanishes is
+// below 2^-32 of the one at the maximum in use.
 //
 // MMAs of one thread run in order, so the logits of step i + 1 may be issued right
 // after the product that reads step i - 1's weights, which lie in the same columns.
@@ -612,6 +615,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         // of the places that hold something the row sees u < us and ua <= u, below ub
         const int ub = pos + 1 - J.base, us = max(J.first, P.sinks - J.base);
         const int ua = P.window > 0 ? pos - P.window + 1 - J.base : 0;
+        constexpr float LIFT = Elem<T>::TOP > RAISE ? Elem<T>::TOP - RAISE : 0.f;   // log2 of what weights are multiplied by
         float m = NEG_INF;
         // the sum of the weights: of the last few steps, and of those before.  One running sum
         // would lose, one by one, the thousands of weights below 2^-24 of it that a long flat
@@ -681,7 +685,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
                     tmem_stored();
                 }
             }
-            const float off = m == NEG_INF ? 0.f : -m;
+            const float off = m == NEG_INF ? 0.f : LIFT - m;
             // weights over the logits' columns
             const unsigned long long s2 = pair(P.scale2, P.scale2), o2 = pair(off, off);
             unsigned long long l2[2] = {pair(l[0].x, l[0].y), pair(l[1].x, l[1].y)};
@@ -752,7 +756,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
             }
             __syncwarp();
         }
-        if (live) P.lse[row] = !ok ? inv : sum == 0.f ? NEG_INF : (m + log2f(sum)) * LN2;
+        if (live) P.lse[row] = !ok ? inv : sum == 0.f ? NEG_INF : (m - LIFT + log2f(sum)) * LN2;
         if (J.steps) stage0 += J.steps + 2;
         done += steps;
         ends += steps > 0;

@@ -111,3 +111,46 @@ def test_prefill_sums_a_long_flat_tail(dtype):
         for h in range(4):
             _, wl, _, _, _, e = base.attend(q[t, h], k, v, table, 0, 0, n - new + t, 1.0, 0, 0, n)
             assert abs(float(lse[t, h]) - wl) <= e + 2.0 ** -19 * (1 + abs(wl)), (float(lse[t, h]), wl)
+
+
+# -- one strong key beside a long flat tail ---------------------------------------------
+#
+# The first slot's logit is 18 above all others', whose weights are then about 2^-26 of
+# the largest, and its value is 0: what comes out is the tail's.  fp16's smallest numbers
+# are 2^-24 apart, so a weight among them is rounded by up to 2^-25, however small it is
+# itself: with weights multiplied by 2^x, by 2^-(25 + x) of the largest weight, x = 7 in
+# prefill and 15 in decode.  That, for every visible slot and times the largest |v| of 1.5,
+# is added to the bound of a weight's relative rounding.
+
+def peaked(lengths, hq, hkv, d, page, dtype, tokens, seed=3):
+    k, v, table, L = make_cache(lengths, hkv, d, page, dtype, seed, garbage=False)
+    g = torch.Generator(device=DEV).manual_seed(seed + 1)
+    k.mul_(0.3)
+    k[..., 0] = 0
+    v.copy_(torch.rand(v.shape, generator=g, device=DEV) + 0.5)
+    for b in range(len(lengths)):
+        k[table[b, 0], :, 0, 0] = 2.25
+        v[table[b, 0], :, 0] = 0
+    q = (torch.randn((tokens, hq, d), generator=g, device=DEV) * 0.05).to(dtype)
+    q[..., 0] = 8
+    return q, k, v, table, L
+
+
+def check_tail(out, lse, want, u, lost):
+    j, wl, wo, wa, _, e = want
+    assert abs(float(lse) - wl) <= e + 2.0 ** -19 * (1 + abs(wl))
+    bound = u * wo.abs() + (u + 2 * e + 2.0 ** -18) * wa + 2.0 ** -25 + len(j) * 1.5 * lost
+    over = ((out.double() - wo).abs() / bound).max()
+    assert over <= 1, float(over)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,new,hq,hkv,d,window", [(3000, 200, 2, 2, 64, 0), (3000, 200, 8, 2, 128, 0), (70000, 9, 4, 1, 64, 0),
+                                                   (3000, 200, 4, 2, 64, 1500)])
+def test_prefill_keeps_a_long_flat_tail(n, new, hq, hkv, d, window, dtype):
+    q, k, v, table, L = peaked([n], hq, hkv, d, 64, dtype, new)
+    out, lse = A.prefill(q, k, v, table, ints(0, new), L, scale=1.0, window=window, sinks=1 if window else 0)
+    for t in (0, new // 2, new - 1):
+        for h in {0, hq - 1}:
+            want = base.attend(q[t, h], k, v, table, 0, h * hkv // hq, n - new + t, 1.0, window, 1 if window else 0, n)
+            check_tail(out[t, h], lse[t, h], want, base.U[dtype], 2.0 ** -32)
