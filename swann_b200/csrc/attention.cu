@@ -19,7 +19,9 @@
 // its 8 columns, so a group of up to 8 heads wastes little (a tcgen05 tile of 128
 // would be nine tenths empty, and the tensor pipe is not what bounds this).
 // Weights are rounded to the cache's 16 bits for the second product, as its other
-// operand is; their sum l is taken before that.
+// operand is; their sum l is taken before that.  In fp16 they and l are 2^15 times
+// what they are against the running maximum, so that those of a long flat tail
+// beside one strong key stay far above fp16's smallest steps.
 //
 // Who walks what.  Few pairs: the pairs' units of 64 keys are laid end to end
 // and every CTA of a grid that the SMs hold at once takes an equal run of them,
@@ -171,6 +173,7 @@ constexpr int cta_per_sm(int d) { return d == 128 ? 2 : 4; }
 template <typename T, int D, int NT>
 struct Rows {
     static constexpr int MT = D / 16;
+    static constexpr float LIFT = Elem<T>::TOP;        // log2 of what weights are multiplied by
     float o[MT][NT][4], m[NT][2], l[NT][2];
     uint32_t q[D / 16][NT][2];                         // the query rows as fragments of the second operand
 
@@ -253,7 +256,7 @@ struct Rows {
         uint32_t pf[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float s0 = m[n][0] == NEG_INF ? 0.f : m[n][0], s1 = m[n][1] == NEG_INF ? 0.f : m[n][1];
+            const float s0 = m[n][0] == NEG_INF ? 0.f : m[n][0] - LIFT, s1 = m[n][1] == NEG_INF ? 0.f : m[n][1] - LIFT;
             const float w0 = exp2_fast(y[n][0] - s0), w1 = exp2_fast(y[n][1] - s1);
             const float w2 = exp2_fast(y[n][2] - s0), w3 = exp2_fast(y[n][3] - s1);
             l[n][0] += w0 + w2;
@@ -270,14 +273,17 @@ struct Rows {
             for (int n = 0; n < NT; ++n) Elem<T>::mma(o[j][n], f, pf[n][0], pf[n][1]);
         }
     }
-    // the sums over all keys: l of a column in every lane that has it
+    // the sums over all keys: l of a column in every lane that has it; from here on m is
+    // what l and o are weights against, LIFT below the maximum
     __device__ __forceinline__ void sum() {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 2; ++e) {
 #pragma unroll
                 for (int s = 4; s <= 16; s <<= 1) l[n][e] += __shfl_xor_sync(FULL, l[n][e], s);
+                m[n][e] -= LIFT;
+            }
     }
 };
 

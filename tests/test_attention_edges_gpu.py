@@ -154,3 +154,30 @@ def test_prefill_keeps_a_long_flat_tail(n, new, hq, hkv, d, window, dtype):
         for h in {0, hq - 1}:
             want = base.attend(q[t, h], k, v, table, 0, h * hkv // hq, n - new + t, 1.0, window, 1 if window else 0, n)
             check_tail(out[t, h], lse[t, h], want, base.U[dtype], 2.0 ** -32)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("B,n,hq,hkv,d", [
+    (1, 3000, 8, 1, 128),       # runs of one unit
+    (40, 3000, 16, 8, 64),      # runs longer than a pair
+    (40, 3000, 160, 8, 64),     # and of two products' rows
+    (640, 400, 4, 1, 64),       # a warp a pair
+    (640, 400, 1, 1, 128)])     # of one row
+def test_decode_keeps_a_long_flat_tail(B, n, hq, hkv, d, dtype):
+    q, k, v, table, L = peaked([n] * B, hq, hkv, d, 16, dtype, B)
+    prior = (torch.full((B, hq, d), 0.5, device=DEV).to(dtype), torch.full((B, hq), 0.0, device=DEV))
+    w = torch.empty((B, hkv, table.shape[1] * 16), device=DEV)
+    out, lse = A.decode(q, k, v, table, L, scale=1.0)
+    both = A.decode(q, k, v, table, L, scale=1.0, prior=prior, weights=w)
+    for b in (0, B - 1):
+        for h in {0, hq - 1}:
+            j, wl, wo, wa, p, e = want = base.attend(q[b, h], k, v, table, b, h * hkv // hq, n - 1, 1.0, 0, 0, n)
+            check_tail(out[b, h], lse[b, h], want, base.U[dtype], 2.0 ** -40)
+            # with a part of lse 0 beside it: e^-wl of the sum
+            x = math.exp(-wl) / (1 + math.exp(-wl))
+            y = (1 - x) * wo + x * 0.5
+            check_tail(both[0][b, h], both[1][b, h], (j, math.log(math.exp(wl) + 1), y, y.abs(), p, e), base.U[dtype], 2.0 ** -40)
+        tail = w[b, 0, 1:n].double().sum()
+        heads = hq // hkv
+        want = sum(float(base.attend(q[b, h], k, v, table, b, 0, n - 1, 1.0, 0, 0, n)[4][1:].sum()) for h in range(heads))
+        assert abs(float(tail) - want) <= (2 * e + 2.0 ** -18) * want
