@@ -24,7 +24,7 @@ nothing.  With pages of one row the table lists rows: the ids that
 `KVCache` keeps the pieces together for the ordinary case.  Nothing here reads
 a device value on the host: the calls queue on the current stream and can be
 captured in a CUDA graph.  There is no backward pass: the package serves
-models, it does not train them.
+models, it does not train them, and refuses tensors that want a gradient.
 """
 from __future__ import annotations
 
@@ -55,6 +55,12 @@ def _call(what, fn, t, *args):
         N.check(rc, what)
 
 
+def _no_gradient(what, name, t):
+    """A gradient would be lost without a word."""
+    if t.requires_grad and torch.is_grad_enabled():
+        _fail(what, f"{name} requires a gradient, and there is no backward pass: call under torch.no_grad()")
+
+
 def _ints(what, name, t, shape, dev):
     if t.dtype is not torch.int32 or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
         _fail(what, f"{name} must be contiguous int32 {list(shape)} on cuda:{dev}")
@@ -71,6 +77,8 @@ def _cache_arg(what, k, v, table, lengths):
     shape, strides = k.shape, k.stride()
     if len(shape) != 4 or v.shape != shape or v.stride() != strides or v.get_device() != dev:
         _fail(what, "k and v must be [pages, kv_heads, page_size, head_dim] with the same strides")
+    _no_gradient(what, "the cache", k)
+    _no_gradient(what, "the cache", v)
     pages, heads, page, d = shape
     ps, hs, rs, es = strides
     if d not in HEAD_DIMS:
@@ -100,14 +108,14 @@ def _heads(what, name, t, d, dtype, dev, heads=None):
         _fail(what, f"{name} must have {heads} heads")
     if strides[2] != 1:
         _fail(what, f"the rows of {name} must be contiguous")
-    if t.requires_grad and torch.is_grad_enabled():
-        _fail(what, f"{name} requires a gradient, and there is no backward pass: call under torch.no_grad()")
+    _no_gradient(what, name, t)
     return shape, strides
 
 
 def _given(what, name, t, shape, dtype, dev):
     if t.shape != shape or t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
         _fail(what, f"{name} must be contiguous {dtype} {list(shape)} on cuda:{dev}")
+    _no_gradient(what, name, t)
     return t
 
 
@@ -155,6 +163,7 @@ def rope_append(q, k, v, cos, sin, k_cache, v_cache, table, starts, lengths, *, 
     for t in (cos, sin):
         if t.dtype is not torch.float32 or t.get_device() != dev or not t.is_contiguous():
             _fail(what, f"cos and sin must be contiguous float32 on cuda:{dev}")
+        _no_gradient(what, "the rotation table", t)
     if q_norm is not None:
         _given(what, "q_norm", q_norm, (d,), q.dtype, dev)
     if k_norm is not None:

@@ -181,3 +181,37 @@ def test_decode_keeps_a_long_flat_tail(B, n, hq, hkv, d, dtype):
         heads = hq // hkv
         want = sum(float(base.attend(q[b, h], k, v, table, b, 0, n - 1, 1.0, 0, 0, n)[4][1:].sum()) for h in range(heads))
         assert abs(float(tail) - want) <= (2 * e + 2.0 ** -18) * want
+
+
+def every_call():
+    """Each call's tensors of numbers by name, and the calls."""
+    k, v, table, L = make_cache([40, 8], 2, 64, 16, torch.float16, 41, garbage=False)
+    x = torch.randn((2, 8, 64), device=DEV).half()
+    starts, seen = ints(0, 1, 2), L.clone()
+    half = dict(q=x[:, :4].contiguous(), kn=x[:, 4:6], vn=x[:, 6:], k=k, v=v, q_norm=torch.ones(64, device=DEV).half(),
+                k_norm=torch.ones(64, device=DEV).half(), prior=torch.zeros((2, 4, 64), device=DEV).half(),
+                out=torch.zeros((2, 4, 64), device=DEV).half())
+    full = dict(cos=torch.ones((64, 32), device=DEV), sin=torch.zeros((64, 32), device=DEV), prior_lse=torch.zeros((2, 4), device=DEV),
+                weights=torch.zeros((2, 2, 48), device=DEV))
+    pos = torch.zeros((2, 2, 48), dtype=torch.int32, device=DEV)
+    calls = {
+        "rope_append": lambda t: A.rope_append(t["q"], t["kn"], t["vn"], t["cos"], t["sin"], t["k"], t["v"], table, starts, L,
+                                               q_norm=t["q_norm"], k_norm=t["k_norm"], out=t["out"]),
+        "decode": lambda t: A.decode(t["q"], t["k"], t["v"], table, L, prior=(t["prior"], t["prior_lse"]), weights=t["weights"], out=t["out"]),
+        "prefill": lambda t: A.prefill(t["q"], t["k"], t["v"], table, starts, L, out=t["out"]),
+        "evict": lambda t: A.evict(t["k"], t["v"], table, L, t["weights"], pos, 8, seen=seen)}
+    return {**half, **full}, calls
+
+
+@pytest.mark.parametrize("call,names", [
+    ("rope_append", ["q", "kn", "vn", "cos", "sin", "k", "v", "q_norm", "k_norm", "out"]),
+    ("decode", ["q", "k", "v", "prior", "prior_lse", "weights", "out"]), ("prefill", ["q", "k", "v", "out"]), ("evict", ["k", "v", "weights"])])
+def test_no_tensor_that_wants_a_gradient_is_taken(call, names):
+    tensors, calls = every_call()
+    calls[call](tensors)
+    for name in names:
+        wants = {**tensors, name: tensors[name].detach().clone().requires_grad_()}
+        with pytest.raises(ValueError, match="no backward pass"):
+            calls[call](wants)
+        with torch.no_grad():
+            calls[call](wants)
