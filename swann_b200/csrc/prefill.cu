@@ -272,6 +272,10 @@ struct Job {
     __device__ __forceinline__ bool holds(int u) const { return u < n && (u < first || base + u >= lo); }
 };
 
+// how far x lies past y, 0 if it does not; x and y differ by up to 2^32: a window may be
+// any 32-bit number, and tokens lie before slot 0 where lengths do not count them all
+__device__ __forceinline__ int past(int64_t x, int64_t y) { return (int)max((int64_t)0, x - y); }
+
 // item `item` of all; false past the last
 __device__ __forceinline__ bool find_job(const Prefill& P, int item, Job& J) {
     if (item >= P.items) return false;
@@ -289,7 +293,7 @@ __device__ __forceinline__ bool find_job(const Prefill& P, int item, Job& J) {
         if (mine < P.c.seqs) {
             from = (int)clamp_start(P.starts, mine, P.tokens);
             n = (int)clamp_start(P.starts, mine + 1, P.tokens) - from;
-            held = P.c.lengths[mine];
+            held = max(0, P.c.lengths[mine]);
             t = n > 0 ? (n + step - 1) / step : 0;
         }
         int sum = t;
@@ -320,7 +324,7 @@ __device__ __forceinline__ bool find_job(const Prefill& P, int item, Job& J) {
     J.live = min(step, ntok - tile * step);
     J.pos0 = length - ntok + tile * step;
     const int end = (int)max((int64_t)0, min((int64_t)J.pos0 + J.live, P.c.capacity()));
-    J.lo = P.window > 0 ? min(max(0, J.pos0 - P.window + 1), end) : 0;
+    J.lo = P.window > 0 ? min(past((int64_t)J.pos0 + 1, P.window), end) : 0;
     J.first = min(P.sinks, J.lo);
     J.base = (J.lo - J.first) / STEP * STEP;
     J.n = end - J.base;
@@ -342,9 +346,9 @@ __device__ __forceinline__ Span span_of(const Prefill& P, const Job& J, int t) {
     const int ub = min(J.n, s.pos + s.tokens - J.base);               // end of what its last token sees
     s.z = (max(0, ub) + STEP - 1) / STEP;
     // what its first token sees begins here, but for first tokens
-    if (P.window > 0 && P.sinks == 0) s.a = min(s.z, max(0, s.pos - P.window + 1 - J.base) / STEP);
+    if (P.window > 0 && P.sinks == 0) s.a = min(s.z, past((int64_t)s.pos + 1 - J.base, P.window) / STEP);
     // from where its last token's window has begun, to what its first token sees
-    s.f0 = P.window > 0 ? (max(0, s.pos + s.tokens - P.window - J.base) + STEP - 1) / STEP : 0;
+    s.f0 = P.window > 0 ? (past((int64_t)s.pos + s.tokens - J.base, P.window) + STEP - 1) / STEP : 0;
     s.f1 = max(0, s.pos + 1 - J.base) / STEP;
     return s;
 }
@@ -614,7 +618,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         const uint32_t ot = tmem + quarter + 2 * TILE + t * D;
         // of the places that hold something the row sees u < us and ua <= u, below ub
         const int ub = pos + 1 - J.base, us = max(J.first, P.sinks - J.base);
-        const int ua = P.window > 0 ? pos - P.window + 1 - J.base : 0;
+        const int ua = P.window > 0 ? past((int64_t)pos + 1 - J.base, P.window) : 0;
         constexpr float LIFT = Elem<T>::TOP > RAISE ? Elem<T>::TOP - RAISE : 0.f;   // log2 of what weights are multiplied by
         float m = NEG_INF;
         // the sum of the weights: of the last few steps, and of those before.  One running sum

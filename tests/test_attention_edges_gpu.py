@@ -215,3 +215,17 @@ def test_no_tensor_that_wants_a_gradient_is_taken(call, names):
             calls[call](wants)
         with torch.no_grad():
             calls[call](wants)
+
+
+@pytest.mark.parametrize("length", [0, 5, 9, 64, 70, 100, 2 ** 31 - 1, -7, -2 ** 31])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (3, 0), (3, 2), (2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (2 ** 31 - 5, 1)])
+def test_prefill_of_lengths_that_the_tokens_or_the_table_do_not_fit(length, window, sinks):
+    """Fewer slots than new tokens: the first lie before slot 0 and see nothing.  More than the table: no slot there."""
+    k, v, table, _ = make_cache([64], 1, 64, 16, torch.float16, 6)
+    q = torch.randn((70, 2, 64), device=DEV).half()
+    out, lse = A.prefill(q, k, v, table, ints(0, 70), ints(length), window=window, sinks=sinks)
+    n = max(0, length)
+    for t in (0, 1, 5, 31, 60, 61, 64, 65, 66, 69):
+        for h in range(2):
+            want = base.attend(q[t, h], k, v, table, 0, 0, n - 70 + t, 0.125, window, sinks, n)
+            base.check_row(out[t, h], lse[t, h], want, base.U[torch.float16])
