@@ -79,13 +79,16 @@ __device__ __forceinline__ Range visible(int pos, int window, int sinks, int64_t
     return r;
 }
 
+// the slot of sequence b's newest token, -1 without one
+__device__ __forceinline__ int newest(const Cache& c, int b) { return max(c.lengths[b], 0) - 1; }
+
 template <int D>
 __device__ __forceinline__ uint32_t swz(int row, int chunk) {
     return (uint32_t)(row * D * 2 + ((chunk ^ (row & 7)) << 4));
 }
 
 __device__ __forceinline__ int units_of(const Walk& P, int b) {
-    const Range r = visible(P.c.lengths[b] - 1, P.window, P.sinks, P.c.capacity());
+    const Range r = visible(newest(P.c, b), P.window, P.sinks, P.c.capacity());
     return max(1, (r.n + UNIT - 1) / UNIT);
 }
 
@@ -357,7 +360,7 @@ __global__ void __launch_bounds__(WARPS * 32, cta_per_sm(D)) walk_kernel(const _
         const int b = at.b, g = at.h / P.head_tiles, ht = at.h % P.head_tiles;
         const int heads = min(P.tile_heads, P.group - ht * P.tile_heads);
         const int64_t row0 = (int64_t)b * P.q_heads + g * P.group + ht * P.tile_heads;   // first output row
-        const Range rg = visible(P.c.lengths[b] - 1, P.window, P.sinks, P.c.capacity());
+        const Range rg = visible(newest(P.c, b), P.window, P.sinks, P.c.capacity());
         const int take = min(left, at.units - at.unit);
         const int u0 = min(rg.n, at.unit * UNIT), u1 = min(rg.n, u0 + take * UNIT);
         const bool entire = take == at.units;          // nothing of the pair is left to others
@@ -491,7 +494,7 @@ __global__ void __launch_bounds__(32, pair_ctas(D)) pair_kernel(const __grid_con
     const int b = (int)(blockIdx.x / tiles), h = (int)(blockIdx.x % tiles), g = h / P.head_tiles, ht = h % P.head_tiles;
     const int heads = min(P.tile_heads, P.group - ht * P.tile_heads), head0 = g * P.group + ht * P.tile_heads;
     const int64_t row0 = (int64_t)b * P.q_heads + head0;
-    const Range rg = visible(P.c.lengths[b] - 1, P.window, P.sinks, P.c.capacity());
+    const Range rg = visible(newest(P.c, b), P.window, P.sinks, P.c.capacity());
     const int blocks = (rg.n + KEYS - 1) / KEYS;
     const T* kp = static_cast<const T*>(P.c.k) + (int64_t)g * P.c.head_stride;
     const T* vp = static_cast<const T*>(P.c.v) + (int64_t)g * P.c.head_stride;
@@ -564,7 +567,7 @@ __global__ void __launch_bounds__(ROW_WARPS * 32, 7) row_kernel(const __grid_con
     const int64_t pair = (int64_t)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
     if (pair >= pairs) return;                                   // whole warps; nothing below is the CTA's
     const int b = (int)(pair / P.c.kv_heads), g = (int)(pair % P.c.kv_heads);
-    const Range rg = visible(P.c.lengths[b] - 1, P.window, P.sinks, P.c.capacity());
+    const Range rg = visible(newest(P.c, b), P.window, P.sinks, P.c.capacity());
     const int64_t head = (int64_t)g * P.c.head_stride + c * 8;
     const T* kp = static_cast<const T*>(P.c.k) + head;
     const T* vp = static_cast<const T*>(P.c.v) + head;

@@ -229,3 +229,15 @@ def test_prefill_of_lengths_that_the_tokens_or_the_table_do_not_fit(length, wind
         for h in range(2):
             want = base.attend(q[t, h], k, v, table, 0, 0, n - 70 + t, 0.125, window, sinks, n)
             base.check_row(out[t, h], lse[t, h], want, base.U[torch.float16])
+
+
+@pytest.mark.parametrize("B,hq", [(1, 4), (700, 4), (700, 1)])
+@pytest.mark.parametrize("length", [0, -1, -2 ** 31])
+def test_decode_of_lengths_below_nothing(B, hq, length):
+    k, v, table, _ = make_cache([64], 1, 64, 16, torch.float16, 6)
+    table, L = table.expand(B, 4), torch.full((B,), length, dtype=torch.int32, device=DEV)
+    w = torch.full((B, 1, 64), math.nan, device=DEV)
+    q = torch.randn((B, hq, 64), device=DEV).half()
+    for window in (0, 5, 2 ** 31 - 1):
+        out, lse = A.decode(q, k, v, table, L, window=window, sinks=2, weights=w)
+        assert (out == 0).all() and (lse == -math.inf).all() and (w == 0).all()
