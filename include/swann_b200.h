@@ -380,7 +380,8 @@ SWB_API uint64_t swb_attn_decode_workspace(const swb_kv_cache* cache, int q_head
 
 /* Attention of many new tokens, the last of their sequences' slots (starts as
  * in swb_rope_append, the keys written before): the token at slot i sees the
- * slots j <= i with window == 0, j > i - window or j < sinks.
+ * slots j <= i with window == 0, j > i - window or j < sinks.  What sees nothing,
+ * a token of no sequence among it, gives 0 and -inf.
  * q [tokens, q_heads, head_dim]; out and lse contiguous, out on a 16-byte boundary.
  *   status   optional int32 device word: SWB_ERR_TIMEOUT where a bounded device-side
  *            wait gave up (the rows concerned are NaN) */

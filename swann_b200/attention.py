@@ -229,7 +229,8 @@ def prefill(q, k_cache, v_cache, table, starts, lengths, *, scale=None, window=0
     q [tokens, q_heads, d]; starts and lengths as in `rope_append`, which has
     written the tokens' keys: a token at slot i sees the slots j <= i and, with
     a window, of those only j > i - window and j < sinks.  Returns out
-    [tokens, q_heads, d] and lse float32 [tokens, q_heads]."""
+    [tokens, q_heads, d] and lse float32 [tokens, q_heads], 0 and -inf where
+    nothing is seen and for tokens of no sequence."""
     what = "prefill"
     arg, dev = _cache_arg(what, k_cache, v_cache, table, lengths)
     d = arg.head_dim

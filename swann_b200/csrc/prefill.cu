@@ -545,6 +545,14 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         stage0 += J.steps + 2;
         ++jobs;
         }
+        // tokens of no sequence, before the first or after the last, see nothing
+        const int64_t s0 = clamp_start(P.starts, 0, P.tokens), s1 = max(s0, clamp_start(P.starts, P.c.seqs, P.tokens));
+        for (int64_t i = (int64_t)blockIdx.x * PRODUCERS + w; i < s0 + P.tokens - s1; i += (int64_t)gridDim.x * PRODUCERS) {
+            const int64_t row = (i < s0 ? i : s1 + i - s0) * P.q_heads;
+            for (int64_t c = lane; c < (int64_t)P.q_heads * CH; c += 32)
+                *reinterpret_cast<uint4*>(static_cast<T*>(P.out) + row * D + c * 8) = make_uint4(0u, 0u, 0u, 0u);
+            for (int h = lane; h < P.q_heads; h += 32) P.lse[row + h] = NEG_INF;
+        }
     } else if (warp == MMA_WARP) {
         // ---------------- MMA issuer
         const uint32_t tm = __shfl_sync(FULL, tmem, 0);
@@ -828,7 +836,7 @@ extern "C" int swb_attn_prefill(const void* q, int64_t q_token_stride, int64_t q
     pre::Prefill p = {};
     int rc = check_cache(cache, &p.c);
     if (rc) return rc;
-    if (p.c.seqs == 0 || tokens <= 0) return SWB_OK;
+    if (tokens <= 0) return SWB_OK;
     rc = check_query(q, q_token_stride, q_head_stride, q_heads, p.c);
     if (rc) return rc;
     if (!starts || !out || !lse) return abi::fail(SWB_ERR_ARG, "null buffer");

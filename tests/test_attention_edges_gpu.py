@@ -241,3 +241,34 @@ def test_decode_of_lengths_below_nothing(B, hq, length):
     for window in (0, 5, 2 ** 31 - 1):
         out, lse = A.decode(q, k, v, table, L, window=window, sinks=2, weights=w)
         assert (out == 0).all() and (lse == -math.inf).all() and (w == 0).all()
+
+
+def prefill_into(q, k, v, table, starts, L, dtype):
+    """The native call with outputs that hold NaN."""
+    T, hq, d = q.shape
+    out, lse = torch.full((T, hq, d), math.nan, dtype=dtype, device=DEV), torch.full((T, hq), math.nan, device=DEV)
+    arg, _ = A._cache_arg("prefill", k, v, table, L)
+    N.check(N.lib().swb_attn_prefill(q.data_ptr(), hq * d, d, hq, starts.data_ptr(), T, arg, d ** -0.5, 0, 0, out.data_ptr(),
+                                     lse.data_ptr(), None, torch.cuda.current_stream().cuda_stream))
+    return out, lse
+
+
+@pytest.mark.parametrize("starts", [(0, 20, 30), (3, 20, 30), (7, 7, 7), (0, 0, 0), (40, 40, 40), (0, 40, 40), (2, 5, 1000)])
+@pytest.mark.parametrize("T", [40, 1000])
+@pytest.mark.parametrize("hq,d", [(2, 64), (40, 128)])
+def test_prefill_writes_every_row_of_a_padded_batch(starts, T, hq, d):
+    k, v, table, L = make_cache([50, 60], 2, d, 16, torch.float16, 16)
+    q = torch.randn((T, hq, d), device=DEV).half()
+    out, lse = prefill_into(q, k, v, table, ints(*starts), L, torch.float16)
+    a, e = min(T, starts[0]), min(T, starts[2])
+    for none in (slice(0, a), slice(e, T)):
+        assert (out[none] == 0).all() and (lse[none] == -math.inf).all()
+    if e > a:
+        want = A.prefill(q[a:e].contiguous(), k, v, table, ints(*(min(T, s) - a for s in starts)), L)
+        assert torch.equal(out[a:e], want[0]) and torch.equal(lse[a:e], want[1])
+
+
+def test_prefill_without_sequences():
+    k, v, table, L = make_cache([8], 1, 64, 16, torch.float16, 24)
+    out, lse = prefill_into(torch.randn((5, 2, 64), device=DEV).half(), k, v, table[:0], ints(0), L[:0], torch.float16)
+    assert (out == 0).all() and (lse == -math.inf).all()
