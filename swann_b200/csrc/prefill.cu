@@ -40,7 +40,8 @@
 // after the product that reads step i - 1's weights, which lie in the same columns.
 // CTAs stay and take job after job, the longest first; queries, keys and logits of
 // the next one are under way while the last rows of this one are written.  All waits
-// are bounded; if one runs out the CTA's rows are NaN and the status word is set.
+// are bounded; if one runs out the CTA's rows are NaN and the status word is set, once
+// copies and products in flight are done (or have had milliseconds to).
 //
 // Measured: 2049 tokens over 8193 slots, 32 heads of 128 over 8: 235 us, 1025 TFLOP/s
 // (61% of a cuBLAS bf16 product's rate).  A step of the two tiles takes about 1700
@@ -94,8 +95,8 @@ struct Layout {
     static constexpr int SLOTS = D == 128 ? 4 : 8;
     static constexpr int Q = 0;                                 // two tiles
     static constexpr int RING = 2 * QB;
-    static constexpr int BARS = RING + SLOTS * STAGEB;          // full, empty, q, q let go, s[2][2], p[2][2], o[2][2]
-    static constexpr int SEENB = BARS + (2 * SLOTS + 14) * 8;   // uint32 [SEEN][2], on an 8-byte boundary
+    static constexpr int BARS = RING + SLOTS * STAGEB;          // full, empty, q, q let go, s[2][2], p[2][2], o[2][2], end
+    static constexpr int SEENB = BARS + (2 * SLOTS + 15) * 8;   // uint32 [SEEN][2], on an 8-byte boundary
     static constexpr int OUT = (SEENB + SEEN * 2 * 4 + 15) / 16 * 16;   // a warp's 32 rows of 64 dimensions, on their way out
     static constexpr int TOTAL = OUT + 2 * SOFTMAX * 32 * 128;
 };
@@ -242,13 +243,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // mbar_wait with nothing on the way of a phase that is complete: the clock is only
 // read after many tries
-__device__ __forceinline__ bool await(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool await(uint64_t* bar, uint32_t parity, long long limit = 1ll << 32) {
     long long t0 = 0;
     for (uint32_t n = 1; !mbar_try_wait(bar, parity); ++n) {
         if ((n & 255u) == 0) {
             const long long t = clock64();
             if (t0 == 0) t0 = t;
-            else if (t - t0 > (1ll << 32)) return false;
+            else if (t - t0 > limit) return false;
         }
     }
     return true;
@@ -367,6 +368,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     uint64_t* sbar = qbar + 2;           // [tile][buffer]
     uint64_t* pbar = sbar + 4;
     uint64_t* obar = pbar + 4;
+    uint64_t* endbar = obar + 4;         // all products
     volatile uint32_t* s_seen = reinterpret_cast<volatile uint32_t*>(sm + Ly::SEENB);
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort_store;
@@ -388,6 +390,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
                 mbar_init(&obar[2 * t + k], 1);   // the product of the last step but one, and of the last
             }
         }
+        mbar_init(endbar, 1);
         fence_mbar_init();
     }
     if (warp == MMA_WARP) {
@@ -417,6 +420,7 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
             }
         };
         constexpr int QPIECES = TILE / 32;
+        uint32_t boxed = 0, turn = 0;       // ring slots that boxes went to, and the parity of their last turn
         Job J;
         for (int item = blockIdx.x; !*s_abort && find_job(P, item, J); item += gridDim.x) {
         if (J.steps == 0) continue;
@@ -507,6 +511,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
             if (P.tma && (seen0 & seen1) == FULL && step * STEP >= J.first) {
                 if (lane == 0) mbar_expect_tx(&full[slot], Ly::KB);
                 __syncwarp();
+                boxed |= 1u << slot;
+                turn = (turn & ~(1u << slot)) | ((uint32_t)((stage / SLOTS) & 1) << slot);
                 // a lane a box: rows from the lane's own on, a panel of 64 dimensions
                 const CUtensorMap* map = is_v ? &tmv : &tmk;
                 if ((lane & (P.tma - 1)) == 0) {
@@ -545,6 +551,11 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         stage0 += J.steps + 2;
         ++jobs;
         }
+        // boxes that nobody waits for any more must not outlive the CTA
+        if (*s_abort)
+            for (int k = 0; k < SLOTS; ++k)
+                if ((boxed >> k) & 1u) await(&full[k], (turn >> k) & 1u, 1ll << 24);
+        __syncwarp();
         // tokens of no sequence, before the first or after the last, see nothing
         const int64_t s0 = clamp_start(P.starts, 0, P.tokens), s1 = max(s0, clamp_start(P.starts, P.c.seqs, P.tokens));
         for (int64_t i = (int64_t)blockIdx.x * PRODUCERS + w; i < s0 + P.tokens - s1; i += (int64_t)gridDim.x * PRODUCERS) {
@@ -610,6 +621,12 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
         done[0] += sp[0].z - sp[0].a;
         done[1] += sp[1].z - sp[1].a;
         }
+        // nor must products, which read its shared memory, nor their commits
+        if (elect_one()) {
+            umma_commit(endbar);
+            if (!await(endbar, 0)) *s_abort = 1;
+        }
+        __syncwarp();
     } else {
         // ---------------- softmax: a thread is a row
         const int t = warp / SOFTMAX, r = threadIdx.x & (TILE - 1);
