@@ -383,11 +383,16 @@ SWB_API uint64_t swb_attn_decode_workspace(const swb_kv_cache* cache, int q_head
  * slots j <= i with window == 0, j > i - window or j < sinks.  What sees nothing,
  * a token of no sequence among it, gives 0 and -inf.
  * q [tokens, q_heads, head_dim]; out and lse contiguous, out on a 16-byte boundary.
- *   status   optional int32 device word: SWB_ERR_TIMEOUT where a bounded device-side
- *            wait gave up (the rows concerned are NaN) */
+ *   status   int32 word that the device can write: SWB_ERR_TIMEOUT where a bounded
+ *            device-side wait gave up (the rows concerned are NaN).  NULL: a word of the
+ *            process's own, which the next of the calls above and below that finds it
+ *            set returns, once, in place of doing its work */
 SWB_API int swb_attn_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_heads,
                      const int32_t* starts, int64_t tokens, const swb_kv_cache* cache, float scale,
                      int window, int sinks, void* out, float* lse, int32_t* status, void* stream);
+
+/* That word, in host memory; NULL before the first prefill that needs it. */
+SWB_API int32_t* swb_attn_status(void);
 
 /* Cuts every sequence to `budget` slots.  Per key head the slots stay whose
  * position is below `sinks` or among the `recent` newest of the seen[b] given

@@ -75,6 +75,7 @@ SIGNATURES = {
                                _vp, _u64, _vp]),
     "swb_attn_decode_workspace": (_u64, [_kv, _i32, _i32]),
     "swb_attn_prefill": (_i32, [_vp, _i64, _i64, _i32, _vp, _i64, _kv, _f32, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "swb_attn_status": (_vp, []),
     "swb_kv_evict": (_i32, [_kv, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _u64, _vp]),
     "swb_kv_evict_workspace": (_u64, [_i32, _i32, _i32]),
     "swb_last_error": (C.c_char_p, []),

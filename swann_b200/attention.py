@@ -23,7 +23,9 @@ nothing.  With pages of one row the table lists rows: the ids that
 
 `KVCache` keeps the pieces together for the ordinary case.  Nothing here reads
 a device value on the host: the calls queue on the current stream and can be
-captured in a CUDA graph.  There is no backward pass: the package serves
+captured in a CUDA graph.  `prefill` waits inside its kernel, with a limit of
+seconds; should a wait give up, its rows are NaN and the next call here that is
+made after that raises SwannError.  There is no backward pass: the package serves
 models, it does not train them, and refuses tensors that want a gradient.
 """
 from __future__ import annotations

@@ -964,6 +964,8 @@ extern "C" int swb_attn_decode(const void* q, int64_t q_seq_stride, int64_t q_he
         return abi::fail(SWB_ERR_ARG, "out and the prior rows must start on 8-byte boundaries");
     if (sp.total && reinterpret_cast<uintptr_t>(workspace) % 16)
         return abi::fail(SWB_ERR_ARG, "the workspace must start on a 16-byte boundary");
+    rc = earlier_wait();
+    if (rc) return rc;
     cudaStream_t st = (cudaStream_t)stream;
     char* ws = static_cast<char*>(workspace);
     w.q = q;

@@ -185,6 +185,40 @@ inline cudaError_t allow_smem(const void* kernel, int bytes, std::atomic<uint64_
     return e;
 }
 
+// Where a prefill whose caller gives no status word says that a wait gave up: a word of
+// host memory that the device writes, one for the process, made by its first prefill.
+// Every call looks at it (nothing waits for that) and reports what it finds once, as
+// the errors of earlier launches are reported.
+inline std::atomic<int32_t*>& wait_word() {
+    static std::atomic<int32_t*> word{nullptr};
+    return word;
+}
+inline int32_t* make_wait_word() {
+    int32_t* w = wait_word().load(std::memory_order_acquire);
+    if (w) return w;
+    // a stream may be capturing: this touches none
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+    void* p = nullptr;
+    const cudaError_t e = cudaHostAlloc(&p, sizeof(int32_t), cudaHostAllocPortable | cudaHostAllocMapped);
+    if (e != cudaSuccess) cudaGetLastError();
+    else *static_cast<volatile int32_t*>(p) = 0;
+    int32_t* mine = e == cudaSuccess ? static_cast<int32_t*>(p) : nullptr;
+    if (mine && !wait_word().compare_exchange_strong(w, mine, std::memory_order_acq_rel)) {
+        cudaFreeHost(mine);
+        mine = w;
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    return mine;
+}
+inline int earlier_wait() {
+    volatile int32_t* w = wait_word().load(std::memory_order_acquire);
+    const int code = w ? *w : 0;
+    if (!code) return SWB_OK;
+    *w = 0;
+    return abi::fail(code, "an earlier prefill failed: a device-side wait gave up, and rows of its are NaN");
+}
+
 // Launches a kernel that may begin while the one before it in the stream ends:
 // the kernel itself waits (dependency_wait) before it reads what that wrote.
 template <typename... P, typename... A>

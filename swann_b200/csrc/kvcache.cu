@@ -465,7 +465,7 @@ extern "C" int swb_rope_append(const void* q, int64_t q_token_stride, int64_t q_
                                const int32_t* positions, const swb_kv_cache* cache, void* out,
                                int32_t* slot_positions, int64_t slot_width, void* stream) {
     Append a = {};
-    const int rc = check_cache(cache, &a.c);
+    int rc = check_cache(cache, &a.c);
     if (rc) return rc;
     if (tokens <= 0) return SWB_OK;
     if (!q || !k || !v || !starts || !out) return abi::fail(SWB_ERR_ARG, "null buffer");
@@ -481,6 +481,8 @@ extern "C" int swb_rope_append(const void* q, int64_t q_token_stride, int64_t q_
     for (int i = 0; i < 6; ++i)
         if (reinterpret_cast<uintptr_t>(at[i]) % 16 || strides[i] % 8)
             return abi::fail(SWB_ERR_ARG, "rows must start on 16-byte boundaries");
+    rc = earlier_wait();
+    if (rc) return rc;
     a.q = q;
     a.k = k;
     a.v = v;
@@ -521,7 +523,7 @@ extern "C" int swb_kv_evict(const swb_kv_cache* cache, const int32_t* seen, cons
                             int32_t* new_lengths, float* new_weights, int32_t* new_positions, void* workspace,
                             uint64_t ws_bytes, void* stream) {
     Evict e = {};
-    const int rc = check_cache(cache, &e.c);
+    int rc = check_cache(cache, &e.c);
     if (rc) return rc;
     if (budget < 1 || sinks < 0 || recent < 0) return abi::fail(SWB_ERR_ARG, "budget, sinks or recent out of range");
     if ((int64_t)sinks + recent > budget) return abi::fail(SWB_ERR_ARG, "sinks and recent do not fit the budget");
@@ -535,6 +537,8 @@ extern "C" int swb_kv_evict(const swb_kv_cache* cache, const int32_t* seen, cons
         return abi::fail(SWB_ERR_ARG, "workspace too small");
     const int64_t heads = (int64_t)e.c.seqs * e.c.kv_heads;
     if (heads >= ((int64_t)1 << 31)) return abi::fail(SWB_ERR_ARG, "too many sequences in one call");
+    rc = earlier_wait();
+    if (rc) return rc;
     e.budget = budget;
     e.sinks = sinks;
     e.recent = recent;
@@ -558,8 +562,8 @@ extern "C" int swb_kv_evict(const swb_kv_cache* cache, const int32_t* seen, cons
     if (err != cudaSuccess) return abi::cuda_fail(err, "cudaFuncSetAttribute(evict)");
     if (few) select_kernel<8><<<(unsigned)heads, SELECT_THREADS, smem, st>>>(e);
     else select_kernel<16><<<(unsigned)heads, SELECT_THREADS, smem, st>>>(e);
-    const int rc2 = abi::cuda_check("evict launch");
-    if (rc2) return rc2;
+    rc = abi::cuda_check("evict launch");
+    if (rc) return rc;
     // at most min(budget, slots beyond it) rows of a head move, and slots beyond the
     // budget or the shortest length hold nothing
     const int64_t beyond = e.c.capacity() - budget;

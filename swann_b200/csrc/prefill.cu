@@ -794,7 +794,8 @@ __global__ void __launch_bounds__(THREADS, 1) prefill_kernel(const __grid_consta
     }
     tc_fence_before();
     __syncthreads();
-    if (*s_abort && threadIdx.x == 0 && P.status) atomicExch(P.status, *s_abort == 2 ? SWB_ERR_SMEM : ERR_TIMEOUT);
+    if (*s_abort && threadIdx.x == 0 && P.status)
+        *static_cast<volatile int32_t*>(P.status) = *s_abort == 2 ? SWB_ERR_SMEM : ERR_TIMEOUT;
     if (warp == MMA_WARP) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
@@ -847,6 +848,8 @@ int launch(Prefill p, int64_t items, cudaStream_t st) {
 using namespace swb;
 using namespace swb::attn;
 
+extern "C" int32_t* swb_attn_status(void) { return wait_word().load(std::memory_order_acquire); }
+
 extern "C" int swb_attn_prefill(const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_heads,
                                 const int32_t* starts, int64_t tokens, const swb_kv_cache* cache, float scale,
                                 int window, int sinks, void* out, float* lse, int32_t* status, void* stream) {
@@ -876,7 +879,9 @@ extern "C" int swb_attn_prefill(const void* q, int64_t q_token_stride, int64_t q
     p.sinks = sinks;
     p.out = out;
     p.lse = lse;
-    p.status = status;
+    rc = earlier_wait();
+    if (rc) return rc;
+    p.status = status ? status : make_wait_word();
     // every sequence may end in a tile that is not full
     const int64_t step = 2 * p.tile_tokens;
     const int64_t items = ((tokens + step - 1) / step + p.c.seqs) * p.c.kv_heads * p.head_tiles;

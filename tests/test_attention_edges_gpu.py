@@ -1,5 +1,9 @@
 """The attention operators at the edges of what their calls allow, against their definitions in 64 bits."""
+import ctypes as C
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import test_attention_gpu as base
@@ -272,3 +276,38 @@ def test_prefill_without_sequences():
     k, v, table, L = make_cache([8], 1, 64, 16, torch.float16, 24)
     out, lse = prefill_into(torch.randn((5, 2, 64), device=DEV).half(), k, v, table[:0], ints(0), L[:0], torch.float16)
     assert (out == 0).all() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("call", ["rope_append", "decode", "prefill", "evict"])
+def test_a_wait_that_gave_up_is_reported_by_the_next_call(call):
+    """The word that the kernel writes then, written by the host."""
+    tensors, calls = every_call()
+    calls["prefill"](tensors)
+    torch.cuda.synchronize()
+    word = C.c_int32.from_address(N.lib().swb_attn_status())
+    assert word.value == 0
+    word.value = N.ERR_TIMEOUT
+    with pytest.raises(N.SwannError, match="gave up") as e:
+        calls[call](tensors)
+    assert e.value.code == N.ERR_TIMEOUT and word.value == 0
+    calls[call](tensors)
+
+
+def test_a_first_prefill_under_capture():
+    """The word is made while a stream is capturing, in a process of its own."""
+    code = """
+import torch
+from swann_b200 import _lib as N, attention as A
+k = torch.randn((4, 1, 16, 64), device="cuda").half()
+table, L = torch.arange(4, dtype=torch.int32, device="cuda").view(1, 4), torch.full((1,), 60, dtype=torch.int32, device="cuda")
+q, starts = torch.randn((20, 2, 64), device="cuda").half(), torch.tensor([0, 20], dtype=torch.int32, device="cuda")
+assert not N.lib().swb_attn_status()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out, lse = A.prefill(q, k, k, table, starts, L)
+assert N.lib().swb_attn_status()
+graph.replay()
+want = A.prefill(q, k, k, table, starts, L)
+assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=Path(__file__).resolve().parent.parent, timeout=300)
