@@ -293,7 +293,12 @@ class KVCache:
     has had in `attend` so far (float32 and int32 [seqs, kv_heads, slots]).
     The pools and the table are plain tensors (k, v, table, lengths, seen) and may be
     handed to this module's functions; `lengths` and `seen` are on the device,
-    and nothing here waits for them: tokens past the last slot are not stored."""
+    and nothing here waits for them: tokens past the last slot are not stored.
+    All of them are the same tensors for the cache's life, written in place (clone
+    what is to be kept), so a captured step goes on from where the last replay
+    ended.  What a captured step cannot know is an eviction outside of it: its
+    `window`, which the slots' order then no longer allows, is refused at the
+    capture or not at all."""
 
     def __init__(self, seqs, slots, kv_heads, head_dim, *, page_size=64, dtype=torch.float16, device="cuda",
                  track=False):
@@ -330,16 +335,20 @@ class KVCache:
             starts = self._each
         _ints("append", "starts", starts, (seqs + 1,), self.k.get_device())
         counts = starts.diff()
-        lengths, seen = self.lengths + counts, self.seen + counts
+        lengths = self.lengths + counts
         positions = None
-        if self._evicted and n and seqs:            # slots are no longer positions
-            at = torch.arange(n, dtype=torch.int32, device=starts.device)
-            # a token's sequence: whatever starts holds, one that there is
-            of = torch.searchsorted(starts[1:], at, right=True).clamp_(max=seqs - 1)
-            positions = at + (self.seen - starts[:-1])[of]
+        if self.weights is not None and n and seqs:     # after an eviction slots are not positions
+            if starts is self._each:
+                positions = self.seen
+            elif self._evicted or torch.cuda.is_current_stream_capturing():
+                at = torch.arange(n, dtype=torch.int32, device=starts.device)
+                # a token's sequence: whatever starts holds, one that there is
+                of = torch.searchsorted(starts[1:], at, right=True).clamp_(max=seqs - 1)
+                positions = at + (self.seen - starts[:-1])[of]
         out = rope_append(q, k, v, cos, sin, self.k, self.v, self.table, starts, lengths, q_norm=q_norm, k_norm=k_norm,
                           eps=eps, positions=positions, interleaved=interleaved, slot_positions=self.positions)
-        self.lengths, self.seen = lengths, seen
+        self.lengths.copy_(lengths)
+        self.seen.add_(counts)
         return out
 
     def prefill(self, q, starts, *, scale=None, window=0, sinks=0):
@@ -359,7 +368,8 @@ class KVCache:
         """Every sequence cut to `budget` slots: its first `sinks` and newest `recent` positions, then by weight."""
         if self.weights is None:
             _fail("evict", "the cache was made without track=True")
-        self.lengths, self.weights, self.positions = evict(
-            self.k, self.v, self.table, self.lengths, self.weights, self.positions, budget, seen=self.seen, sinks=sinks,
-            recent=recent)
+        new = evict(self.k, self.v, self.table, self.lengths, self.weights, self.positions, budget, seen=self.seen,
+                    sinks=sinks, recent=recent)
+        for mine, its in zip((self.lengths, self.weights, self.positions), new):
+            mine.copy_(its)
         self._evicted = True

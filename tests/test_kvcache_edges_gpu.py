@@ -56,3 +56,59 @@ def test_append_of_a_padded_batch(evicted):
     assert (caches[0].positions[2, :, held[2]:held[2] + 5] == ints(6, 7, 8, 9, 10)).all()
     assert (caches[0].positions[0, :, held[0]:held[0] + 2] == ints(3, 4)).all()
     assert (caches[0].positions[2, :, held[2] + 5:] == -1).all()
+
+
+@pytest.mark.parametrize("budget", [None, 8])
+@pytest.mark.parametrize("prompt", [1, 20])
+def test_a_captured_step_goes_on_by_itself(budget, prompt):
+    """append, attend and evict captured before the first eviction and replayed: as the same calls one by one."""
+    cos, sin = turns(128)
+    caches = [swann.KVCache(3, 96, 2, 64, page_size=16, track=True) for _ in range(2)]
+    starts = ints(0, prompt, prompt + 1, 2 * prompt + 1)
+    q, k, v = qkv(3 + 2 * prompt + 1)
+    x = torch.empty((3, 8, 64), device=DEV).half()
+    for c in caches:
+        c.append(q[:2 * prompt + 1], k[:2 * prompt + 1], v[:2 * prompt + 1], cos, sin, starts)
+
+    def step(c):
+        got = c.attend(c.append(x[:, :4], x[:, 4:6], x[:, 6:], cos, sin))
+        if budget:
+            c.evict(budget, sinks=1, recent=2)
+        return got
+
+    held = {name: getattr(caches[0], name) for name in ("lengths", "seen", "weights", "positions", "k", "v", "table")}
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(caches[0])
+    assert all(getattr(caches[0], name) is t for name, t in held.items())
+    for i in range(12):
+        x.copy_(torch.randn((3, 8, 64), generator=torch.Generator(device=DEV).manual_seed(i), device=DEV))
+        graph.replay()
+        want = step(caches[1])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), i
+        for name in held:
+            assert torch.equal(getattr(caches[0], name), getattr(caches[1], name)), (i, name)
+    assert caches[0].seen.tolist() == [prompt + 12, 13, prompt + 12]
+    if budget:
+        assert caches[0].lengths.tolist() == [8] * 3
+
+
+def test_a_captured_prompt_after_an_eviction():
+    """Several tokens a sequence, captured before the cache is evicted: their positions come from `seen`."""
+    cos, sin = turns(128)
+    caches = [swann.KVCache(2, 96, 2, 64, page_size=16, track=True) for _ in range(2)]
+    starts = ints(0, 5, 7)
+    x = qkv(7)
+    for c in caches:
+        c.append(*x, cos, sin, starts)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = caches[0].append(*x, cos, sin, starts)
+    for _ in range(3):
+        for c in caches:
+            c.evict(4, recent=2)
+        graph.replay()
+        want = caches[1].append(*x, cos, sin, starts)
+        assert torch.equal(got, want)
+        for name in ("lengths", "seen", "positions", "k", "v"):
+            assert torch.equal(getattr(caches[0], name), getattr(caches[1], name)), name
