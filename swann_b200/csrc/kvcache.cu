@@ -537,6 +537,13 @@ extern "C" int swb_kv_evict(const swb_kv_cache* cache, const int32_t* seen, cons
         return abi::fail(SWB_ERR_ARG, "workspace too small");
     const int64_t heads = (int64_t)e.c.seqs * e.c.kv_heads;
     if (heads >= ((int64_t)1 << 31)) return abi::fail(SWB_ERR_ARG, "too many sequences in one call");
+    // at most min(budget, slots beyond it) rows of a head move, and slots beyond the
+    // budget or the shortest length hold nothing
+    const int64_t beyond = e.c.capacity() - budget;
+    const int64_t most = beyond < budget ? (beyond > 0 ? beyond : 0) : budget;
+    const int64_t rows = (most + MOVE_ROWS - 1) / MOVE_ROWS, slots = (width + MOVE_SLOTS - 1) / MOVE_SLOTS;
+    const int64_t by = rows > slots ? rows : slots;
+    if (by > 65535) return abi::fail(SWB_ERR_ARG, "budget or weights too wide");
     rc = earlier_wait();
     if (rc) return rc;
     e.budget = budget;
@@ -564,14 +571,7 @@ extern "C" int swb_kv_evict(const swb_kv_cache* cache, const int32_t* seen, cons
     else select_kernel<16><<<(unsigned)heads, SELECT_THREADS, smem, st>>>(e);
     rc = abi::cuda_check("evict launch");
     if (rc) return rc;
-    // at most min(budget, slots beyond it) rows of a head move, and slots beyond the
-    // budget or the shortest length hold nothing
-    const int64_t beyond = e.c.capacity() - budget;
-    const int64_t most = beyond < budget ? (beyond > 0 ? beyond : 0) : budget;
-    const int64_t rows = (most + MOVE_ROWS - 1) / MOVE_ROWS, slots = (width + MOVE_SLOTS - 1) / MOVE_SLOTS;
-    const int64_t by = rows > slots ? rows : slots;
     if (by == 0) return SWB_OK;
-    if (by > 65535) return abi::fail(SWB_ERR_ARG, "budget too large");
     err = launch_after(move_kernel, dim3((unsigned)heads, (unsigned)by), dim3(MOVE_THREADS), 0, st, e);
     if (err != cudaSuccess) return abi::cuda_fail(err, "evict move launch");
     return abi::cuda_check("evict move launch");

@@ -11,3 +11,10 @@ from swann_b200 import _lib as N
 def test_decode_refuses_rows_and_workspaces_that_it_cannot_access(args, why):
     assert decode(cache(), **args) == N.ERR_ARG
     assert "boundar" in N.lib().swb_last_error().decode() and why in N.lib().swb_last_error().decode()
+
+
+@pytest.mark.parametrize("width,budget", [(65536 * 4096, 8), (1 << 40, 8), (1 << 23, 1 << 22)])
+def test_evict_refuses_what_its_second_kernel_cannot_take_before_the_first(width, budget):
+    arg = cache(max_pages=1 << 19)
+    assert N.lib().swb_kv_evict(arg, P, P, P, width, budget, 0, 0, P + 64, P + 64, P + 64, P, 1 << 40, None) == N.ERR_ARG
+    assert "wide" in N.lib().swb_last_error().decode()
