@@ -986,6 +986,7 @@ extern "C" int swb_attn_decode(const void* q, int64_t q_seq_stride, int64_t q_he
     w.part_out = reinterpret_cast<float*>(ws + sp.out);
     w.part_ml = reinterpret_cast<float2*>(ws + sp.ml);
     w.cuts = reinterpret_cast<int4*>(ws + sp.cuts);
+    if (weights_width == 0) weights = nullptr;      // of no slots: nothing to write
     w.lse2 = weights ? reinterpret_cast<float*>(ws + sp.lse2) : nullptr;
     w.logits = weights ? reinterpret_cast<float*>(ws + sp.logits) : nullptr;
     const int64_t pairs = (int64_t)c.seqs * c.kv_heads * w.head_tiles;

@@ -311,3 +311,18 @@ want = A.prefill(q, k, k, table, starts, L)
 assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
 """
     subprocess.run([sys.executable, "-c", code], check=True, cwd=Path(__file__).resolve().parent.parent, timeout=300)
+
+
+@pytest.mark.parametrize("B", [1, 2, 700])
+def test_decode_with_weights_of_no_slots(B):
+    """A table without columns: the native call with weights of width 0."""
+    table, L = torch.zeros((B, 0), dtype=torch.int32, device=DEV), torch.full((B,), 3, dtype=torch.int32, device=DEV)
+    k = torch.zeros((2, 1, 16, 64), dtype=torch.float16, device=DEV)
+    q = torch.ones((B, 4, 64), dtype=torch.float16, device=DEV)
+    out, lse, w = torch.full_like(q, 7), torch.zeros((B, 4), device=DEV), torch.full((4,), 7.0, device=DEV)
+    arg, _ = A._cache_arg("decode", k, k, table, L)
+    need = N.lib().swb_attn_decode_workspace(arg, 4, 1)
+    ws = torch.empty(need, dtype=torch.uint8, device=DEV)
+    N.check(N.lib().swb_attn_decode(q.data_ptr(), 256, 64, 4, arg, 0.1, 0, 0, None, None, out.data_ptr(), lse.data_ptr(),
+                                    w.data_ptr(), 0, 0, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream))
+    assert (out == 0).all() and (lse == -math.inf).all() and (w == 7).all()
