@@ -83,6 +83,8 @@ def _cache_arg(what, k, v, table, lengths):
     _no_gradient(what, "the cache", v)
     pages, heads, page, d = shape
     ps, hs, rs, es = strides
+    if heads < 1:
+        _fail(what, "the cache must have a key head")
     if d not in HEAD_DIMS:
         _fail(what, f"head_dim must be one of {HEAD_DIMS}")
     if es != 1:

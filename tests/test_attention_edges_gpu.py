@@ -326,3 +326,11 @@ def test_decode_with_weights_of_no_slots(B):
     N.check(N.lib().swb_attn_decode(q.data_ptr(), 256, 64, 4, arg, 0.1, 0, 0, None, None, out.data_ptr(), lse.data_ptr(),
                                     w.data_ptr(), 0, 0, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream))
     assert (out == 0).all() and (lse == -math.inf).all() and (w == 7).all()
+
+
+@pytest.mark.parametrize("call", ["rope_append", "decode", "prefill", "evict"])
+def test_a_cache_without_key_heads_is_refused(call):
+    tensors, calls = every_call()
+    none = {**tensors, "k": tensors["k"][:, :0], "v": tensors["v"][:, :0]}
+    with pytest.raises(ValueError, match="key head"):
+        calls[call](none)
