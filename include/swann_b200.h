@@ -399,7 +399,10 @@ SWB_API int32_t* swb_attn_status(void);
  * out, then those with the largest weight, ties to the lowest slot (NaN below
  * every number).  Kept slots below the budget stay in place; kept ones beyond
  * it go, in order, to the free slots below it, in order.  Rows move in the
- * pools; lengths, weights and positions [seqs, kv_heads, width] are written to
+ * pools, so every slot below the length needs a page, and no page may be named
+ * twice: a page that tables share (which the other calls read as it is) would
+ * change under the other sequence, and a row that moves to a slot without a page
+ * is lost.  lengths, weights and positions [seqs, kv_heads, width] are written to
  * new buffers (0 and -1 in slots that hold nothing).
  *   workspace: at least swb_kv_evict_workspace(...) bytes */
 SWB_API int swb_kv_evict(const swb_kv_cache* cache, const int32_t* seen, const float* weights,

@@ -259,7 +259,9 @@ def evict(k_cache, v_cache, table, lengths, weights, positions, budget, *, seen,
     largest weight, ties to the lowest slot.  Kept slots below the budget stay
     in place, kept ones beyond it move, in order, to the free slots below it,
     in order: the order of slots is then no longer the order of positions.
-    Rows move inside the pools; returns the new (lengths, weights, positions)
+    Rows move inside the pools: every slot that a sequence holds must have a page,
+    and no page may be in the table twice (`decode` and `prefill` read pages that
+    sequences share; here one's rows would move under the other).  Returns the new (lengths, weights, positions)
     as tensors of their own, 0 and -1 in slots that hold nothing."""
     what = "evict"
     arg, dev = _cache_arg(what, k_cache, v_cache, table, lengths)
@@ -292,7 +294,9 @@ class KVCache:
         out, lse = cache.attend(q, window=4096, sinks=4)
 
     `track` keeps what eviction goes by: every slot's position and the weight it
-    has had in `attend` so far (float32 and int32 [seqs, kv_heads, slots]).
+    has had in `attend` so far (int32 and float32 [seqs, kv_heads, slots]).  An
+    `attend` that tracks holds its logits meanwhile: float32 for every query head
+    and slot of the table, whatever the lengths are.
     The pools and the table are plain tensors (k, v, table, lengths, seen) and may be
     handed to this module's functions; `lengths` and `seen` are on the device,
     and nothing here waits for them: tokens past the last slot are not stored.
@@ -367,7 +371,11 @@ class KVCache:
                       weights=self.weights, accumulate=True)
 
     def evict(self, budget, *, sinks=0, recent=0):
-        """Every sequence cut to `budget` slots: its first `sinks` and newest `recent` positions, then by weight."""
+        """Every sequence cut to `budget` slots: its first `sinks` and newest `recent` positions, then by weight.
+
+        Weight comes from `attend` alone.  Slots that no token has attended yet, a prompt's before the first, have
+        none, and among equal weights the lowest slots stay: cut a prompt after some tokens have attended it, or
+        write weights of your own into `weights`."""
         if self.weights is None:
             _fail("evict", "the cache was made without track=True")
         new = evict(self.k, self.v, self.table, self.lengths, self.weights, self.positions, budget, seen=self.seen,
