@@ -334,3 +334,59 @@ def test_a_cache_without_key_heads_is_refused(call):
     none = {**tensors, "k": tensors["k"][:, :0], "v": tensors["v"][:, :0]}
     with pytest.raises(ValueError, match="key head"):
         calls[call](none)
+
+
+@pytest.mark.parametrize("lengths,hq,hkv,window,sinks", [
+    ([3000, 70, 0], 8, 2, 200, 5), ([3000, 70, 1], 40, 2, 0, 0), ([300] * 5, 36, 1, 64, 0), ([(37 * b) % 91 for b in range(700)], 12, 1, 21, 3),
+    ([(37 * b) % 91 for b in range(700)], 1, 1, 21, 3)])
+def test_decode_accumulates_beside_a_window_and_many_heads(lengths, hq, hkv, window, sinks):
+    """What is added is what a call that writes gives: one fp32 addition, 2^-24 of the sum; unseen slots stay as they are."""
+    k, v, table, L = make_cache(lengths, hkv, 64, 16, torch.float16, 5)
+    q = torch.randn((len(lengths), hq, 64), device=DEV).half()
+    once = torch.full((len(lengths), hkv, table.shape[1] * 16 + 3), math.nan, device=DEV)
+    w = torch.rand(once.shape, device=DEV)
+    w0 = w.clone()
+    a = A.decode(q, k, v, table, L, window=window, sinks=sinks, weights=once)
+    b = A.decode(q, k, v, table, L, window=window, sinks=sinks, weights=w, accumulate=True)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    j, n = torch.arange(once.shape[2], device=DEV), L.long()[:, None]
+    seen = (j < n) & ((j >= n - window) | (j < sinks) if window else j >= 0)
+    assert (once.masked_select(~seen[:, None]) == 0).all()
+    assert torch.equal(w.masked_select(~seen[:, None].expand_as(w)), w0.masked_select(~seen[:, None].expand_as(w)))
+    want = w0.double() + once.double()
+    assert ((w.double() - want).abs() <= 2.0 ** -24 * want).all()
+    total = hq // hkv * (n > 0).double()
+    assert torch.allclose(once.double().sum(-1), total.expand(-1, hkv), rtol=1e-4, atol=0)
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype,window,sinks", [(130, 1, 64, torch.float16, 0, 0), (129, 1, 128, torch.bfloat16, 40, 2),
+                                                         (400, 2, 64, torch.bfloat16, 0, 0), (256, 1, 128, torch.float16, 9, 0)])
+def test_prefill_of_more_heads_to_a_key_head_than_a_tile_has_rows(hq, hkv, d, dtype, window, sinks):
+    new, held = [3, 0, 70], [0, 9, 130]
+    lengths = [a + b for a, b in zip(new, held)]
+    k, v, table, L = make_cache(lengths, hkv, d, 16, dtype, 17)
+    q = (torch.randn((73, hq, d), device=DEV) * 1.5).to(dtype)
+    out, lse = A.prefill(q, k, v, table, ints(0, 3, 3, 73), L, window=window, sinks=sinks)
+    G = hq // hkv
+    for b, t in ((0, 0), (0, 2), (2, 0), (2, 1), (2, 33), (2, 69)):
+        row = t + (3 if b else 0)
+        for h in {0, 1, 127, 128, hq - 1, hq // 2}:
+            want = base.attend(q[row, h], k, v, table, b, h // G, held[b] + t, d ** -0.5, window, sinks, lengths[b])
+            base.check_row(out[row, h], lse[row, h], want, base.U[dtype])
+    assert torch.isfinite(out).all()
+
+
+def test_pages_that_sequences_share_are_read_as_they_are():
+    """A common beginning: the first pages of three sequences are the same."""
+    k, v, table, L = make_cache([100, 90, 64], 2, 64, 16, torch.float16, 18)
+    table[1, :4] = table[2, :4] = table[0, :4]
+    q = torch.randn((33, 4, 64), device=DEV).half()
+    starts = [0, 10, 30, 33]
+    out, lse = A.prefill(q, k, v, table, ints(*starts), L)
+    one, one_lse = A.decode(q[:3], k, v, table, L)
+    for b, n in enumerate([100, 90, 64]):
+        for h in range(4):
+            base.check_row(one[b, h], one_lse[b, h], base.attend(q[b, h], k, v, table, b, h // 2, n - 1, 0.125, 0, 0, n), base.U[torch.float16])
+            for t in (starts[b], starts[b + 1] - 1):
+                want = base.attend(q[t, h], k, v, table, b, h // 2, n - starts[b + 1] + t, 0.125, 0, 0, n)
+                base.check_row(out[t, h], lse[t, h], want, base.U[torch.float16])
