@@ -86,9 +86,8 @@ __global__ void __launch_bounds__(APPEND_THREADS, APPEND_CTAS) append_kernel(con
     const int c0 = halves ? idx : 2 * idx, c1 = halves ? idx + hc : 2 * idx + 1;
     const bool turned = idx < hc;
 
-    int b = 0;
-    bool ours = false;
-    int64_t slot = 0, pos = 0, row = 0;
+    int b = 0, slot = 0, pos = 0;
+    int64_t row = 0;
     float co[8], si[8];
     for (int hb = threadIdx.x / LPH; hb - (int)threadIdx.x / LPH < heads; hb += HP * U) {
         uint4 raw[U][2];
@@ -114,17 +113,18 @@ __global__ void __launch_bounds__(APPEND_THREADS, APPEND_CTAS) append_kernel(con
                 else hi = mid;
             }
             slot = -1;
+            bool ours = false;
             if (P.c.seqs > 0) {
-                const int from = P.starts[b], to = P.starts[b + 1];
-                ours = from <= tok && tok < to;
-                if (ours) slot = (int64_t)P.c.lengths[b] - (to - tok);
+                const int to = P.starts[b + 1];
+                ours = P.starts[b] <= tok && tok < to;
+                if (ours) slot = max(P.c.lengths[b], 0) - (to - (int)tok);
             }
-            pos = P.positions ? (int64_t)P.positions[tok] : slot;
-            row = slot >= 0 && slot < P.c.capacity() ? P.c.row(b, (int)slot) : -1;
+            pos = P.positions ? P.positions[tok] : slot;
+            row = slot >= 0 && slot < P.c.capacity() ? P.c.row(b, slot) : -1;
             if (turned) {
                 if (pos >= 0 && pos < P.table_rows) {
-                    const float4* pc = reinterpret_cast<const float4*>(P.cos + pos * P.half + idx * 8);
-                    const float4* ps = reinterpret_cast<const float4*>(P.sin + pos * P.half + idx * 8);
+                    const float4* pc = reinterpret_cast<const float4*>(P.cos + (int64_t)pos * P.half + idx * 8);
+                    const float4* ps = reinterpret_cast<const float4*>(P.sin + (int64_t)pos * P.half + idx * 8);
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         *reinterpret_cast<float4*>(co + 4 * e) = pc[e];
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, APPEND_CTAS) append_kernel(con
                 const int kh = is_v ? h - values : h - keys;
                 dst = static_cast<T*>(const_cast<void*>(is_v ? P.c.v : P.c.k)) + row + kh * P.c.head_stride;
                 if (P.slot_positions && !is_v && idx == 0 && slot < P.width)
-                    P.slot_positions[((int64_t)b * P.c.kv_heads + kh) * P.width + slot] = (int32_t)pos;
+                    P.slot_positions[((int64_t)b * P.c.kv_heads + kh) * P.width + slot] = pos;
             }
             *reinterpret_cast<uint4*>(dst + c0 * 8) = raw[i][0];
             *reinterpret_cast<uint4*>(dst + c1 * 8) = raw[i][1];
