@@ -222,7 +222,9 @@ struct Evict {
     int row_chunks;               // 16-byte chunks of a row
 
     // slots of sequence b that there are: of the table and of a row of weights
-    __device__ __forceinline__ int held(int b) const { return (int)min((int64_t)c.length(b), width); }
+    __device__ __forceinline__ int held(int b) const {
+        return (int)max((int64_t)0, min((int64_t)c.lengths[b], min(c.capacity(), width)));
+    }
 };
 
 constexpr int SELECT_THREADS = 1024;
