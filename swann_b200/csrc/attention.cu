@@ -861,12 +861,20 @@ __global__ void __launch_bounds__(JOIN_THREADS) finish_kernel(const __grid_const
 
 // -- host side --------------------------------------------------------------
 
-// Whether a warp takes a whole pair.  With short tables (search results) a run of a
-// CTA would be many short pairs, each joined by its warps.  With long ones it needs
-// enough pairs that the last round of unequal lengths is short.
-inline bool whole_pairs(const Cache& c, int64_t pairs) {
-    const int64_t warps = 8ll * abi::num_sms();
-    return c.capacity() <= 512 ? pairs >= warps / 2 : pairs >= 16 * warps;
+// Whether a warp takes a whole pair.  Where pairs are many and short (search results) a
+// run of a CTA would be many of them, each joined by its warps; where they are few or
+// long, a warp a pair leaves SMs idle, more so with one query row, whose kernel loads
+// little at a time.  Lengths uniform up to the table's slots, fp16, head_dim 128, us by
+// runs / by whole pairs:
+//   one row    512 slots: 592 pairs 26 / 94, 4096 140 / 118;  128 slots: 1184 23 / 22, 4096 82 / 34
+//              2048 slots: 18944 pairs 1661 / 1790
+//   four rows  512 slots: 148 pairs 11 / 23, 1184 39 / 34;  2048 slots: 592 52 / 100, 18944 1310 / 1243
+// The two meet where pairs are about twice the slots (2 to 16 rows, head_dim 64 and 128,
+// 64 to 4096 slots), with one row about eight times and beyond 1024 slots nowhere.
+inline bool whole_pairs(const Cache& c, int group, int64_t pairs) {
+    const int64_t sms = abi::num_sms(), slots = c.capacity();
+    if (group == 1) return slots <= 1024 && pairs >= 4 * sms && pairs >= 8 * slots;
+    return pairs >= sms && pairs >= 2 * slots;
 }
 
 template <typename T, int D, int NT>
@@ -914,7 +922,7 @@ inline int tiles_of(int group) { return (group + ROWS - 1) / ROWS; }
 inline Space decode_space(const Cache& c, int d, int q_heads, bool weights) {
     Space s;
     const int64_t pairs = (int64_t)c.seqs * c.kv_heads * tiles_of(q_heads / c.kv_heads);
-    s.runs = whole_pairs(c, pairs) ? 0 : cta_per_sm(d) * abi::num_sms();
+    s.runs = whole_pairs(c, q_heads / c.kv_heads, pairs) ? 0 : cta_per_sm(d) * abi::num_sms();
     // no more runs than there can be units
     const int64_t most = pairs * ((c.capacity() + UNIT - 1) / UNIT + 1);
     if (s.runs > most) s.runs = (int)most;

@@ -165,8 +165,8 @@ def test_prefill_keeps_a_long_flat_tail(n, new, hq, hkv, d, window, dtype):
     (1, 3000, 8, 1, 128),       # runs of one unit
     (40, 3000, 16, 8, 64),      # runs longer than a pair
     (40, 3000, 160, 8, 64),     # and of two products' rows
-    (640, 400, 4, 1, 64),       # a warp a pair
-    (640, 400, 1, 1, 128)])     # of one row
+    (900, 400, 4, 1, 64),       # a warp a pair
+    (1000, 100, 1, 1, 128)])    # of one row
 def test_decode_keeps_a_long_flat_tail(B, n, hq, hkv, d, dtype):
     q, k, v, table, L = peaked([n] * B, hq, hkv, d, 16, dtype, B)
     prior = (torch.full((B, hq, d), 0.5, device=DEV).to(dtype), torch.full((B, hq), 0.0, device=DEV))
@@ -338,7 +338,7 @@ def test_a_cache_without_key_heads_is_refused(call):
 
 @pytest.mark.parametrize("lengths,hq,hkv,window,sinks", [
     ([3000, 70, 0], 8, 2, 200, 5), ([3000, 70, 1], 40, 2, 0, 0), ([300] * 5, 36, 1, 64, 0), ([(37 * b) % 91 for b in range(700)], 12, 1, 21, 3),
-    ([(37 * b) % 91 for b in range(700)], 1, 1, 21, 3)])
+    ([(37 * b) % 91 for b in range(900)], 1, 1, 21, 3)])
 def test_decode_accumulates_beside_a_window_and_many_heads(lengths, hq, hkv, window, sinks):
     """What is added is what a call that writes gives: one fp32 addition, 2^-24 of the sum; unseen slots stay as they are."""
     k, v, table, L = make_cache(lengths, hkv, 64, 16, torch.float16, 5)
@@ -390,3 +390,10 @@ def test_pages_that_sequences_share_are_read_as_they_are():
             for t in (starts[b], starts[b + 1] - 1):
                 want = base.attend(q[t, h], k, v, table, b, h // 2, n - starts[b + 1] + t, 0.125, 0, 0, n)
                 base.check_row(out[t, h], lse[t, h], want, base.U[torch.float16])
+
+
+@pytest.mark.parametrize("B,hq,hkv,d,page,dtype", [(900, 1, 1, 128, 1, torch.float16), (800, 1, 1, 64, 1, torch.bfloat16),
+                                                   (450, 2, 2, 64, 8, torch.float16)])
+@pytest.mark.parametrize("window,sinks,extra", [(0, 0, "prior"), (0, 0, "weights"), (21, 3, "plain")])
+def test_decode_of_enough_one_row_pairs_for_a_warp_each(B, hq, hkv, d, page, dtype, window, sinks, extra):
+    base.test_decode_of_very_many_short_sequences(B, hq, hkv, d, page, dtype, window, sinks, extra)
