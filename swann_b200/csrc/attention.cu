@@ -27,10 +27,10 @@
 // and every CTA of a grid that the SMs hold at once takes an equal run of them,
 // whatever the sequences' lengths are; a pair cut by the end of a run leaves
 // parts (m, l, unnormalised rows), at most two a CTA, which a second kernel
-// joins.  Very many pairs: a warp a pair.
+// joins.  Many short pairs: a warp a pair.
 //
 // Measured: 48 sequences of up to 8191 slots, 32 heads of 128 over 8: 95 us, 6.1 TB/s
-// (94% of a copy's rate); one of 131071 slots with 4 key heads and weights: 64 us, of
+// (94% of a copy's rate); one of 131071 slots with 4 key heads and weights: 62 us, of
 // which 46 walk; one of 1027: 7 us, launch and latency.
 
 #include "attn.cuh"
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(WARPS * 32, cta_per_sm(D)) walk_kernel(const _
     }
 }
 
-// -- very many pairs ------------------------------------------------------------
+// -- many short pairs -----------------------------------------------------------
 
 constexpr int PAIR_STAGES = 2;
 // one-warp CTAs that an SM holds: with short pairs what counts is how many chains of

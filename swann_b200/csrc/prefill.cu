@@ -43,12 +43,12 @@
 // are bounded; if one runs out the CTA's rows are NaN and the status word is set, once
 // copies and products in flight are done (or have had milliseconds to).
 //
-// Measured: 2049 tokens over 8193 slots, 32 heads of 128 over 8: 235 us, 1025 TFLOP/s
-// (61% of a cuBLAS bf16 product's rate).  A step of the two tiles takes about 1700
+// Measured: 2049 tokens over 8193 slots, 32 heads of 128 over 8: 239 us, 1007 TFLOP/s
+// (60% of a cuBLAS bf16 product's rate).  A step of the two tiles takes about 1700
 // cycles, 1320 of them in the tensor pipe: Q K^T with 64 keys a product is bound by
 // reading Q from shared memory (50 cycles a product of 32 cycles' work), and a
 // row's chain of wait, maximum, exponentials and hand-over is about as long.  8192
-// tokens by window 1024: 167 us, where 18 steps a job leave its ends a third of the time.
+// tokens by window 1024: 170 us, where 18 steps a job leave its ends a third of the time.
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
