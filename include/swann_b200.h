@@ -381,7 +381,9 @@ SWB_API uint64_t swb_attn_decode_workspace(const swb_kv_cache* cache, int q_head
 /* Attention of many new tokens, the last of their sequences' slots (starts as
  * in swb_rope_append, the keys written before): the token at slot i sees the
  * slots j <= i with window == 0, j > i - window or j < sinks.  What sees nothing,
- * a token of no sequence among it, gives 0 and -inf.
+ * a token of no sequence among it, gives 0 and -inf.  An infinity or NaN in the
+ * value row of a slot that is held can make NaN of tokens of the call near it
+ * which do not see it.
  * q [tokens, q_heads, head_dim]; out and lse contiguous, out on a 16-byte boundary.
  *   status   int32 word that the device can write: SWB_ERR_TIMEOUT where a bounded
  *            device-side wait gave up (the rows concerned are NaN).  NULL: a word of the

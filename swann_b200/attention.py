@@ -195,8 +195,8 @@ def decode(q, k_cache, v_cache, table, lengths, *, scale=None, window=0, sinks=0
     prior (out, lse): attention over other keys, joined as if those had been
     in the cache too.  weights float32 [seqs, kv_heads, slots]: each slot's
     share of the (joined) softmax, summed over the query heads of its key head,
-    is written there, or added with `accumulate`.  Returns out [seqs, q_heads,
-    d] and lse float32 [seqs, q_heads], 0 and -inf where nothing is seen."""
+    is written there, or added with `accumulate`.  `out` and prior rows start on
+    8-byte boundaries.  Returns out [seqs, q_heads, d] and lse float32 [seqs, q_heads], 0 and -inf where nothing is seen."""
     what = "decode"
     arg, dev = _cache_arg(what, k_cache, v_cache, table, lengths)
     d, dtype = arg.head_dim, k_cache.dtype
@@ -234,7 +234,9 @@ def prefill(q, k_cache, v_cache, table, starts, lengths, *, scale=None, window=0
     written the tokens' keys: a token at slot i sees the slots j <= i and, with
     a window, of those only j > i - window and j < sinks.  Returns out
     [tokens, q_heads, d] and lse float32 [tokens, q_heads], 0 and -inf where
-    nothing is seen and for tokens of no sequence."""
+    nothing is seen and for tokens of no sequence.  Rows that no slot holds may be
+    anything; an infinity or NaN in the value row of a slot that is held can make
+    NaN of tokens of the batch near it which do not see it."""
     what = "prefill"
     arg, dev = _cache_arg(what, k_cache, v_cache, table, lengths)
     d = arg.head_dim
