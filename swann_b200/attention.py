@@ -196,7 +196,8 @@ def decode(q, k_cache, v_cache, table, lengths, *, scale=None, window=0, sinks=0
     in the cache too.  weights float32 [seqs, kv_heads, slots]: each slot's
     share of the (joined) softmax, summed over the query heads of its key head,
     is written there, or added with `accumulate`.  `out` and prior rows start on
-    8-byte boundaries.  Returns out [seqs, q_heads, d] and lse float32 [seqs, q_heads], 0 and -inf where nothing is seen."""
+    8-byte boundaries.  Returns out [seqs, q_heads, d] and lse float32 [seqs,
+    q_heads], 0 and -inf where nothing is seen."""
     what = "decode"
     arg, dev = _cache_arg(what, k_cache, v_cache, table, lengths)
     d, dtype = arg.head_dim, k_cache.dtype

@@ -397,3 +397,25 @@ def test_pages_that_sequences_share_are_read_as_they_are():
 @pytest.mark.parametrize("window,sinks,extra", [(0, 0, "prior"), (0, 0, "weights"), (21, 3, "plain")])
 def test_decode_of_enough_one_row_pairs_for_a_warp_each(B, hq, hkv, d, page, dtype, window, sinks, extra):
     base.test_decode_of_very_many_short_sequences(B, hq, hkv, d, page, dtype, window, sinks, extra)
+
+
+@pytest.mark.parametrize("lengths,hq,hkv", [([5000], 8, 1), ([90] * 300, 8, 2), ([90] * 900, 1, 1)])
+@pytest.mark.parametrize("at", [0, 1, 2, 3, 4, 8, 12])
+def test_decode_rows_at_any_offset_are_right_or_refused(lengths, hq, hkv, at):
+    """Contiguous views that begin `at` elements into a buffer: 8 bytes are 4 of them."""
+    k, v, table, L = make_cache(lengths, hkv, 64, 16, torch.float16, 26)
+    B = len(lengths)
+    q, po = torch.randn((B, hq, 64), device=DEV).half(), torch.randn((B, hq, 64), device=DEV).half()
+    lse = torch.randn((B, hq), device=DEV)
+    want = A.decode(q, k, v, table, L, prior=(po, lse))
+
+    def moved(t):
+        return torch.empty(t.numel() + 16, dtype=t.dtype, device=DEV)[at:at + t.numel()].view(t.shape).copy_(t)
+
+    for kw in (dict(out=moved(q), prior=(po, lse)), dict(prior=(moved(po), moved(lse)))):
+        if at % 4:
+            with pytest.raises(ValueError, match="8-byte"):
+                A.decode(q, k, v, table, L, **kw)
+        else:
+            got = A.decode(q, k, v, table, L, **kw)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
